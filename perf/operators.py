@@ -1,0 +1,389 @@
+"""The layers and the optimizer step that a trainable Gaussian parameter head is made of, as they
+are measured: each operator's cases, its inputs, its plain form in elementary torch operations and
+the call of the framework's own kernels.
+
+  norm    layer norm over the last dimension, forward, or forward and backward (dx, dweight, dbias)
+  gated   h = act(x Wg^T + bg) * (x Wu^T + bu), forward, or forward and backward (all gradients)
+  adamw   one AdamW step over many tensors, its moments in 32 bits or in 8
+
+``own`` selects the side that ``run`` takes: False the plain form, True the framework's calls.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+_TYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
+_EPS = 1e-5
+_ADAMW = {"lr": 1e-3, "betas": (0.9, 0.999), "eps": 1e-8, "weight_decay": 0.01, "step": 20}
+_ALIGN = 256           # elements: every tensor of a flat parameter buffer starts at a multiple
+_M_TOP = 448.0         # largest value of an e4m3 code
+_R_TOP = 507904.0      # largest value of a root code: 31 * 2^14
+_TINY = 2.0 ** -100    # blocks whose largest magnitude is below this hold zeros
+
+
+def listed():
+    return [
+        # the Gaussian parameter head's features at its selection cap: 16000 voxels of 8 channels
+        {"name": "norm_head", "op": "norm", "rows": 16000, "dim": 8, "pad": 0, "type": "float32", "train": True},
+        # one row through a wide layer: latency
+        {"name": "norm_token", "op": "norm", "rows": 1, "dim": 4096, "pad": 0, "type": "bfloat16", "train": False},
+        # odd sizes, rows of a wider buffer
+        {"name": "norm_odd", "op": "norm", "rows": 5003, "dim": 1031, "pad": 5, "type": "float16", "train": True},
+        # a long training batch
+        {"name": "norm_large", "op": "norm", "rows": 32768, "dim": 4096, "pad": 0, "type": "bfloat16", "train": True},
+        # the parameter head's hidden layer: 8 channels to 128, in the framework's fp32
+        {"name": "gated_head", "op": "gated", "rows": 16000, "dim": 8, "hidden": 128, "type": "float32", "act": "silu",
+         "bias": True, "train": True},
+        # a wider fp32 head over the same rows
+        {"name": "gated_wide_f32", "op": "gated", "rows": 16000, "dim": 256, "hidden": 512, "type": "float32", "act": "silu",
+         "bias": True, "train": True},
+        # one row: the weights are read once and nothing is reused
+        {"name": "gated_token", "op": "gated", "rows": 1, "dim": 4096, "hidden": 11264, "type": "bfloat16", "act": "silu",
+         "bias": False, "train": False},
+        # odd sizes
+        {"name": "gated_odd", "op": "gated", "rows": 777, "dim": 509, "hidden": 1363, "type": "float16", "act": "gelu",
+         "bias": True, "train": True},
+        # a long training batch through a wide block
+        {"name": "gated_large", "op": "gated", "rows": 16384, "dim": 2048, "hidden": 5632, "type": "bfloat16", "act": "silu",
+         "bias": False, "train": True},
+        # the parameter head's own tensors: a few small ones, latency
+        {"name": "adamw_head", "op": "adamw", "rows": 0, "layers": 1, "dim": 8, "hidden": 128, "type": "float32", "bits": 32},
+        # 2 M Gaussians' rows and a small head, moments in 8 bits
+        {"name": "adamw_scene_8bit", "op": "adamw", "rows": 2000000, "layers": 1, "dim": 64, "hidden": 256,
+         "type": "float32", "bits": 8},
+        # many layers' weights in bf16, moments in 32 bits
+        {"name": "adamw_layers", "op": "adamw", "rows": 0, "layers": 12, "dim": 1024, "hidden": 4096, "type": "bfloat16",
+         "bits": 32},
+    ]
+
+
+def _spread(rng, low, high):
+    """A whole number between low and high, spread over its logarithm; every other one odd."""
+    n = int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+    return max(low, min(high, n | 1 if rng.random() < 0.5 else n))
+
+
+def draw(rng):
+    op = rng.choice(["norm", "gated", "adamw"])
+    kind = rng.choice(["float32", "bfloat16", "float16"])
+    if op == "norm":
+        dim = _spread(rng, 4, 8192)     # below 4 the gradient is what rounding leaves of a difference
+        rows = _spread(rng, 1, min(1 << 18, (1 << 27) // dim // (2 if kind == "float32" else 1)))
+        return {"op": op, "rows": rows, "dim": dim, "pad": rng.choice([0, 0, 8, 3]), "type": kind,
+                "train": rng.random() < 0.7}
+    if op == "gated":
+        dim, hidden = _spread(rng, 1, 4096), _spread(rng, 8, 12288)
+        # at fp32 a pass costs several times what it costs in 16 bits
+        most = 16384 * 2048 * 5632 // (8 if kind == "float32" else 1)
+        rows = _spread(rng, 1, max(1, min(16384, most // (dim * hidden))))
+        train = rng.random() < 0.7
+        # relu's slope jumps at 0, so its gradient there turns on the last bit: forward only
+        return {"op": op, "rows": rows, "dim": dim, "hidden": hidden, "type": kind,
+                "act": rng.choice(["silu", "gelu", "sigmoid"] + ([] if train else ["relu"])), "bias": rng.random() < 0.5,
+                "train": train}
+    return {"op": op, "rows": rng.choice([0, _spread(rng, 100, 2000000)]), "layers": rng.randrange(1, 9),
+            "dim": _spread(rng, 8, 1024), "hidden": _spread(rng, 16, 4096), "type": rng.choice(["float32", "bfloat16"]),
+            "bits": rng.choice([32, 8])}
+
+
+def _shapes(case):
+    """The tensors of an AdamW case: the Gaussians' rows, and each layer's norm, gated and output weights."""
+    d, h = case["dim"], case["hidden"]
+    layer = [(d,), (d,), (h, d), (h, d), (h,), (h,), (14, h), (14,)]
+    return ([(case["rows"], 14)] if case["rows"] else []) + layer * case["layers"]
+
+
+def _at(shapes):
+    """(starts, length) of the tensors in a flat buffer."""
+    starts, n = [], 0
+    for s in shapes:
+        starts.append(n)
+        n += -(-math.prod(s) // _ALIGN) * _ALIGN
+    return starts, n
+
+
+def _views(flat, shapes, starts):
+    return [flat[a:a + math.prod(s)].view(s) for s, a in zip(shapes, starts)]
+
+
+def _generator(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def prepare(case, seed):
+    g = _generator(seed)
+    t = _TYPES[case["type"]]
+
+    def normal(*shape, scale=1.0):
+        return torch.randn(*shape, device="cuda", generator=g).mul_(scale).to(t)
+
+    if case["op"] == "norm":
+        r, d = case["rows"], case["dim"]
+        x = (normal(r, d + case["pad"]) + 0.5)[:, :d].detach().requires_grad_(case["train"])
+        w = (1 + normal(d, scale=0.2)).requires_grad_(case["train"])
+        b = normal(d, scale=0.2).requires_grad_(case["train"])
+        return {"case": case, "x": x, "w": w, "b": b, "dy": normal(r, d) if case["train"] else None}
+    if case["op"] == "gated":
+        r, d, h = case["rows"], case["dim"], case["hidden"]
+        s = {"case": case, "x": normal(r, d), "wg": normal(h, d, scale=d ** -0.5), "wu": normal(h, d, scale=d ** -0.5),
+             "bg": normal(h, scale=0.2) if case["bias"] else None, "bu": normal(h, scale=0.2) if case["bias"] else None}
+        for v in (s["x"], s["wg"], s["wu"], s["bg"], s["bu"]):
+            if v is not None:
+                v.requires_grad_(case["train"])
+        s["dh"] = normal(r, h) if case["train"] else None
+        return s
+    shapes = _shapes(case)
+    starts, n = _at(shapes)
+    inside = torch.zeros(n, device="cuda", dtype=torch.bool)
+    for v in _views(inside, shapes, starts):
+        v.fill_(True)
+    # gradients of very different sizes side by side, and rows that no pixel saw
+    size = torch.randn(n, device="cuda", generator=g).mul_(1.5).sub_(6).exp_().mul_(inside)
+    size *= torch.rand(n, device="cuda", generator=g) > 0.05
+    p = torch.randn(n, device="cuda", generator=g).mul_(0.1).mul_(inside).to(t)
+    grad = torch.randn(n, device="cuda", generator=g).mul_(size).to(t)
+    m = torch.randn(n, device="cuda", generator=g).mul_(size).mul_(0.3)
+    v = torch.rand(n, device="cuda", generator=g).add_(0.5).mul_(size).mul_(size).mul_(0.02)
+    del size, inside
+    s = {"case": case, "shapes": shapes, "starts": starts, "p": p, "grad": grad}
+    if case["bits"] == 32:
+        s |= {"m": m, "v": v}
+    else:
+        s["m"], s["mu"] = _encode_mean(m)
+        s["v"], s["vu"] = _encode_root(v.sqrt_())
+    s["params"], s["grads"] = _views(p, shapes, starts), _views(grad, shapes, starts)
+    s["ms"], s["vs"] = _views(s["m"], shapes, starts), _views(s["v"], shapes, starts)
+    if case["bits"] == 8:
+        blocks = [(-(-math.prod(x) // _ALIGN),) for x in shapes]
+        s["mus"] = _views(s["mu"], blocks, [a // _ALIGN for a in starts])
+        s["vus"] = _views(s["vu"], blocks, [a // _ALIGN for a in starts])
+    return s
+
+
+def _unit(blocks, top):
+    """Each block's unit: its largest magnitude over the largest code's value."""
+    most = blocks.abs().amax(1)
+    return torch.where(most < _TINY, torch.zeros_like(most), most * (1.0 / top))
+
+
+def _inverse(unit):
+    return torch.where(unit == 0, torch.zeros_like(unit), torch.ones_like(unit) / unit)
+
+
+def _encode_mean(m):
+    b = m.view(-1, _ALIGN)
+    unit = _unit(b, _M_TOP)
+    q = (b * _inverse(unit)[:, None]).clamp(-_M_TOP, _M_TOP)
+    return q.float().to(torch.float8_e4m3fn).view(-1), unit
+
+
+def _encode_root(r):
+    """Roots as 8-bit codes: 16 whole numbers from 0, then 15 doublings of 16 steps each."""
+    b = r.view(-1, _ALIGN)
+    unit = _unit(b, _R_TOP)
+    q = (b * _inverse(unit)[:, None]).clamp(max=_R_TOP)
+    up = torch.frexp(q.clamp_min(16.0)).exponent - 5
+    q = torch.ldexp(torch.round(torch.ldexp(q, -up)), up)         # ties to even
+    up = torch.frexp(q.clamp_min(16.0)).exponent - 5              # a carry opens the next doubling
+    code = up * 16 + torch.ldexp(q, -up).to(torch.int32)
+    code = torch.where((b > 0) & (unit > 0)[:, None], code.clamp_min(1), code)   # a root that is not zero stays so
+    return code.to(torch.uint8).view(-1), unit
+
+
+def _decode_root(code, unit):
+    c = code.view(-1, _ALIGN).to(torch.int32)
+    up = (c >> 4).clamp_min(1) - 1
+    value = ((c - up * 16) << up).to(unit.dtype)
+    return (value * unit[:, None]).view(-1)
+
+
+def _activation(kind, g):
+    """act(g) and its derivative."""
+    if kind == "relu":
+        return g.clamp_min(0), (g > 0).to(g.dtype)
+    if kind == "gelu":
+        half = 0.5 * torch.erf(g * math.sqrt(0.5)) + 0.5
+        return g * half, half + g * torch.exp(-0.5 * g * g) * (1 / math.sqrt(2 * math.pi))
+    s = 1 / (1 + torch.exp(-g))
+    return (s, s * (1 - s)) if kind == "sigmoid" else (g * s, s * (1 + g * (1 - s)))
+
+
+def _norm(x, w, b, dy, t):
+    """In the type t; rounded to the inputs' own at the end."""
+    xf, wf = x.to(t), w.to(t)
+    xc = xf - xf.mean(1, keepdim=True)
+    rstd = torch.rsqrt((xc * xc).mean(1, keepdim=True) + _EPS)
+    xhat = xc * rstd
+    y = xhat * wf + b.to(t)
+    if dy is None:
+        return [y]
+    dyf = dy.to(t)
+    wdy = dyf * wf
+    dx = (wdy - wdy.mean(1, keepdim=True) - xhat * (wdy * xhat).mean(1, keepdim=True)) * rstd
+    return [y, dx, (dyf * xhat).sum(0), dyf.sum(0)]
+
+
+def _gated(s, t):
+    x, wg, wu = s["x"].to(t), s["wg"].to(t), s["wu"].to(t)
+    g, u = x @ wg.t(), x @ wu.t()
+    if s["bg"] is not None:
+        g, u = g + s["bg"].to(t), u + s["bu"].to(t)
+    a, da = _activation(s["case"]["act"], g)
+    h = a * u
+    if s["dh"] is None:
+        return [h]
+    dh = s["dh"].to(t)
+    dg, du = dh * u * da, dh * a
+    out = [h, dg @ wg + du @ wu, dg.t() @ x, du.t() @ x]
+    return out + ([dg.sum(0), du.sum(0)] if s["bg"] is not None else [])
+
+
+def _adamw(s, t):
+    """The step on the flat buffers in the type t: new parameters, first moment and second moment (or its root)."""
+    a = _ADAMW
+    b1, b2 = a["betas"]
+    p, g = s["p"].to(t), s["grad"].to(t)
+    if s["case"]["bits"] == 32:
+        m, v = s["m"].to(t), s["v"].to(t)
+    else:
+        m = (s["m"].to(t).view(-1, _ALIGN) * s["mu"].to(t)[:, None]).view(-1)
+        r = _decode_root(s["v"], s["vu"].to(t))
+        v = r * r
+    m = m * b1 + g * (1 - b1)
+    v = v * b2 + (g * g) * (1 - b2)
+    root = torch.sqrt(v)
+    denom = root * (1 / math.sqrt(1 - b2 ** a["step"])) + a["eps"]
+    p = p * (1 - a["lr"] * a["weight_decay"]) - m * (a["lr"] / (1 - b1 ** a["step"])) / denom
+    return p, m, v if s["case"]["bits"] == 32 else root
+
+
+def _own():
+    package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pose-splatter_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    from gsr import layers, optim
+    return layers, optim
+
+
+def run(state):
+    s, case = state, state["case"]
+    if own:
+        layers, optim = _own()
+        if case["op"] == "adamw":
+            more = {} if case["bits"] == 32 else {"exp_avg_units": s["mus"], "exp_avg_root_units": s["vus"]}
+            optim.adamw_step(s["params"], s["grads"], s["ms"], s["vs"], **more, **_ADAMW)
+            if case["bits"] == 32:
+                return [s["p"], s["m"], s["v"]]
+            return [s["p"], s["m"], s["mu"], optim.decode_root(s["v"], s["vu"]), s["vu"]]
+        with torch.set_grad_enabled(case["train"]):
+            if case["op"] == "norm":
+                y = layers.layer_norm(s["x"], s["w"], s["b"], eps=_EPS)
+                leaves, dy = [s["x"], s["w"], s["b"]], s["dy"]
+            else:
+                y = layers.gated_linear(s["x"], s["wg"], s["wu"], s["bg"], s["bu"], activation=case["act"])
+                leaves, dy = [v for v in (s["x"], s["wg"], s["wu"], s["bg"], s["bu"]) if v is not None], s["dh"]
+            return [y.detach(), *torch.autograd.grad(y, leaves, dy)] if case["train"] else [y]
+    with torch.no_grad():
+        t = _TYPES[case["type"]]
+        if case["op"] == "norm":
+            return [v.to(t) for v in _norm(s["x"], s["w"], s["b"], s["dy"], torch.float32)]
+        if case["op"] == "gated":
+            return [v.to(t) for v in _gated(s, torch.float32)]
+        p, m, v = _adamw(s, torch.float32)
+        s["p"].copy_(p)
+        if case["bits"] == 32:
+            s["m"].copy_(m)
+            s["v"].copy_(v)
+            return [s["p"], s["m"], s["v"]]
+        for name, unit, (code, scale) in (("m", "mu", _encode_mean(m)), ("v", "vu", _encode_root(v))):
+            s[name].copy_(code)
+            s[unit].copy_(scale)
+        return [s["p"], s["m"], s["mu"], _decode_root(s["v"], s["vu"]), s["vu"]]
+
+
+def work(case):
+    size = 4 if case["type"] == "float32" else 2
+    if case["op"] == "norm":
+        n, d = case["rows"] * case["dim"], case["dim"]
+        if not case["train"]:
+            return {"bytes": size * (2 * n + 2 * d), "flops": 8 * n}
+        return {"bytes": size * (4 * n + 4 * d), "flops": 20 * n}       # x, dy in; y, dx out
+    if case["op"] == "gated":
+        r, d, h = case["rows"], case["dim"], case["hidden"]
+        weights = 2 * h * d + (2 * h if case["bias"] else 0)
+        if not case["train"]:
+            return {"bytes": size * (r * d + r * h + weights), "flops": 4 * r * d * h}
+        return {"bytes": size * (2 * r * d + 2 * r * h + 2 * weights), "flops": 12 * r * d * h}
+    n = sum(math.prod(x) for x in _shapes(case))
+    if case["bits"] == 32:
+        return {"bytes": n * (3 * size + 16), "flops": 14 * n}          # p, m, v in and out, g in
+    return {"bytes": n * (3 * size + 4 + 4 + 4 / 64), "flops": 30 * n}  # 8-bit moments; their roots decoded at the end
+
+
+def exact(case, seed):
+    """The operators in 64 bits, written from their definitions."""
+    s = prepare(case, seed)
+    with torch.no_grad():
+        if case["op"] == "norm":
+            x, w = s["x"].double(), s["w"].double()
+            mean, var = x.mean(1, keepdim=True), x.var(1, unbiased=False, keepdim=True)
+            sigma = (var + _EPS).sqrt()
+            z = (x - mean) / sigma
+            out = [z * w + s["b"].double()]
+            if case["train"]:
+                dy = s["dy"].double()
+                dz = dy * w
+                n = case["dim"]
+                dx = (n * dz - dz.sum(1, keepdim=True) - z * (dz * z).sum(1, keepdim=True)) / (n * sigma)
+                out += [dx, (dy * z).sum(0), dy.sum(0)]
+            return out
+        if case["op"] == "gated":
+            x, wg, wu = (s[k].double() for k in ("x", "wg", "wu"))
+            g, u = torch.mm(x, wg.t()), torch.mm(x, wu.t())
+            if case["bias"]:
+                g += s["bg"].double()
+                u += s["bu"].double()
+            kind = case["act"]
+            if kind == "relu":
+                a, slope = torch.where(g > 0, g, 0.0), torch.where(g > 0, 1.0, 0.0).double()
+            elif kind == "gelu":
+                area = 0.5 * torch.special.erfc(-g / math.sqrt(2.0))
+                a, slope = g * area, area + g * torch.exp(-g.square() / 2) / math.sqrt(2 * math.pi)
+            else:
+                s1 = torch.sigmoid(g)
+                a, slope = (s1, s1 * torch.sigmoid(-g)) if kind == "sigmoid" else (g * s1, s1 + g * s1 * torch.sigmoid(-g))
+            out = [a * u]
+            if case["train"]:
+                dh = s["dh"].double()
+                du = dh * a
+                del a
+                dg = dh * u * slope
+                del u, g, slope, dh
+                out += [torch.mm(dg, wg).addmm_(du, wu), torch.mm(dg.t(), x), torch.mm(du.t(), x)]
+                out += [dg.sum(0), du.sum(0)] if case["bias"] else []
+            return out
+        c = _ADAMW
+        p, g = s["p"].double(), s["grad"].double()
+        if case["bits"] == 32:
+            m, v = s["m"].double(), s["v"].double()
+        else:
+            m = s["m"].double() * s["mu"].double().repeat_interleave(_ALIGN)
+            levels = [float(k) for k in range(16)] + [float((16 + k) << e) for e in range(15) for k in range(16)]
+            table = torch.tensor(levels, device="cuda", dtype=torch.float64)
+            v = (table[s["v"].int()] * s["vu"].double().repeat_interleave(_ALIGN)).square()
+        b1, b2 = c["betas"]
+        m += (1 - b1) * (g - m)
+        v += (1 - b2) * (g.square() - v)
+        m_hat, v_hat = m / (1 - b1 ** c["step"]), v / (1 - b2 ** c["step"])
+        p -= c["lr"] * c["weight_decay"] * p + c["lr"] * m_hat / (v_hat.sqrt() + c["eps"])
+        if case["bits"] == 32:
+            return [p, m, v]
+        mu = m.view(-1, _ALIGN).abs().amax(1) / _M_TOP
+        vu = v.view(-1, _ALIGN).amax(1).sqrt() / _R_TOP
+        safe = torch.where(mu > 0, mu, 1.0).repeat_interleave(_ALIGN)
+        # the root's code next to a border turns on the last bit of 32: no value in 64
+        return [p, (m / safe).float().to(torch.float8_e4m3fn).double(), mu, None, vu]
