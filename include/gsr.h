@@ -191,7 +191,7 @@ int gsr_version(void);
 /* Revision 14 (round 6): gsr3d_raster_fwd, gsr3d_raster_fwd_lazy, gsr3d_raster_bwd and
  * gsr3d_raster_bwd_loss take box_masks (before the stream): the forward's per-chunk box
  * survivor masks, stats->masks bit 2. */
-#define GSR_ABI_VERSION 14
+#define GSR_ABI_VERSION 15
 int gsr_abi_version(void);
 const char* gsr_last_error(void);
 
@@ -675,6 +675,59 @@ int gsr_carve_volume(const float* grid, int64_t n_voxels, const float* center, d
 size_t gsr_carve_medoids_workspace(int C);
 int gsr_carve_medoids(const float* masks, int C, int height, int width, void* ws, size_t ws_bytes, int32_t* medoid,
                       void* stream);
+
+/* ---- Layers and optimizer of a trainable parameter head --------------------------------
+ * Element types of the tensors below: GSR_F32, GSR_BF16 or GSR_F16; arithmetic, sums and
+ * statistics are fp32 whatever the type. */
+#define GSR_F32 0
+#define GSR_BF16 1
+#define GSR_F16 2
+
+/* Layer norm of `rows` rows of `dim` elements (row stride `stride` elements, unit stride inside
+ * a row; any alignment): y = (x - mean) / sqrt(var + eps) * w + b, var the biased variance.
+ * w / b [dim] of type wtype, or NULL (1 / 0).  y [rows, dim] contiguous, of x's type.
+ * stats: float [rows][2] = mean, 1/sqrt(var + eps) for the backward, or NULL.
+ * bwd: dx [rows, dim] contiguous (or NULL), dw / db [dim] of type wtype (either or both NULL);
+ * dy has x's type and the row stride dy_stride.  workspace: device, gsr_layer_norm_workspace
+ * bytes (only when dw or db is asked for).  Fixed-order sums: the same bits every run. */
+int gsr_layer_norm_fwd(const void* x, int64_t rows, int64_t dim, int64_t stride, int32_t xtype, const void* w,
+                       const void* b, int32_t wtype, float eps, void* y, float* stats, void* stream);
+size_t gsr_layer_norm_workspace(int64_t rows, int64_t dim, int32_t xtype);
+int gsr_layer_norm_bwd(const void* x, const void* dy, int64_t rows, int64_t dim, int64_t stride, int64_t dy_stride,
+                       int32_t xtype, const void* w, int32_t wtype, const float* stats, void* dx, void* dw, void* db,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* One AdamW step over `count` tensors (a HOST list) in place:
+ *   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+ *   p = p (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+ * bits 32: m, v are fp32 [n].  bits 8: m holds e4m3 codes and v codes of sqrt(v), n bytes each,
+ * in blocks of GSR_ADAMW_BLOCK elements with one fp32 unit a block (m_unit, v_unit
+ * [ceil(n / GSR_ADAMW_BLOCK)]); zeroed codes and units are zero moments.  A code c of sqrt(v)
+ * stands for c units below 16, else for (16 + c % 16) * 2^(c / 16 - 1).  A gradient that is not
+ * finite makes its element's moments NaN or infinite, in 8 bits its whole block's.
+ * A tensor's step count (>= 1) and lr are read from the device where its `step` / lr_dev is not
+ * NULL (a captured step), else taken from the host values.  The tensors must not overlap.  gsr_adamw_decode_root
+ * writes the n roots sqrt(v) that codes stand for. */
+#define GSR_ADAMW_BLOCK 256
+typedef struct {
+  void* p;
+  const void* g;
+  void* m;
+  void* v;
+  float* m_unit;
+  float* v_unit;
+  const int64_t* step;
+  int64_t n;
+} gsr_adamw_tensor;
+typedef struct {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;
+  const float* lr_dev;
+  int32_t bits, reserved;
+} gsr_adamw_args;
+int gsr_adamw_step(const gsr_adamw_tensor* tensors, int32_t count, int32_t ptype, int32_t gtype,
+                   const gsr_adamw_args* args, void* stream);
+int gsr_adamw_decode_root(const uint8_t* codes, const float* units, int64_t n, float* out, void* stream);
 
 #ifdef __cplusplus
 }

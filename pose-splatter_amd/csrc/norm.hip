@@ -1,0 +1,468 @@
+// Layer norm over rows, forward and backward.
+//
+//   y = xhat w + b,  xhat = (x - mean) rstd,  rstd = 1 / sqrt(var + eps)
+//   dx = rstd (w dy - mean(w dy) - xhat mean(w dy xhat)),  dw = sum_rows dy xhat,  db = sum_rows dy
+//
+// Both passes are bound by memory: a row is read once and stays in registers while its mean,
+// then its variance about that mean (two sums, so no cancellation of E[x^2] - mean^2) are
+// reduced.  LANES lanes share a row -- part of a wave for short rows, a wave, or a whole
+// workgroup -- each holding NV vectors of V elements.  The backward's workgroups walk rows with
+// the grid's stride and keep dw and db of their columns in registers; each writes one row of
+// partial sums, which a second kernel adds in a fixed order: no atomics, the same bits every run.
+// Sums, statistics and partials are fp32; only y, dx, dw and db are rounded to their types.
+#include "types.h"
+
+namespace gsr {
+
+constexpr int kNormParts = 512;   // partial rows of dw/db at most: two workgroups per CU
+
+template <typename T>
+struct NormVec {
+  static constexpr int V = sizeof(T) == 4 ? 4 : 8;   // 16 bytes
+};
+
+// Sum over the LANES lanes of a row, in all of them.  Workgroup rows (LANES > 64) go through
+// `lds`, of which a caller alternates two halves so that one barrier a sum is enough.
+template <int LANES, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float* lds) {
+  if constexpr (LANES < 64) {
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], d);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+    if constexpr (LANES > 64) {
+      constexpr int W = LANES / 64;
+      if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) lds[i * W + threadIdx.x / 64] = v[i];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) s += lds[i * W + w];
+        v[i] = s;
+      }
+    }
+  }
+}
+
+template <typename T, int LANES, int NV>
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_norm_fwd(const T* x, int64_t rows, int64_t dim, int64_t stride,
+                                                                        const void* w, const void* b, int wtype, float eps,
+                                                                        T* y, float2* stats) {
+  constexpr int V = NormVec<T>::V, THREADS = LANES > 256 ? LANES : 256, RPB = THREADS / LANES;
+  __shared__ float lds[LANES > 64 ? 2 * (LANES / 64) : 1];
+  const int lane = threadIdx.x % LANES;
+  for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES; row < rows; row += (int64_t)gridDim.x * RPB) {
+  const T* xr = x + row * stride;
+  float v[NV][V];
+  float s[1] = {0.f};
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int64_t c = (int64_t)(k * LANES + lane) * V;
+    load_upto(xr + c, dim - c, v[k]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[0] += v[k][i];
+  }
+  row_sum<LANES>(s, lds);
+  const float mean = s[0] / (float)dim;
+  s[0] = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int64_t c = (int64_t)(k * LANES + lane) * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      v[k][i] -= mean;
+      s[0] += c + i < dim ? v[k][i] * v[k][i] : 0.f;
+    }
+  }
+  row_sum<LANES>(s, lds + (LANES > 64 ? LANES / 64 : 0));
+  const float rstd = 1.f / sqrtf(s[0] / (float)dim + eps);
+  if (stats && lane == 0) stats[row] = make_float2(mean, rstd);
+  T* yr = y + row * dim;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int64_t c = (int64_t)(k * LANES + lane) * V;
+    if (c < dim) {
+      float wv[V], bv[V];
+      load_param(w, wtype, c, dim - c, wv, 1.f);
+      load_param(b, wtype, c, dim - c, bv, 0.f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[k][i] = v[k][i] * rstd * wv[i] + bv[i];
+      store_upto(yr + c, dim - c, v[k]);
+    }
+  }
+  }
+}
+
+// Rows of any length: the row is read three times (from cache after the first).
+template <typename T>
+__global__ __launch_bounds__(1024) void k_norm_fwd_long(const T* x, int64_t rows, int64_t dim, int64_t stride, const void* w,
+                                                        const void* b, int wtype, float eps, T* y, float2* stats) {
+  constexpr int V = NormVec<T>::V;
+  __shared__ float lds[2 * 16];
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+  const T* xr = x + row * stride;
+  float s[1] = {0.f};
+  for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
+    float v[V];
+    load_upto(xr + c, dim - c, v);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[0] += v[i];
+  }
+  row_sum<1024>(s, lds);
+  const float mean = s[0] / (float)dim;
+  s[0] = 0.f;
+  for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
+    float v[V];
+    load_upto(xr + c, dim - c, v, mean);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[0] += (v[i] - mean) * (v[i] - mean);
+  }
+  row_sum<1024>(s, lds + 16);
+  const float rstd = 1.f / sqrtf(s[0] / (float)dim + eps);
+  if (stats && threadIdx.x == 0) stats[row] = make_float2(mean, rstd);
+  for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
+    float v[V], wv[V], bv[V];
+    load_upto(xr + c, dim - c, v);
+    load_param(w, wtype, c, dim - c, wv, 1.f);
+    load_param(b, wtype, c, dim - c, bv, 0.f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (v[i] - mean) * rstd * wv[i] + bv[i];
+    store_upto(y + row * dim + c, dim - c, v);
+  }
+  }
+}
+
+// parts: [gridDim.x][2][dim] partial sums of dw and db (NULL: neither is wanted).
+template <typename T, int LANES, int NV>
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_norm_bwd(const T* x, const T* dy, int64_t rows, int64_t dim,
+                                                                        int64_t stride, int64_t dy_stride, const void* w,
+                                                                        int wtype, const float2* stats, T* dx, float* parts) {
+  constexpr int V = NormVec<T>::V, THREADS = LANES > 256 ? LANES : 256, RPB = THREADS / LANES;
+  constexpr int W = LANES / 64;
+  __shared__ float lds[LANES > 64 ? 4 * W : 1];
+  const int lane = threadIdx.x % LANES;
+  const float inv = 1.f / (float)dim;
+  float wv[NV][V], aw[NV][V] = {}, ab[NV][V] = {};
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int64_t c = (int64_t)(k * LANES + lane) * V;
+    load_param(w, wtype, c, dim - c, wv[k], 1.f);
+  }
+  int half = 0;
+  for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES; row < rows; row += (int64_t)gridDim.x * RPB) {
+    const float2 st = stats[row];
+    float xv[NV][V], g[NV][V], s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int64_t c = (int64_t)(k * LANES + lane) * V;
+      load_upto(x + row * stride + c, dim - c, xv[k], st.x);
+      load_upto(dy + row * dy_stride + c, dim - c, g[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float z = (xv[k][i] - st.x) * st.y;
+        xv[k][i] = z;
+        aw[k][i] += g[k][i] * z;
+        ab[k][i] += g[k][i];
+        g[k][i] *= wv[k][i];
+        s[0] += g[k][i];
+        s[1] += g[k][i] * z;
+      }
+    row_sum<LANES>(s, lds + half * 2 * W);
+    half ^= 1;
+    if (dx) {
+      const float m0 = s[0] * inv, m1 = s[1] * inv;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int64_t c = (int64_t)(k * LANES + lane) * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[k][i] = (g[k][i] - m0 - xv[k][i] * m1) * st.y;
+        if (c < dim) store_upto(dx + row * dim + c, dim - c, g[k]);
+      }
+    }
+  }
+  if (!parts) return;
+  // the workgroup's rows: lanes of a wave that hold the same columns, then the waves through LDS
+  float* out = parts + (int64_t)blockIdx.x * 2 * dim;
+  if constexpr (LANES < 64) {
+#pragma unroll
+    for (int d = LANES; d < 64; d <<= 1)
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          aw[k][i] += __shfl_xor(aw[k][i], d);
+          ab[k][i] += __shfl_xor(ab[k][i], d);
+        }
+  }
+  if constexpr (LANES <= 64) {
+    constexpr int COLS = LANES * V;
+    __shared__ float sum[4][2][COLS];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (threadIdx.x % 64 < LANES)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          sum[threadIdx.x / 64][0][lane * V + i] = aw[k][i];
+          sum[threadIdx.x / 64][1][lane * V + i] = ab[k][i];
+        }
+      __syncthreads();
+      for (int j = threadIdx.x; j < 2 * COLS; j += THREADS) {
+        const int which = j / COLS, c = j % COLS;
+        const int64_t col = (int64_t)k * COLS + c;
+        if (col < dim)
+          out[which * dim + col] = (sum[0][which][c] + sum[1][which][c]) + (sum[2][which][c] + sum[3][which][c]);
+      }
+      __syncthreads();
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int64_t c = (int64_t)(k * LANES + lane) * V;
+      if (c < dim) {
+        store_upto(out + c, dim - c, aw[k]);
+        store_upto(out + dim + c, dim - c, ab[k]);
+      }
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void k_norm_bwd_long(const T* x, const T* dy, int64_t rows, int64_t dim, int64_t stride,
+                                                        int64_t dy_stride, const void* w, int wtype, const float2* stats,
+                                                        T* dx) {
+  constexpr int V = NormVec<T>::V;
+  __shared__ float lds[2][2 * 16];
+  int half = 0;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, half ^= 1) {
+  const float2 st = stats[row];
+  const T *xr = x + row * stride, *gr = dy + row * dy_stride;
+  float s[2] = {0.f, 0.f};
+  for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
+    float v[V], g[V], wv[V];
+    load_upto(xr + c, dim - c, v, st.x);
+    load_upto(gr + c, dim - c, g);
+    load_param(w, wtype, c, dim - c, wv, 1.f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      s[0] += g[i] * wv[i];
+      s[1] += g[i] * wv[i] * ((v[i] - st.x) * st.y);
+    }
+  }
+  row_sum<1024>(s, lds[half]);
+  const float m0 = s[0] / (float)dim, m1 = s[1] / (float)dim;
+  for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
+    float v[V], g[V], wv[V];
+    load_upto(xr + c, dim - c, v, st.x);
+    load_upto(gr + c, dim - c, g);
+    load_param(w, wtype, c, dim - c, wv, 1.f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) g[i] = (g[i] * wv[i] - m0 - (v[i] - st.x) * st.y * m1) * st.y;
+    store_upto(dx + row * dim + c, dim - c, g);
+  }
+  }
+}
+
+// Partial dw/db of long rows: a thread per column, blockIdx.y's share of the rows.
+template <typename T>
+__global__ __launch_bounds__(256) void k_norm_cols(const T* x, const T* dy, int64_t rows, int64_t dim, int64_t stride,
+                                                   int64_t dy_stride, const float2* stats, float* parts) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= dim) return;
+  float aw = 0.f, ab = 0.f;
+  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+    const float2 st = stats[row];
+    const float g = to_f(dy[row * dy_stride + c]);
+    aw += g * ((to_f(x[row * stride + c]) - st.x) * st.y);
+    ab += g;
+  }
+  parts[(int64_t)blockIdx.y * 2 * dim + c] = aw;
+  parts[(int64_t)blockIdx.y * 2 * dim + dim + c] = ab;
+}
+
+// dw, db = the sum of n partial rows: 16 groups of lanes a column, each a fixed share of the
+// rows, then the groups in order.
+__global__ __launch_bounds__(1024) void k_norm_join(const float* parts, int n, int64_t dim, void* dw, void* db, int wtype) {
+  __shared__ float sum[16][65];
+  const int col = threadIdx.x % 64, grp = threadIdx.x / 64;
+  const int64_t c = (int64_t)blockIdx.x * 64 + col;
+  float s = 0.f;
+  if (c < 2 * dim)
+    for (int r = grp; r < n; r += 16) s += parts[(int64_t)r * 2 * dim + c];
+  sum[grp][col] = s;
+  __syncthreads();
+  if (grp == 0 && c < 2 * dim) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += sum[k][col];
+    if (c < dim) {
+      if (dw) store_param(dw, wtype, c, s);
+    } else if (db) {
+      store_param(db, wtype, c - dim, s);
+    }
+  }
+}
+
+// Vectors a row -> the layout that holds it: lanes a row (a power of two up to a wave, then 256
+// and 1024) and vectors a lane; 0 lanes: longer than registers hold.
+static void norm_layout(int64_t vecs, int* lanes, int* nv) {
+  int l = 1;
+  while (l < 64 && l < vecs) l <<= 1;
+  *lanes = l;
+  *nv = 1;
+  if (vecs <= 64) return;
+  if (vecs <= 256) {
+    *nv = vecs <= 128 ? 2 : 4;
+  } else if (vecs <= 1024) {
+    *lanes = 256;
+    *nv = vecs <= 512 ? 2 : 4;
+  } else if (vecs <= 4096) {
+    *lanes = 1024;
+    *nv = vecs <= 2048 ? 2 : 4;
+  } else {
+    *lanes = 0;
+  }
+}
+
+// Workgroups of a pass: one a row (or group of rows) up to 2^20, which then walk on by the grid's
+// stride (a launch may hold 2^32 threads).
+static unsigned norm_grid(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)); }
+
+#define GSR_NORM_DISPATCH(CALL)                 \
+  switch (lanes * 8 + nv) {                     \
+    case 1 * 8 + 1: CALL(1, 1); break;          \
+    case 2 * 8 + 1: CALL(2, 1); break;          \
+    case 4 * 8 + 1: CALL(4, 1); break;          \
+    case 8 * 8 + 1: CALL(8, 1); break;          \
+    case 16 * 8 + 1: CALL(16, 1); break;        \
+    case 32 * 8 + 1: CALL(32, 1); break;        \
+    case 64 * 8 + 1: CALL(64, 1); break;        \
+    case 64 * 8 + 2: CALL(64, 2); break;        \
+    case 64 * 8 + 4: CALL(64, 4); break;        \
+    case 256 * 8 + 2: CALL(256, 2); break;      \
+    case 256 * 8 + 4: CALL(256, 4); break;      \
+    case 1024 * 8 + 2: CALL(1024, 2); break;    \
+    case 1024 * 8 + 4: CALL(1024, 4); break;    \
+  }
+
+// Partial rows of dw/db that a backward writes.
+static int norm_parts(int64_t rows, int64_t dim, int xtype) {
+  int lanes, nv;
+  norm_layout(ceil_div64(dim, xtype == GSR_F32 ? 4 : 8), &lanes, &nv);
+  const int rpb = lanes == 0 || lanes > 256 ? 1 : 256 / lanes;
+  const int64_t blocks = ceil_div64(rows, rpb);
+  const int most = lanes == 0 ? 64 : kNormParts;
+  return (int)(blocks < most ? blocks : most);
+}
+
+template <typename T>
+static void norm_fwd(const void* x, int64_t rows, int64_t dim, int64_t stride, const void* w, const void* b, int wtype,
+                     float eps, void* y, float* stats, hipStream_t s) {
+  int lanes, nv;
+  norm_layout(ceil_div64(dim, NormVec<T>::V), &lanes, &nv);
+  if (lanes == 0) {
+    k_norm_fwd_long<T><<<norm_grid(rows), 1024, 0, s>>>((const T*)x, rows, dim, stride, w, b, wtype, eps, (T*)y, (float2*)stats);
+    return;
+  }
+  const int rpb = lanes > 256 ? 1 : 256 / lanes;
+  const unsigned grid = norm_grid(ceil_div64(rows, rpb));
+#define GSR_CALL(L, N)                                                                                                    \
+  k_norm_fwd<T, L, N><<<grid, L > 256 ? L : 256, 0, s>>>((const T*)x, rows, dim, stride, w, b, wtype, eps, (T*)y, \
+                                                         (float2*)stats)
+  GSR_NORM_DISPATCH(GSR_CALL)
+#undef GSR_CALL
+}
+
+template <typename T>
+static void norm_bwd(const void* x, const void* dy, int64_t rows, int64_t dim, int64_t stride, int64_t dy_stride,
+                     const void* w, int wtype, const float* stats, void* dx, float* parts, int n, hipStream_t s) {
+  int lanes, nv;
+  norm_layout(ceil_div64(dim, NormVec<T>::V), &lanes, &nv);
+  if (lanes == 0) {
+    if (dx)
+      k_norm_bwd_long<T><<<norm_grid(rows), 1024, 0, s>>>((const T*)x, (const T*)dy, rows, dim, stride, dy_stride, w, wtype,
+                                                         (const float2*)stats, (T*)dx);
+    if (parts)
+      k_norm_cols<T><<<dim3((unsigned)ceil_div64(dim, 256), n), 256, 0, s>>>((const T*)x, (const T*)dy, rows, dim, stride,
+                                                                            dy_stride, (const float2*)stats, parts);
+    return;
+  }
+#define GSR_CALL(L, N)                                                                                                     \
+  k_norm_bwd<T, L, N><<<n, L > 256 ? L : 256, 0, s>>>((const T*)x, (const T*)dy, rows, dim, stride, dy_stride, w, wtype, \
+                                                      (const float2*)stats, (T*)dx, parts)
+  GSR_NORM_DISPATCH(GSR_CALL)
+#undef GSR_CALL
+}
+
+static int norm_check(const char* who, int64_t rows, int64_t dim, int64_t stride, int xtype, int wtype) {
+  GSR_REQUIRE(rows >= 0 && rows <= INT32_MAX, "%s: bad rows %lld", who, (long long)rows);
+  GSR_REQUIRE(dim >= 1 && dim <= INT32_MAX, "%s: bad dim %lld", who, (long long)dim);
+  GSR_REQUIRE(rows <= 1 || stride >= dim, "%s: row stride %lld below dim %lld", who, (long long)stride, (long long)dim);
+  GSR_REQUIRE(known_type(xtype) && known_type(wtype), "%s: bad type (%d, %d)", who, xtype, wtype);
+  return 0;
+}
+
+}  // namespace gsr
+
+using namespace gsr;
+
+extern "C" int gsr_layer_norm_fwd(const void* x, int64_t rows, int64_t dim, int64_t stride, int32_t xtype, const void* w,
+                                  const void* b, int32_t wtype, float eps, void* y, float* stats, void* stream) {
+  if (const int e = norm_check("gsr_layer_norm_fwd", rows, dim, stride, xtype, wtype)) return e;
+  GSR_REQUIRE(eps >= 0.f, "gsr_layer_norm_fwd: bad eps %g", eps);
+  if (rows == 0) return 0;
+  GSR_REQUIRE(x && y, "gsr_layer_norm_fwd: null x or y");
+  const auto s = (hipStream_t)stream;
+  if (xtype == GSR_F32) {
+    norm_fwd<float>(x, rows, dim, stride, w, b, wtype, eps, y, stats, s);
+  } else if (xtype == GSR_BF16) {
+    norm_fwd<bf16>(x, rows, dim, stride, w, b, wtype, eps, y, stats, s);
+  } else {
+    norm_fwd<f16>(x, rows, dim, stride, w, b, wtype, eps, y, stats, s);
+  }
+  GSR_LAUNCH_CHECK("gsr_layer_norm_fwd");
+  return 0;
+}
+
+extern "C" size_t gsr_layer_norm_workspace(int64_t rows, int64_t dim, int32_t xtype) {
+  if (rows <= 0 || dim <= 0 || !known_type(xtype)) return 0;
+  return (size_t)norm_parts(rows, dim, xtype) * 2 * (size_t)dim * sizeof(float);
+}
+
+extern "C" int gsr_layer_norm_bwd(const void* x, const void* dy, int64_t rows, int64_t dim, int64_t stride,
+                                  int64_t dy_stride, int32_t xtype, const void* w, int32_t wtype, const float* stats,
+                                  void* dx, void* dw, void* db, void* workspace, size_t workspace_bytes, void* stream) {
+  if (const int e = norm_check("gsr_layer_norm_bwd", rows, dim, stride, xtype, wtype)) return e;
+  GSR_REQUIRE(rows <= 1 || dy_stride >= dim, "gsr_layer_norm_bwd: dy row stride %lld below dim", (long long)dy_stride);
+  const bool sums = dw || db;
+  if (!dx && !sums) return 0;
+  const auto s = (hipStream_t)stream;
+  const int n = rows ? norm_parts(rows, dim, xtype) : 0;
+  if (sums)
+    GSR_REQUIRE(workspace_bytes >= gsr_layer_norm_workspace(rows, dim, xtype) && (workspace || !rows),
+                "gsr_layer_norm_bwd: workspace too small (%zu bytes)", workspace_bytes);
+  if (rows) {
+    GSR_REQUIRE(x && dy && stats, "gsr_layer_norm_bwd: null x, dy or stats");
+    float* parts = sums ? (float*)workspace : nullptr;
+    if (xtype == GSR_F32) {
+      norm_bwd<float>(x, dy, rows, dim, stride, dy_stride, w, wtype, stats, dx, parts, n, s);
+    } else if (xtype == GSR_BF16) {
+      norm_bwd<bf16>(x, dy, rows, dim, stride, dy_stride, w, wtype, stats, dx, parts, n, s);
+    } else {
+      norm_bwd<f16>(x, dy, rows, dim, stride, dy_stride, w, wtype, stats, dx, parts, n, s);
+    }
+    GSR_LAUNCH_CHECK("gsr_layer_norm_bwd");
+  }
+  if (sums) {
+    k_norm_join<<<(unsigned)ceil_div64(2 * dim, 64), 1024, 0, s>>>((const float*)workspace, n, dim, dw, db, wtype);
+    GSR_LAUNCH_CHECK("gsr_layer_norm_bwd (join)");
+  }
+  return 0;
+}

@@ -10,7 +10,8 @@ import ctypes
 import os
 import threading
 
-__all__ = ["LIB_PATH", "GsrLibraryError", "lib", "check", "BinStats", "BinCaps", "LossTerms", "EXPORTS", "ABI_VERSION",
+__all__ = ["LIB_PATH", "GsrLibraryError", "lib", "check", "BinStats", "BinCaps", "LossTerms", "AdamwTensor",
+           "AdamwArgs", "EXPORTS", "ABI_VERSION", "F32", "BF16", "F16", "ADAMW_BLOCK",
            "RADIUS_OPACITY_AABB", "RADIUS_ISOTROPIC_3SIGMA", "ORDER_DEPTH", "ORDER_INDEX", "TILE"]
 
 LIB_PATH = os.environ.get(
@@ -25,8 +26,11 @@ ORDER_DEPTH = 0
 ORDER_INDEX = 1
 INPUT_ADAPTER = 0
 INPUT_GSPLAT = 1
+# element types of the layer and optimizer calls (include/gsr.h GSR_F32 / GSR_BF16 / GSR_F16)
+F32, BF16, F16 = 0, 1, 2
+ADAMW_BLOCK = 256   # GSR_ADAMW_BLOCK: elements that share a unit of an 8-bit moment
 
-ABI_VERSION = 14   # include/gsr.h GSR_ABI_VERSION this binding is written for
+ABI_VERSION = 15   # include/gsr.h GSR_ABI_VERSION this binding is written for
 # gsr_set_bwd2d_parts at load (profiles/r05_ab5_bwd2d_parts_sweep.txt; GSR_BWD2D_PART_WGS overrides it
 # for measurements, tools/parts_sweep.sh)
 BWD2D_PART_WORKGROUPS = int(os.environ.get("GSR_BWD2D_PART_WGS", "4608"))
@@ -73,6 +77,20 @@ class LossTerms(ctypes.Structure):
     _fields_ = [("rgb", ctypes.c_void_p), ("target_img", ctypes.c_void_p), ("target_mask", ctypes.c_void_p),
                 ("sums", ctypes.c_void_p), ("grad_out", ctypes.c_void_p), ("v_rgb_extra", ctypes.c_void_p),
                 ("v_alpha_extra", ctypes.c_void_p), ("img_lambda", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+class AdamwTensor(ctypes.Structure):
+    """gsr_adamw_tensor (include/gsr.h): one tensor of an AdamW step."""
+    _fields_ = [("p", ctypes.c_void_p), ("g", ctypes.c_void_p), ("m", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("m_unit", ctypes.c_void_p), ("v_unit", ctypes.c_void_p), ("step", ctypes.c_void_p),
+                ("n", ctypes.c_int64)]
+
+
+class AdamwArgs(ctypes.Structure):
+    """gsr_adamw_args (include/gsr.h)."""
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double), ("step", ctypes.c_int64),
+                ("lr_dev", ctypes.c_void_p), ("bits", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
 _P = ctypes.c_void_p
@@ -148,6 +166,12 @@ EXPORTS = {
                                         _P, _P]),
     "gsr_carve_medoids_workspace": (_SZ, [_I32]),
     "gsr_carve_medoids": (ctypes.c_int, [_P, _I32, _I32, _I32, _P, _SZ, _P, _P]),
+    "gsr_layer_norm_fwd": (ctypes.c_int, [_P, _I64, _I64, _I64, _I32, _P, _P, _I32, _F, _P, _P, _P]),
+    "gsr_layer_norm_workspace": (_SZ, [_I64, _I64, _I32]),
+    "gsr_layer_norm_bwd": (ctypes.c_int, [_P, _P, _I64, _I64, _I64, _I64, _I32, _P, _I32, _P, _P, _P, _P, _P, _SZ,
+                                          _P]),
+    "gsr_adamw_step": (ctypes.c_int, [_P, _I32, _I32, _I32, ctypes.POINTER(AdamwArgs), _P]),
+    "gsr_adamw_decode_root": (ctypes.c_int, [_P, _P, _I64, _P, _P]),
 }
 
 _lock = threading.Lock()
