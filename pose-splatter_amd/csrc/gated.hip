@@ -1,0 +1,418 @@
+// Gated block  h = act(x Wg^T + bg) * (x Wu^T + bu)  and its backward pass.
+//
+//   g = x Wg^T + bg,  u = x Wu^T + bu,  h = act(g) u
+//   dg = dh u act'(g),  du = dh act(g)
+//   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dbg, dbu = column sums of dg, du
+//
+// Three products.  The forward's one launch computes both projections of a tile side by side, so
+// that g, u and the activation never leave registers; the backward computes them again with
+// the gradients as its epilogue (2 of its 6 product units, against 16 bytes an element of memory
+// kept from the forward and moved twice), then takes dx from K = [dg | du] and both weight
+// gradients from M = [dg | du].
+//
+// k_tile: 64 x 64 tiles of any shape, stride and alignment, with 16x16 matrix instructions: fp32
+// ones for fp32 (exact fp32 products), bf16/fp16 ones with fp32 sums.  A weight gradient's sum
+// over rows is split over workgroups where there are few tiles; the parts are joined in order.
+#include "gated.h"
+
+namespace gsr {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+// One matrix operand: element (i, k) at p[i * outer + k * inner], one of the strides 1.
+template <typename T>
+struct Operand {
+  const T* p;
+  int64_t stride;
+};
+
+template <typename T>
+struct TileK {
+  static constexpr int V = 16 / sizeof(T);    // elements of a 16-byte load
+  static constexpr int BK = 4 * V;            // K of a step: 32 in 16 bits, 16 in fp32
+  static constexpr int LD = BK + V;           // a row in shared memory, padded by 16 bytes
+};
+
+// 16 bytes of one operand's tile in flight, and where they go in shared memory.  KC: K is the
+// contiguous index.
+template <typename T, bool KC>
+__device__ __forceinline__ void tile_fetch(Operand<T> a, int64_t i0, int64_t rows, int64_t k0, int64_t k1,
+                                           float (&v)[TileK<T>::V]) {
+  constexpr int V = TileK<T>::V;
+  const int t = threadIdx.x;
+  if constexpr (KC) {
+    const int64_t i = i0 + t / 4, k = k0 + (t % 4) * V;
+    load_upto(a.p + i * a.stride + k, i < rows ? k1 - k : 0, v);
+  } else {
+    const int64_t k = k0 + t / (64 / V), i = i0 + (t % (64 / V)) * V;
+    load_upto(a.p + k * a.stride + i, k < k1 ? rows - i : 0, v);
+  }
+}
+
+template <typename T, bool KC>
+__device__ __forceinline__ void tile_keep(T* lds, const float (&v)[TileK<T>::V]) {
+  constexpr int V = TileK<T>::V, LD = TileK<T>::LD;
+  const int t = threadIdx.x;
+  if constexpr (KC) {
+    store_vec(lds + (t / 4) * LD + (t % 4) * V, v);
+  } else {
+    const int k = t / (64 / V), i = (t % (64 / V)) * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) lds[(i + j) * LD + k] = from_f<T>(v[j]);
+  }
+}
+
+// c += a b over one step of K: a, b the 16 rows' 16 bytes of this lane (row lane % 16, K
+// group lane / 16; the order of K is the same in both, so the sum does not care).
+template <typename T>
+__device__ __forceinline__ v4f tile_mma(const T* a, const T* b, v4f c);
+template <>
+__device__ __forceinline__ v4f tile_mma<bf16>(const bf16* a, const bf16* b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const v8bf*)a, *(const v8bf*)b, c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ v4f tile_mma<f16>(const f16* a, const f16* b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const v8h*)a, *(const v8h*)b, c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ v4f tile_mma<float>(const float* a, const float* b, v4f c) {
+  const v4f x = *(const v4f*)a, y = *(const v4f*)b;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s], y[s], c, 0, 0, 0);
+  return c;
+}
+
+// acc[NB][nb][mb]: this wave's 32 x 32 of the tile (wave w: rows 32 (w % 2), columns 32 (w / 2)); a
+// lane holds row m = 16 mb + lane % 16 and columns n = 16 nb + 4 (lane / 16) + 0..3.
+// B(k): the operands for K step k0 (the gradient product changes matrices midway).
+template <typename T, int NB, bool AKC, bool BKC, typename FB>
+__device__ __forceinline__ void tile_product(Operand<T> a, int64_t m0, int64_t M, FB b_at, int64_t n0, int64_t N,
+                                             int64_t k0, int64_t k1, v4f (&acc)[NB][2][2]) {
+  constexpr int V = TileK<T>::V, BK = TileK<T>::BK, LD = TileK<T>::LD;
+  __shared__ __attribute__((aligned(16))) T as[64 * LD];
+  __shared__ __attribute__((aligned(16))) T bs[NB][64 * LD];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int at = (lane % 16) * LD + (lane / 16) * V, wm = wave % 2 * 32, wn = wave / 2 * 32;
+#pragma unroll
+  for (int q = 0; q < NB; ++q)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[q][i / 2][i % 2] = v4f{0.f, 0.f, 0.f, 0.f};
+  float av[V], bv[NB][V];
+  const auto fetch = [&](int64_t k) {
+    tile_fetch<T, AKC>(a, m0, M, k, k1, av);
+#pragma unroll
+    for (int q = 0; q < NB; ++q) {
+      const auto o = b_at(q, k);
+      tile_fetch<T, BKC>(o.op, n0, N, o.k, o.kend < k1 ? o.kend : k1, bv[q]);
+    }
+  };
+  if (k0 < k1) fetch(k0);
+  for (int64_t k = k0; k < k1; k += BK) {
+    __syncthreads();
+    tile_keep<T, AKC>(as, av);
+#pragma unroll
+    for (int q = 0; q < NB; ++q) tile_keep<T, BKC>(bs[q], bv[q]);
+    __syncthreads();
+    if (k + BK < k1) fetch(k + BK);   // in flight over the products
+#pragma unroll
+    for (int q = 0; q < NB; ++q)
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb)
+          acc[q][nb][mb] = tile_mma<T>(bs[q] + (wn + nb * 16) * LD + at, as + (wm + mb * 16) * LD + at, acc[q][nb][mb]);
+  }
+}
+
+template <typename T>
+struct OperandAt {
+  Operand<T> op;
+  int64_t k, kend;   // where the step's K lies in op, and its end there
+};
+
+// Forward (dgu NULL) or the gradients of the projections (h NULL): dgu [rows][2 gated_pad(hidden)],
+// parts [row blocks][2][hidden] the column sums of each block of 64 rows (NULL: not wanted).
+template <typename T>
+__global__ __launch_bounds__(256) void k_tile_gated(const T* x, int64_t x_stride, const T* wg, const T* wu, const T* bg,
+                                                    const T* bu, int act, GatedShape s, T* h, const T* dh,
+                                                    int64_t dh_stride, T* dgu, float* parts) {
+  const int64_t m0 = (int64_t)blockIdx.x * 64, n0 = (int64_t)blockIdx.y * 64;
+  v4f acc[2][2][2];
+  tile_product<T, 2, true, true>(
+      Operand<T>{x, x_stride}, m0, s.rows,
+      [&](int q, int64_t k) { return OperandAt<T>{Operand<T>{q ? wu : wg, s.dim}, k, s.dim}; }, n0, s.hidden, 0, s.dim, acc);
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int64_t pad = gated_pad(s.hidden);
+  __shared__ float sums[2][2][64];   // [row half][dg, du][column]
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb) {
+    const int64_t n = n0 + wave / 2 * 32 + nb * 16 + lane / 16 * 4, left = s.hidden - n;
+    float gb[4], ub[4], sg[4] = {}, su[4] = {};
+    load_upto(bg + n, bg ? left : 0, gb);
+    load_upto(bu + n, bu ? left : 0, ub);
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb) {
+      const int64_t m = m0 + wave % 2 * 32 + mb * 16 + lane % 16;
+      float g[4], u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        g[i] = acc[0][nb][mb][i] + gb[i];
+        u[i] = acc[1][nb][mb][i] + ub[i];
+      }
+      if (!dgu) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float a, slope;
+          activate<T>(act, g[i], a, slope);
+          g[i] = a * u[i];
+        }
+        if (m < s.rows) store_upto(h + m * s.hidden + n, left, g);
+      } else if (m < s.rows) {
+        float d[4];
+        load_upto(dh + m * dh_stride + n, left, d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float a, slope;
+          activate<T>(act, g[i], a, slope);
+          g[i] = i < left ? d[i] * u[i] * slope : 0.f;   // (the padding holds zeros)
+          u[i] = i < left ? d[i] * a : 0.f;
+          sg[i] += g[i];
+          su[i] += u[i];
+        }
+        store_vec(dgu + m * 2 * pad + n, g);   // n + 4 <= pad: the tiles cover the padding exactly
+        store_vec(dgu + m * 2 * pad + pad + n, u);
+      }
+    }
+    if (parts) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) {
+          sg[i] += __shfl_xor(sg[i], d);
+          su[i] += __shfl_xor(su[i], d);
+        }
+        if (lane % 16 == 0) {
+          const int c = wave / 2 * 32 + nb * 16 + lane / 16 * 4 + i;
+          sums[wave % 2][0][c] = sg[i];
+          sums[wave % 2][1][c] = su[i];
+        }
+      }
+    }
+  }
+  if (parts) {
+    __syncthreads();
+    const int c = threadIdx.x % 64, which = threadIdx.x / 64;
+    if (which < 2 && n0 + c < s.hidden)
+      parts[((int64_t)blockIdx.x * 2 + which) * s.hidden + n0 + c] = sums[0][which][c] + sums[1][which][c];
+  }
+}
+
+// dx = [dg | du] [Wg; Wu]
+template <typename T>
+__global__ __launch_bounds__(256) void k_tile_dx(const T* dgu, const T* wg, const T* wu, GatedShape s, T* dx) {
+  const int64_t m0 = (int64_t)blockIdx.x * 64, n0 = (int64_t)blockIdx.y * 64, pad = gated_pad(s.hidden);
+  v4f acc[1][2][2];
+  tile_product<T, 1, true, false>(
+      Operand<T>{dgu, 2 * pad}, m0, s.rows,
+      [&](int, int64_t k) {
+        return k < pad ? OperandAt<T>{Operand<T>{wg, s.dim}, k, s.hidden} : OperandAt<T>{Operand<T>{wu, s.dim}, k - pad, s.hidden};
+      },
+      n0, s.dim, 0, 2 * pad, acc);
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb) {
+      const int64_t m = m0 + wave % 2 * 32 + mb * 16 + lane % 16, n = n0 + wave / 2 * 32 + nb * 16 + lane / 16 * 4;
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = acc[0][nb][mb][i];
+      if (m < s.rows) store_upto(dx + m * s.dim + n, s.dim - n, v);
+    }
+}
+
+// [dWg; dWu] = [dg | du]^T x over the rows of share blockIdx.z.  One share: into dwg, dwu; more:
+// fp32 parts [share][2][hidden][dim].
+template <typename T>
+__global__ __launch_bounds__(256) void k_tile_dw(const T* dgu, const T* x, int64_t x_stride, GatedShape s, int64_t share,
+                                                 T* dwg, T* dwu, float* parts) {
+  const int64_t m0 = (int64_t)blockIdx.x * 64, n0 = (int64_t)blockIdx.y * 64, pad = gated_pad(s.hidden);
+  const int64_t k0 = blockIdx.z * share, k1 = k0 + share < s.rows ? k0 + share : s.rows;
+  v4f acc[1][2][2];
+  tile_product<T, 1, false, false>(
+      Operand<T>{dgu, 2 * pad}, m0, 2 * pad,
+      [&](int, int64_t k) { return OperandAt<T>{Operand<T>{x, x_stride}, k, s.rows}; }, n0, s.dim, k0, k1, acc);
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb) {
+      const int64_t c = m0 + wave % 2 * 32 + mb * 16 + lane % 16, n = n0 + wave / 2 * 32 + nb * 16 + lane / 16 * 4;
+      const int which = c >= pad;
+      const int64_t m = c - which * pad;
+      if (m >= s.hidden) continue;
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = acc[0][nb][mb][i];
+      if (parts) {
+        store_upto(parts + ((blockIdx.z * 2 + which) * s.hidden + m) * s.dim + n, s.dim - n, v);
+      } else if (T* to = which ? dwu : dwg) {
+        store_upto(to + m * s.dim + n, s.dim - n, v);
+      }
+    }
+}
+
+// a, b [n each] = the sum over `count` rows of parts [count][2][n], in order.
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_join(const float* parts, int64_t count, int64_t n, T* a, T* b) {
+  __shared__ float sum[4][64];
+  const int lane = threadIdx.x % 64, grp = threadIdx.x / 64;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (c < 2 * n)
+    for (int64_t r = grp; r < count; r += 4) s += parts[r * 2 * n + c];
+  sum[grp][lane] = s;
+  __syncthreads();
+  if (grp == 0 && c < 2 * n) {
+    s = (sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane]);
+    if (c < n) {
+      if (a) a[c] = from_f<T>(s);
+    } else if (b) {
+      b[c - n] = from_f<T>(s);
+    }
+  }
+}
+
+// Shares of the rows in a weight gradient: enough workgroups for two a CU, each share at least 256
+// rows, and their parts at most 64 MB.
+static int64_t gated_shares(GatedShape s) {
+  const int64_t tiles = ceil_div64(2 * gated_pad(s.hidden), 64) * ceil_div64(s.dim, 64);
+  int64_t n = 512 / tiles;
+  n = n < s.rows / 256 ? n : s.rows / 256;
+  const int64_t most = (64 << 20) / (2 * s.hidden * s.dim * 4);
+  n = n < most ? n : most;
+  return n < 1 ? 1 : n;
+}
+
+struct GatedSpace {
+  int64_t dgu, bias, shares, total;   // byte offsets
+};
+
+static GatedSpace gated_space(GatedShape s, int type) {
+  const auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+  GatedSpace w;
+  w.dgu = 0;
+  w.bias = up(s.rows * 2 * gated_pad(s.hidden) * (int64_t)type_size(type));
+  w.shares = w.bias + up(ceil_div64(s.rows, 64) * 2 * s.hidden * 4);
+  const int64_t n = gated_shares(s);
+  w.total = w.shares + (n > 1 ? up(n * 2 * s.hidden * s.dim * 4) : 0);
+  return w;
+}
+
+template <typename T>
+static void gated_fwd(const void* x, int64_t x_stride, const void* wg, const void* wu, const void* bg, const void* bu, int act,
+                      GatedShape s, void* h, hipStream_t st) {
+  const dim3 grid((unsigned)ceil_div64(s.rows, 64), (unsigned)ceil_div64(s.hidden, 64));
+  k_tile_gated<T><<<grid, 256, 0, st>>>((const T*)x, x_stride, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, act, s,
+                                        (T*)h, nullptr, 0, nullptr, nullptr);
+}
+
+template <typename T>
+static void gated_bwd(const void* x, int64_t x_stride, const void* wg, const void* wu, const void* bg, const void* bu, int act,
+                      GatedShape s, const void* dh, int64_t dh_stride, void* dx, void* dwg, void* dwu, void* dbg, void* dbu,
+                      char* ws, hipStream_t st) {
+  const GatedSpace w = gated_space(s, sizeof(T) == 4 ? GSR_F32 : GSR_BF16);
+  T* dgu = (T*)(ws + w.dgu);
+  float* bias = dbg || dbu ? (float*)(ws + w.bias) : nullptr;
+  const int64_t rb = ceil_div64(s.rows, 64), pad = gated_pad(s.hidden);
+  k_tile_gated<T><<<dim3((unsigned)rb, (unsigned)(pad / 64)), 256, 0, st>>>(
+      (const T*)x, x_stride, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, act, s, nullptr, (const T*)dh, dh_stride,
+      dgu, bias);
+  if (bias)
+    k_gated_join<T><<<(unsigned)ceil_div64(2 * s.hidden, 64), 256, 0, st>>>(bias, rb, s.hidden, (T*)dbg, (T*)dbu);
+  if (dx)
+    k_tile_dx<T><<<dim3((unsigned)rb, (unsigned)ceil_div64(s.dim, 64)), 256, 0, st>>>(dgu, (const T*)wg, (const T*)wu, s,
+                                                                                      (T*)dx);
+  if (dwg || dwu) {
+    const int64_t n = gated_shares(s), share = ceil_div64(ceil_div64(s.rows, n), 32) * 32;
+    const dim3 grid((unsigned)(2 * pad / 64), (unsigned)ceil_div64(s.dim, 64), (unsigned)n);
+    float* parts = n > 1 ? (float*)(ws + w.shares) : nullptr;
+    k_tile_dw<T><<<grid, 256, 0, st>>>(dgu, (const T*)x, x_stride, s, share, (T*)dwg, (T*)dwu, parts);
+    if (parts)
+      k_gated_join<T><<<(unsigned)ceil_div64(2 * s.hidden * s.dim, 64), 256, 0, st>>>(parts, n, s.hidden * s.dim, (T*)dwg,
+                                                                                    (T*)dwu);
+  }
+}
+
+static int gated_check(const char* who, GatedShape s, int64_t x_stride, int type, int act) {
+  GSR_REQUIRE(s.rows >= 0 && s.rows <= (int64_t)1 << 26, "%s: bad rows %lld", who, (long long)s.rows);
+  GSR_REQUIRE(s.dim >= 1 && s.dim <= 1 << 20 && s.hidden >= 1 && s.hidden <= 1 << 20, "%s: bad dim %lld or hidden %lld", who,
+              (long long)s.dim, (long long)s.hidden);
+  GSR_REQUIRE(s.rows <= 1 || x_stride >= s.dim, "%s: row stride %lld below dim %lld", who, (long long)x_stride,
+              (long long)s.dim);
+  GSR_REQUIRE(known_type(type), "%s: bad type %d", who, type);
+  GSR_REQUIRE(act >= GSR_ACT_SILU && act <= GSR_ACT_SIGMOID, "%s: bad activation %d", who, act);
+  return 0;
+}
+
+}  // namespace gsr
+
+using namespace gsr;
+
+extern "C" int gsr_gated_fwd(const void* x, int64_t rows, int64_t dim, int64_t x_stride, int32_t type, const void* wg,
+                             const void* wu, int64_t hidden, const void* bg, const void* bu, int32_t act, void* h,
+                             void* stream) {
+  const GatedShape s{rows, dim, hidden};
+  if (const int e = gated_check("gsr_gated_fwd", s, x_stride, type, act)) return e;
+  if (rows == 0) return 0;
+  GSR_REQUIRE(x && wg && wu && h, "gsr_gated_fwd: null pointer");
+  const auto st = (hipStream_t)stream;
+  if (type == GSR_F32) {
+    gated_fwd<float>(x, x_stride, wg, wu, bg, bu, act, s, h, st);
+  } else if (type == GSR_BF16) {
+    gated_fwd<bf16>(x, x_stride, wg, wu, bg, bu, act, s, h, st);
+  } else {
+    gated_fwd<f16>(x, x_stride, wg, wu, bg, bu, act, s, h, st);
+  }
+  GSR_LAUNCH_CHECK("gsr_gated_fwd");
+  return 0;
+}
+
+extern "C" size_t gsr_gated_bwd_workspace(int64_t rows, int64_t dim, int64_t hidden, int32_t type) {
+  if (rows < 0 || dim < 1 || hidden < 1 || !known_type(type)) return 0;
+  return (size_t)gated_space(GatedShape{rows, dim, hidden}, type).total;
+}
+
+extern "C" int gsr_gated_bwd(const void* x, int64_t rows, int64_t dim, int64_t x_stride, int32_t type, const void* wg,
+                             const void* wu, int64_t hidden, const void* bg, const void* bu, int32_t act, const void* dh,
+                             int64_t dh_stride, void* dx, void* dwg, void* dwu, void* dbg, void* dbu, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  const GatedShape s{rows, dim, hidden};
+  if (const int e = gated_check("gsr_gated_bwd", s, x_stride, type, act)) return e;
+  GSR_REQUIRE(rows <= 1 || dh_stride >= hidden, "gsr_gated_bwd: dh row stride %lld below hidden", (long long)dh_stride);
+  GSR_REQUIRE(wg && wu && (rows == 0 || (x && dh)), "gsr_gated_bwd: null pointer");
+  GSR_REQUIRE(workspace_bytes >= gsr_gated_bwd_workspace(rows, dim, hidden, type) && (workspace || rows == 0),
+              "gsr_gated_bwd: workspace too small (%zu bytes)", workspace_bytes);
+  const auto st = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  if (rows == 0) {   // sums over no rows
+    const auto zero = [&](void* p, int64_t n) {
+      if (p) k_gated_join<bf16><<<(unsigned)ceil_div64(2 * n, 64), 256, 0, st>>>(nullptr, 0, n, (bf16*)p, nullptr);
+    };
+    const int64_t each = type == GSR_F32 ? 2 : 1;   // zeros of any type, 16 bits at a time
+    zero(dwg, hidden * dim * each);
+    zero(dwu, hidden * dim * each);
+    zero(dbg, hidden * each);
+    zero(dbu, hidden * each);
+  } else if (type == GSR_F32) {
+    gated_bwd<float>(x, x_stride, wg, wu, bg, bu, act, s, dh, dh_stride, dx, dwg, dwu, dbg, dbu, ws, st);
+  } else if (type == GSR_BF16) {
+    gated_bwd<bf16>(x, x_stride, wg, wu, bg, bu, act, s, dh, dh_stride, dx, dwg, dwu, dbg, dbu, ws, st);
+  } else {
+    gated_bwd<f16>(x, x_stride, wg, wu, bg, bu, act, s, dh, dh_stride, dx, dwg, dwu, dbg, dbu, ws, st);
+  }
+  GSR_LAUNCH_CHECK("gsr_gated_bwd");
+  return 0;
+}

@@ -9,8 +9,10 @@ Replaces, in PoseSplatter.forward (src/model.py:134-160):
   (src/model.py:258-298, with its per-Gaussian float64 torch.linalg.eigh) by one fused
   per-Gaussian kernel, forward and backward (`gaussian_params_3d`, `pose_transform_3d`).
 
-The MLP itself stays a torch nn.Sequential (two small GEMMs on hipBLASLt).  No CPU path:
-the functions raise on CPU tensors.
+The MLP is any callable on the selected features: the reference's torch nn.Sequential (two
+small GEMMs on hipBLASLt) or `GatedHead` (layer norm and gated block of gsr.layers, then one
+output projection), which trains with gsr.optim.AdamW.  No CPU path: the functions raise on CPU
+tensors.
 """
 from __future__ import annotations
 
@@ -19,9 +21,11 @@ import ctypes
 import torch
 
 from ._lib import check, lib
+from .layers import GatedLinear, LayerNorm
 from .render import _ptr, _require_device, _stream
 
-__all__ = ["select_gaussians", "gaussian_params_3d", "pose_transform_3d", "params_from_volume_3d"]
+__all__ = ["select_gaussians", "gaussian_params_3d", "pose_transform_3d", "params_from_volume_3d",
+           "GatedHead"]
 
 _info_host = {}
 
@@ -153,6 +157,25 @@ def pose_transform_3d(params: torch.Tensor, angle: float, p_3d) -> torch.Tensor:
     if not isinstance(p_3d, torch.Tensor):
         p_3d = torch.tensor(p_3d, dtype=torch.float32)
     return _Pose3D.apply(params, float(angle), p_3d)
+
+
+class GatedHead(torch.nn.Module):
+    """A parameter network for ``params_from_volume_3d`` (the place of the reference's
+    gaussian_param_net, src/model.py:207-208): layer norm over the voxel's channels, a gated
+    hidden layer, and the projection to the ``out`` network outputs of a Gaussian.
+
+        head = GatedHead(channels, hidden=128).to("cuda")
+        params = params_from_volume_3d(volume, head, grid, scale, angle=a, p_3d=p)"""
+
+    def __init__(self, channels: int, hidden: int = 128, out: int = 14, activation: str = "silu", device=None,
+                 dtype=None):
+        super().__init__()
+        self.norm = LayerNorm(channels, device=device, dtype=dtype)
+        self.gated = GatedLinear(channels, hidden, activation, device=device, dtype=dtype)
+        self.out = torch.nn.Linear(hidden, out, device=device, dtype=dtype)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return self.out(self.gated(self.norm(x)))
 
 
 def params_from_volume_3d(volume: torch.Tensor, mlp, grid: torch.Tensor, scale: torch.Tensor, *,

@@ -17,14 +17,15 @@ block are followed in steps.  No CPU path: the functions raise on CPU tensors.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 
 import torch
 
 from . import _lib
 from ._lib import check, lib
-from .layers import _on, _type
-from .render import _require_device, _stream
+from .layers import _on, _raw_stream, _type
+from .render import _require_device
 
 __all__ = ["AdamW", "adamw_step", "decode_root"]
 
@@ -52,14 +53,10 @@ def _layout(t: torch.Tensor):
     return [s for s, d in zip(t.stride(), t.shape) if d != 1]
 
 
-def _check_moment(t: torch.Tensor, p: torch.Tensor, dtype, what: str) -> None:
-    if t.dtype != dtype:
-        raise ValueError(f"adamw_step: {what} must be {dtype}, got {t.dtype}")
+def _check_layout(t: torch.Tensor, p: torch.Tensor, what: str) -> None:
     if t.shape != p.shape or (_layout(t) != _layout(p) if t.numel() else False):
         raise ValueError(f"adamw_step: {what} must have its parameter's shape and strides {tuple(p.shape)}, "
                          f"{p.stride()}; got {tuple(t.shape)}, {t.stride()}")
-    if t.device != p.device:
-        raise ValueError(f"adamw_step: {what} is on {t.device}, its parameter on {p.device}")
 
 
 def _step_args(lr, betas, eps, weight_decay, step, bits):
@@ -133,47 +130,54 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, lr=1e-3, betas=(0.9, 0.9
     else:
         m_type, v_type = torch.float8_e4m3fn, torch.uint8
     groups, ranges, kept = {}, [], []
+    m_size, v_size = m_type.itemsize, v_type.itemsize
     for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
-        if p.device != dev or g.device != dev:
-            raise ValueError(f"adamw_step: tensor {i} is on {p.device}, its gradient on {g.device}, the first on {dev}")
-        pt, gt = _type(p, "adamw_step: a parameter"), _type(g, "adamw_step: a gradient")
-        if g.is_sparse or g.shape != p.shape:
+        if not (p.device == g.device == m.device == v.device == dev):
+            raise ValueError(f"adamw_step: tensor {i}, its gradient and moments are on {p.device}, {g.device}, {m.device} "
+                             f"and {v.device}; the first tensor is on {dev}")
+        types = (p.dtype, g.dtype)
+        group = groups.get(types)
+        if group is None:
+            group = groups[types] = (_type(p, "adamw_step: a parameter"), _type(g, "adamw_step: a gradient"), [])
+        if m.dtype != m_type or v.dtype != v_type:
+            raise ValueError(f"adamw_step: exp_avg must be {m_type} and exp_avg_sq {v_type}, got {m.dtype} and {v.dtype}")
+        if g.layout != torch.strided or g.shape != p.shape:
             raise ValueError(f"adamw_step: gradient {i} must be dense and {tuple(p.shape)}, got {tuple(g.shape)}")
-        if not _dense(p):
-            raise ValueError(f"adamw_step: parameter {i} does not fill its memory (strides {p.stride()})")
-        _check_moment(m, p, m_type, "exp_avg")
-        _check_moment(v, p, v_type, "exp_avg_sq")
+        if not (p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous()
+                and m.shape == p.shape and v.shape == p.shape):
+            if not _dense(p):
+                raise ValueError(f"adamw_step: parameter {i} does not fill its memory (strides {p.stride()})")
+            _check_layout(m, p, "exp_avg")
+            _check_layout(v, p, "exp_avg_sq")
+            if _layout(g) != _layout(p):   # (a gradient of another layout: copied into the parameter's)
+                g = torch.empty_strided(p.shape, p.stride(), dtype=g.dtype, device=dev).copy_(g)
+                kept.append(g)
         n = p.numel()
         if n == 0:
             continue
-        if _layout(g) != _layout(p):   # (a gradient of another layout: copied into the parameter's)
-            g = torch.empty_strided(p.shape, p.stride(), dtype=g.dtype, device=dev).copy_(g)
-            kept.append(g)
-        t = _lib.AdamwTensor()
-        t.p, t.g, t.m, t.v, t.n = p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), n
-        ranges += [(t.p, t.p + n * p.element_size()), (t.m, t.m + n * m.element_size()),
-                   (t.v, t.v + n * v.element_size())]
+        pp, mp, vp, mu, vu, sp = p.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, 0
+        ranges += ((pp, pp + n * p.element_size()), (mp, mp + n * m_size), (vp, vp + n * v_size))
         if bits == 8:
-            for name, u in (("m_unit", exp_avg_units[i]), ("v_unit", exp_avg_root_units[i])):
+            for u in (exp_avg_units[i], exp_avg_root_units[i]):
                 if u.dtype != torch.float32 or u.shape != (_units(n),) or not u.is_contiguous() or u.device != dev:
                     raise ValueError(f"adamw_step: units {i} must be contiguous float32 [{_units(n)}] on {dev}, "
                                      f"got {u.dtype} {tuple(u.shape)} on {u.device}")
-                at = u.data_ptr()
-                setattr(t, name, at)
-                ranges.append((at, at + 4 * u.numel()))
+            mu, vu = exp_avg_units[i].data_ptr(), exp_avg_root_units[i].data_ptr()
+            ranges += ((mu, mu + 4 * _units(n)), (vu, vu + 4 * _units(n)))
         if steps is not None:
             s = steps[i]
             if not isinstance(s, torch.Tensor) or s.numel() != 1 or s.dtype != torch.int64 or s.device != dev:
                 raise ValueError(f"adamw_step: step {i} must be one int64 value on {dev}")
-            t.step = s.data_ptr()
-        groups.setdefault((pt, gt), []).append(t)
+            sp = s.data_ptr()
+        group[2].extend((pp, g.data_ptr(), mp, vp, mu, vu, sp, n))
     _no_overlap(ranges)
     _require_device(params[0], "adamw_step")
     L = lib()
     with _on(dev):
-        stream = _stream(dev)
-        for (pt, gt), ts in groups.items():
-            check(L.gsr_adamw_step((_lib.AdamwTensor * len(ts))(*ts), len(ts), pt, gt, ctypes.byref(args), stream),
+        stream = _raw_stream(dev)
+        for pt, gt, words in groups.values():
+            table = array.array("q", words)   # gsr_adamw_tensor: eight 64-bit fields
+            check(L.gsr_adamw_step(table.buffer_info()[0], len(words) // 8, pt, gt, ctypes.byref(args), stream),
                   "gsr_adamw_step")
     torch.autograd.graph.increment_version(list(params))
 
@@ -191,7 +195,7 @@ def decode_root(codes: torch.Tensor, units: torch.Tensor) -> torch.Tensor:
     out = torch.empty(codes.shape, device=codes.device, dtype=torch.float32)
     with _on(codes.device):
         check(lib().gsr_adamw_decode_root(codes.data_ptr(), units.data_ptr(), codes.numel(), out.data_ptr(),
-                                          _stream(codes.device)), "gsr_adamw_decode_root")
+                                          _raw_stream(codes.device)), "gsr_adamw_decode_root")
     return out
 
 
