@@ -10,10 +10,13 @@
 // kept from the forward and moved twice), then takes dx from K = [dg | du] and both weight
 // gradients from M = [dg | du].
 //
+// Large 16-bit cases run on 256 x 256 tiles (gated_wide.hip); here is what serves all others:
+//
 // k_tile: 64 x 64 tiles of any shape, stride and alignment, with 16x16 matrix instructions: fp32
 // ones for fp32 (exact fp32 products), bf16/fp16 ones with fp32 sums.  A weight gradient's sum
 // over rows is split over workgroups where there are few tiles; the parts are joined in order.
 #include "gated.h"
+#include "gated_wide.h"
 
 namespace gsr {
 
@@ -285,35 +288,111 @@ __global__ __launch_bounds__(256) void k_gated_join(const float* parts, int64_t 
   }
 }
 
-// Shares of the rows in a weight gradient: enough workgroups for two a CU, each share at least 256
-// rows, and their parts at most 64 MB.
-static int64_t gated_shares(GatedShape s) {
-  const int64_t tiles = ceil_div64(2 * gated_pad(s.hidden), 64) * ceil_div64(s.dim, 64);
-  int64_t n = 512 / tiles;
-  n = n < s.rows / 256 ? n : s.rows / 256;
+// Shares of the rows in a weight gradient of `tile` x `tile` tiles: enough workgroups for two 64 x 64
+// (one 256 x 256) tiles a CU, each share at least four tiles of rows, the parts at most 64 MB.
+static int64_t gated_shares(GatedShape s, int64_t tile) {
+  const int64_t tiles = ceil_div64(2 * gated_pad(s.hidden), tile) * ceil_div64(s.dim, tile);
+  int64_t n = (tile == 64 ? 512 : 256) / tiles;
+  n = n < s.rows / (4 * tile) ? n : s.rows / (4 * tile);
   const int64_t most = (64 << 20) / (2 * s.hidden * s.dim * 4);
   n = n < most ? n : most;
   return n < 1 ? 1 : n;
 }
 
+// to [rows][kdim] = p [rows][dim] (row stride `stride`) and zeros: rows that start at 16 bytes and
+// whose length is whole 16-byte pieces.
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_pad(const T* p, int64_t rows, int64_t dim, int64_t stride, int64_t kdim, T* to) {
+  const int64_t per = kdim / 8, n = rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per, c = i % per * 8;
+    float v[8];
+    load_upto(p + r * stride + c, dim - c, v);
+    store_vec(to + r * kdim + c, v);
+  }
+}
+
+template <typename T>
+static const T* gated_padded(const T* p, int64_t rows, int64_t dim, int64_t stride, int64_t kdim, char* to, hipStream_t st) {
+  const int64_t blocks = ceil_div64(rows * (kdim / 8), 256);
+  k_gated_pad<T><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(p, rows, dim, stride, kdim, (T*)to);
+  return (const T*)to;
+}
+
+// Whether a case runs on the 256 x 256 tiles.
+static bool gated_is_wide(GatedShape s, int type) {
+  return type != GSR_F32 && ceil_div64(s.rows, 256) * ceil_div64(s.hidden, 128) >= 128 && s.dim >= 64;
+}
+
+// What a wide case's operands need: rows of whole 16-byte pieces at 16-byte addresses, 256 of them
+// within 31 bits.
+static bool gated_aligned(const void* p, int64_t dim, int64_t stride) {
+  return (uintptr_t)p % 16 == 0 && dim % 8 == 0 && stride % 8 == 0 && stride <= 1 << 21;
+}
+
+// Workspace of a pass, as byte offsets.  Padded copies only where a wide case's inputs need them
+// (an odd dim; a caller whose rows or addresses are odd is told by `copy_x`, `copy_w`).
 struct GatedSpace {
-  int64_t dgu, bias, shares, total;   // byte offsets
+  int64_t x, wg, wu, dgu, bias, shares, total;
+  int64_t kdim, n_shares;
 };
 
-static GatedSpace gated_space(GatedShape s, int type) {
+static GatedSpace gated_space(GatedShape s, int type, bool backward) {
   const auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+  const bool wide = gated_is_wide(s, type);
   GatedSpace w;
-  w.dgu = 0;
-  w.bias = up(s.rows * 2 * gated_pad(s.hidden) * (int64_t)type_size(type));
-  w.shares = w.bias + up(ceil_div64(s.rows, 64) * 2 * s.hidden * 4);
-  const int64_t n = gated_shares(s);
-  w.total = w.shares + (n > 1 ? up(n * 2 * s.hidden * s.dim * 4) : 0);
+  w.kdim = (s.dim + 7) / 8 * 8;
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += up(bytes);
+    return here;
+  };
+  w.x = take(wide ? s.rows * w.kdim * 2 : 0);
+  w.wg = take(wide ? s.hidden * w.kdim * 2 : 0);
+  w.wu = take(wide ? s.hidden * w.kdim * 2 : 0);
+  w.dgu = w.bias = w.shares = at;
+  w.n_shares = 1;
+  if (backward) {
+    w.dgu = take(s.rows * 2 * gated_pad(s.hidden) * (int64_t)type_size(type));
+    w.bias = take(wide ? ceil_div64(s.rows, 256) * 4 * s.hidden * 4 : ceil_div64(s.rows, 64) * 2 * s.hidden * 4);
+    w.n_shares = gated_shares(s, wide ? 256 : 64);
+    w.shares = take(w.n_shares > 1 ? w.n_shares * 2 * s.hidden * s.dim * 4 : 0);
+  }
+  w.total = at;
   return w;
 }
 
 template <typename T>
+static GatedWide gated_wide_args(const void* x, int64_t x_stride, const void* wg, const void* wu, const void* bg,
+                                 const void* bu, int act, GatedShape s, const GatedSpace& w, char* ws, hipStream_t st) {
+  GatedWide a{};
+  a.s = s;
+  a.kdim = s.dim, a.x_stride = x_stride, a.w_stride = s.dim;
+  a.x = x, a.wg = wg, a.wu = wu, a.bg = bg, a.bu = bu, a.act = act;
+  if (!gated_aligned(x, s.dim, x_stride)) {
+    a.x = gated_padded((const T*)x, s.rows, s.dim, x_stride, w.kdim, ws + w.x, st);
+    a.x_stride = w.kdim;
+  }
+  if (!gated_aligned(wg, s.dim, s.dim) || !gated_aligned(wu, s.dim, s.dim)) {
+    a.wg = gated_padded((const T*)wg, s.hidden, s.dim, s.dim, w.kdim, ws + w.wg, st);
+    a.wu = gated_padded((const T*)wu, s.hidden, s.dim, s.dim, w.kdim, ws + w.wu, st);
+    a.w_stride = w.kdim;
+  }
+  if (s.dim % 8) a.kdim = w.kdim;   // (then both were copied)
+  return a;
+}
+
+template <typename T>
 static void gated_fwd(const void* x, int64_t x_stride, const void* wg, const void* wu, const void* bg, const void* bu, int act,
-                      GatedShape s, void* h, hipStream_t st) {
+                      GatedShape s, void* h, char* ws, hipStream_t st) {
+  const int type = __is_same(T, float) ? GSR_F32 : __is_same(T, bf16) ? GSR_BF16 : GSR_F16;
+  if (gated_is_wide(s, type)) {
+    GatedWide a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, gated_space(s, type, false), ws, st);
+    a.h = h;
+    gated_wide(type, kWideFwd, a, 1, st);
+    return;
+  }
   const dim3 grid((unsigned)ceil_div64(s.rows, 64), (unsigned)ceil_div64(s.hidden, 64));
   k_tile_gated<T><<<grid, 256, 0, st>>>((const T*)x, x_stride, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, act, s,
                                         (T*)h, nullptr, 0, nullptr, nullptr);
@@ -323,23 +402,41 @@ template <typename T>
 static void gated_bwd(const void* x, int64_t x_stride, const void* wg, const void* wu, const void* bg, const void* bu, int act,
                       GatedShape s, const void* dh, int64_t dh_stride, void* dx, void* dwg, void* dwu, void* dbg, void* dbu,
                       char* ws, hipStream_t st) {
-  const GatedSpace w = gated_space(s, sizeof(T) == 4 ? GSR_F32 : GSR_BF16);
+  const int type = __is_same(T, float) ? GSR_F32 : __is_same(T, bf16) ? GSR_BF16 : GSR_F16;
+  const GatedSpace w = gated_space(s, type, true);
+  const bool wide = gated_is_wide(s, type);
+  const int64_t rb = ceil_div64(s.rows, 64), pad = gated_pad(s.hidden), n = w.n_shares;
   T* dgu = (T*)(ws + w.dgu);
   float* bias = dbg || dbu ? (float*)(ws + w.bias) : nullptr;
-  const int64_t rb = ceil_div64(s.rows, 64), pad = gated_pad(s.hidden);
-  k_tile_gated<T><<<dim3((unsigned)rb, (unsigned)(pad / 64)), 256, 0, st>>>(
-      (const T*)x, x_stride, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, act, s, nullptr, (const T*)dh, dh_stride,
-      dgu, bias);
+  float* parts = n > 1 ? (float*)(ws + w.shares) : nullptr;
+  GatedWide a{};
+  if (wide) {
+    a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, ws, st);
+    a.dh = dh, a.dh_stride = dh_stride, a.dgu = dgu, a.dx = dx, a.dwg = dwg, a.dwu = dwu, a.parts = bias;
+    gated_wide(type, kWideGrad, a, 1, st);
+  } else {
+    k_tile_gated<T><<<dim3((unsigned)rb, (unsigned)(pad / 64)), 256, 0, st>>>(
+        (const T*)x, x_stride, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, act, s, nullptr, (const T*)dh,
+        dh_stride, dgu, bias);
+  }
   if (bias)
-    k_gated_join<T><<<(unsigned)ceil_div64(2 * s.hidden, 64), 256, 0, st>>>(bias, rb, s.hidden, (T*)dbg, (T*)dbu);
-  if (dx)
+    k_gated_join<T><<<(unsigned)ceil_div64(2 * s.hidden, 64), 256, 0, st>>>(bias, wide ? ceil_div64(s.rows, 256) * 2 : rb,
+                                                                          s.hidden, (T*)dbg, (T*)dbu);
+  if (dx && wide) {
+    gated_wide(type, kWideDx, a, 1, st);
+  } else if (dx) {
     k_tile_dx<T><<<dim3((unsigned)rb, (unsigned)ceil_div64(s.dim, 64)), 256, 0, st>>>(dgu, (const T*)wg, (const T*)wu, s,
                                                                                       (T*)dx);
+  }
   if (dwg || dwu) {
-    const int64_t n = gated_shares(s), share = ceil_div64(ceil_div64(s.rows, n), 32) * 32;
-    const dim3 grid((unsigned)(2 * pad / 64), (unsigned)ceil_div64(s.dim, 64), (unsigned)n);
-    float* parts = n > 1 ? (float*)(ws + w.shares) : nullptr;
-    k_tile_dw<T><<<grid, 256, 0, st>>>(dgu, (const T*)x, x_stride, s, share, (T*)dwg, (T*)dwu, parts);
+    const int64_t share = ceil_div64(ceil_div64(s.rows, n), 64) * 64;
+    if (wide) {
+      a.share = share, a.parts = parts;
+      gated_wide(type, kWideDw, a, (int)n, st);
+    } else {
+      const dim3 grid((unsigned)(2 * pad / 64), (unsigned)ceil_div64(s.dim, 64), (unsigned)n);
+      k_tile_dw<T><<<grid, 256, 0, st>>>(dgu, (const T*)x, x_stride, s, share, (T*)dwg, (T*)dwu, parts);
+    }
     if (parts)
       k_gated_join<T><<<(unsigned)ceil_div64(2 * s.hidden * s.dim, 64), 256, 0, st>>>(parts, n, s.hidden * s.dim, (T*)dwg,
                                                                                     (T*)dwu);
@@ -361,28 +458,32 @@ static int gated_check(const char* who, GatedShape s, int64_t x_stride, int type
 
 using namespace gsr;
 
+extern "C" size_t gsr_gated_workspace(int64_t rows, int64_t dim, int64_t hidden, int32_t type, int32_t backward) {
+  const GatedShape s{rows, dim, hidden};
+  if (gated_check("gsr_gated_workspace", s, dim, type, GSR_ACT_SILU)) return 0;
+  return (size_t)gated_space(s, type, backward != 0).total;
+}
+
 extern "C" int gsr_gated_fwd(const void* x, int64_t rows, int64_t dim, int64_t x_stride, int32_t type, const void* wg,
                              const void* wu, int64_t hidden, const void* bg, const void* bu, int32_t act, void* h,
-                             void* stream) {
+                             void* workspace, size_t workspace_bytes, void* stream) {
   const GatedShape s{rows, dim, hidden};
   if (const int e = gated_check("gsr_gated_fwd", s, x_stride, type, act)) return e;
   if (rows == 0) return 0;
   GSR_REQUIRE(x && wg && wu && h, "gsr_gated_fwd: null pointer");
+  GSR_REQUIRE(workspace_bytes >= gsr_gated_workspace(rows, dim, hidden, type, 0) && (workspace || workspace_bytes == 0),
+              "gsr_gated_fwd: workspace too small (%zu bytes)", workspace_bytes);
+  char* ws = (char*)workspace;
   const auto st = (hipStream_t)stream;
   if (type == GSR_F32) {
-    gated_fwd<float>(x, x_stride, wg, wu, bg, bu, act, s, h, st);
+    gated_fwd<float>(x, x_stride, wg, wu, bg, bu, act, s, h, ws, st);
   } else if (type == GSR_BF16) {
-    gated_fwd<bf16>(x, x_stride, wg, wu, bg, bu, act, s, h, st);
+    gated_fwd<bf16>(x, x_stride, wg, wu, bg, bu, act, s, h, ws, st);
   } else {
-    gated_fwd<f16>(x, x_stride, wg, wu, bg, bu, act, s, h, st);
+    gated_fwd<f16>(x, x_stride, wg, wu, bg, bu, act, s, h, ws, st);
   }
   GSR_LAUNCH_CHECK("gsr_gated_fwd");
   return 0;
-}
-
-extern "C" size_t gsr_gated_bwd_workspace(int64_t rows, int64_t dim, int64_t hidden, int32_t type) {
-  if (rows < 0 || dim < 1 || hidden < 1 || !known_type(type)) return 0;
-  return (size_t)gated_space(GatedShape{rows, dim, hidden}, type).total;
 }
 
 extern "C" int gsr_gated_bwd(const void* x, int64_t rows, int64_t dim, int64_t x_stride, int32_t type, const void* wg,
@@ -393,7 +494,7 @@ extern "C" int gsr_gated_bwd(const void* x, int64_t rows, int64_t dim, int64_t x
   if (const int e = gated_check("gsr_gated_bwd", s, x_stride, type, act)) return e;
   GSR_REQUIRE(rows <= 1 || dh_stride >= hidden, "gsr_gated_bwd: dh row stride %lld below hidden", (long long)dh_stride);
   GSR_REQUIRE(wg && wu && (rows == 0 || (x && dh)), "gsr_gated_bwd: null pointer");
-  GSR_REQUIRE(workspace_bytes >= gsr_gated_bwd_workspace(rows, dim, hidden, type) && (workspace || rows == 0),
+  GSR_REQUIRE(workspace_bytes >= gsr_gated_workspace(rows, dim, hidden, type, 1) && (workspace || rows == 0),
               "gsr_gated_bwd: workspace too small (%zu bytes)", workspace_bytes);
   const auto st = (hipStream_t)stream;
   char* ws = (char*)workspace;

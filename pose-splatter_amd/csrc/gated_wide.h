@@ -1,0 +1,24 @@
+// Launch of the gated block's 256 x 256 products (gated_wide.hip).
+#pragma once
+
+#include "gated.h"
+
+namespace gsr {
+
+enum { kWideFwd, kWideGrad, kWideDx, kWideDw };
+
+// The tensors of one product, 16-bit, x, wg and wu 16-byte aligned with strides (in elements) and
+// kdim, the length of their rows, multiples of 8: the block's dim, or it padded with zeros.
+struct GatedWide {
+  GatedShape s;
+  int64_t kdim, x_stride, w_stride, dh_stride;
+  const void *x, *wg, *wu, *bg, *bu, *dh;
+  void *h, *dgu, *dx, *dwg, *dwu;
+  float* parts;    // gradients: column sums [ceil(rows / 256) * 2][2][hidden]; dW: [share][2][hidden][dim]; or NULL
+  int64_t share;   // dW: rows of x a share, a multiple of 64
+  int act, mt, nt;
+};
+
+void gated_wide(int type, int mode, GatedWide a, int shares, hipStream_t st);
+
+}  // namespace gsr

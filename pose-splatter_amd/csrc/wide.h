@@ -1,0 +1,142 @@
+// 256 x 256 products of 16-bit matrices with fp32 sums: the main loop of the gated block's large cases.
+//
+// A workgroup of four waves owns a 256 x 256 tile, each wave a 128 x 128 quarter of 4 x 4 blocks
+// of 32x32x16 matrix instructions: 256 accumulators a lane.  K advances 64 at a time through two
+// buffers of shared memory (2 x 64 KB).  A quarter that large reads 2 x 128 x 64 elements for
+// 128 x 128 x 64 multiply-adds, 64 bytes of shared memory a cycle and CU at full matrix rate
+// where 128 are available; eight waves of 128 x 64 would need 96 and leave none for the stores.
+//
+// Tiles come straight from global memory into shared memory (16 bytes a lane, no registers).  Each
+// operand is read in the order it lies in memory:
+//   K contiguous     rows of 64 K (128 bytes); 16-byte chunk c of row r sits in slot c ^ (r % 8),
+//                    so the 16-byte reads of eight neighbouring rows hit different banks
+//   K across rows    rows of 256 columns (512 bytes) a K; chunk c of row k sits in slot
+//                    c ^ (2 (k % 4) + 8 (k / 8 % 4)); ds_read_b64_tr_b16 turns 4 K x 16 columns
+//                    into the instruction's K-contiguous operand on the way out
+// The pattern is made by choosing what each lane loads: shared memory itself is filled in lane
+// order.  Loads past an operand's end return zeros (the buffer descriptor's bound), so no tile
+// needs a special case; only K's own end inside a row is checked lane by lane.
+#pragma once
+
+#include "types.h"
+
+namespace gsr {
+
+constexpr int kWideTile = 256, kWideK = 64, kWideThreads = 256;
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef __bf16 wide_v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 wide_v8h __attribute__((ext_vector_type(8)));
+
+template <typename T>
+__device__ __forceinline__ v16f wide_mma(v8s a, v8s b, v16f c) {
+  if constexpr (__is_same(T, bf16)) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(wide_v8bf, a), __builtin_bit_cast(wide_v8bf, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(wide_v8h, a), __builtin_bit_cast(wide_v8h, b), c, 0, 0, 0);
+  }
+}
+
+// A stretch of global memory that ends at base + left: loads at or past the end return zeros.
+struct WideSource {
+  const char* base;
+  int64_t left;   // bytes
+  __device__ __forceinline__ void advance(int64_t bytes) {
+    base += bytes;
+    left -= bytes;
+  }
+  __device__ __forceinline__ v4i descriptor(bool any) const {
+    const uint64_t b = (uint64_t)base;
+    const int64_t n = left < 0 || !any ? 0 : left > 0x7FFFFFFF ? 0x7FFFFFFF : left;
+    return v4i{(int)(uint32_t)b, (int)(uint32_t)(b >> 32) & 0xFFFF, (int)n, 0x00027000};
+  }
+};
+
+// 16 bytes a lane from src + off into shared memory at `lds` (this wave's 1 KB, in lane order).  The
+// loads are written by hand because the compiler would wait for all of them before any read of
+// shared memory; wide_wait() below is their wait.  They name no destination register.
+__device__ __forceinline__ void wide_load(const v4i& src, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(src)
+               : "memory");
+}
+__device__ __forceinline__ void wide_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Orders a wave's own reads and writes of shared memory (they complete in order; the compiler may
+// not move them).
+__device__ __forceinline__ void wide_fence() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
+}
+
+constexpr uint32_t kWideNowhere = 0x80000000u;   // past every descriptor's end
+
+// One operand's tile: this lane's places in it.
+template <bool KC>
+struct WideTile {
+  uint32_t at[8];       // byte offsets of the lane's eight loads from the tile's corner
+  int k;                // KC: the loads' first K
+  uint32_t read[KC ? 4 : 8];   // byte offsets of its reads: per 16 K (KC), or per block and K parity
+
+  // origin: the wave's first row (KC) or column of the tile's 256
+  __device__ __forceinline__ void init(int64_t stride_bytes, int origin) {
+    const int t = threadIdx.x, l = t % 64;
+    if constexpr (KC) {
+      const int c = t % 8 ^ (t / 8 & 7);
+      k = c * 8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) at[j] = (uint32_t)((j * 32 + t / 8) * stride_bytes + c * 16);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) read[kk] = (origin + l % 32) * 128 + ((kk * 2 + l / 32) ^ (l & 7)) * 16;
+    } else {
+      k = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        at[j] = (uint32_t)((j * 8 + t / 32) * stride_bytes + (t % 32 ^ (t / 32 & 3) * 2 ^ (j & 3) * 8) * 16);
+      const int g = l / 16, row = l % 16 / 4;   // K row of the lane's 4 x 16 piece
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int c = origin / 8 + b * 4 + g % 2 * 2 + l % 4 / 2;
+          read[p * 4 + b] = (g / 2 * 8 + row) * 512 + (c ^ row * 2 ^ (p * 2 + g / 2) * 8) * 16 + l % 2 * 8;
+        }
+    }
+  }
+
+  // One of the eight loads that fill the 32 KB at `lds` (j: 4 KB of it), from the lane's j_from-th
+  // place; limit: K left in the source's rows (KC).
+  __device__ __forceinline__ void load(const v4i& d, uint32_t lds, int j, int j_from, int64_t limit) const {
+    wide_load(d, !KC || k < limit ? at[j_from] : kWideNowhere,
+              __builtin_amdgcn_readfirstlane(lds + threadIdx.x / 64 * 1024 + j * 4096));
+  }
+
+  // The operand of the 32 rows from the wave's origin + `off` (a multiple of 32, below 128 where K
+  // runs across rows) and K kk * 16 .. + 15.
+  __device__ __forceinline__ v8s operand(const char* lds, int off, int kk) const {
+    if constexpr (KC) {
+      return *(const v8s*)(lds + read[kk] + off * 128);
+    } else {
+      typedef __attribute__((address_space(3))) v4s lds_v4s;
+      const char* p = lds + read[kk % 2 * 4 + off / 32] + kk * 8192;
+      const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p);
+      const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 2048));
+      return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+// Workgroup `id` of a launch -> its tile.  Workgroups go round the eight XCDs in turn: each XCD gets a
+// run of neighbouring tiles, in groups of eight tile rows, so that its L2 holds what they share.
+__device__ __forceinline__ void wide_tile_of(int id, int mt, int nt, int* m, int* n) {
+  const int total = mt * nt, q = total / 8, r = total % 8, xcd = id % 8;
+  const int pos = (xcd < r ? xcd * (q + 1) : r + xcd * q) + id / 8;
+  const int group = pos / (8 * nt), first = group * 8, rows = mt - first < 8 ? mt - first : 8, in = pos - group * 8 * nt;
+  *m = first + in % rows;
+  *n = in / rows;
+}
+
+}  // namespace gsr

@@ -177,9 +177,12 @@ class _GatedLinear(torch.autograd.Function):
         dev, dim, hidden, t = x.device, x.shape[-1], w_gate.shape[0], _TYPE[x.dtype]
         xr, stride = _as_rows(x, dim)
         h = torch.empty((*x.shape[:-1], hidden), device=dev, dtype=x.dtype)
+        ws_bytes = L.gsr_gated_workspace(xr.shape[0], dim, hidden, t, 0)
+        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws_bytes else None
         with _on(dev):
             check(L.gsr_gated_fwd(xr.data_ptr(), xr.shape[0], dim, stride, t, w_gate.data_ptr(), w_up.data_ptr(), hidden,
-                                  _ptr(b_gate), _ptr(b_up), act, h.data_ptr(), _raw_stream(dev)), "gsr_gated_fwd")
+                                  _ptr(b_gate), _ptr(b_up), act, h.data_ptr(), _ptr(ws), ws_bytes, _raw_stream(dev)),
+                  "gsr_gated_fwd")
         if any(ctx.needs_input_grad):
             ctx.save_for_backward(xr, w_gate, w_up, b_gate, b_up)
             ctx.cfg = (x.shape, stride, t, act)
@@ -201,7 +204,7 @@ class _GatedLinear(torch.autograd.Function):
         sizes = (shape, wg.shape, wu.shape, (hidden,), (hidden,))
         grads = [torch.empty(s, device=dev, dtype=dtype) if need else None
                  for s, need in zip(sizes, ctx.needs_input_grad)]
-        ws_bytes = L.gsr_gated_bwd_workspace(rows, dim, hidden, t)
+        ws_bytes = L.gsr_gated_workspace(rows, dim, hidden, t, 1)
         ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
         with _on(dev):
             check(L.gsr_gated_bwd(xr.data_ptr(), rows, dim, stride, t, wg.data_ptr(), wu.data_ptr(), hidden, _ptr(bg),

@@ -28,7 +28,7 @@ def _act(kind, g):
 
 def _reference(x, wg, wu, bg, bu, dh, kind, dtype):
     x, wg, wu, dh = (t.double() for t in (x, wg, wu, dh))
-    zero = torch.zeros(wg.shape[0], dtype=torch.float64)
+    zero = torch.zeros(wg.shape[0], dtype=torch.float64, device=x.device)
     bg, bu = (zero if b is None else b.double() for b in (bg, bu))
     c = lambda n: (n + 16) * U  # noqa: E731
     short = dtype != torch.float32
@@ -143,6 +143,42 @@ def test_layouts(cuda, kind, layout):
         _check(got.reshape(v.shape), v, t, f"{name} {kind} {layout}")
 
 
+WIDE = [(4096, 64, 1024), (4100, 72, 1025), (4097, 65, 1100), (8192, 200, 600), (300, 130, 8256), (4864, 512, 1030),
+        (2049, 320, 2000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,dim,hidden", WIDE)
+def test_large_cases(cuda, rows, dim, hidden, kind):
+    """The 256 x 256 tiles: whole and ragged tiles in every direction, dims that need padded copies."""
+    args, dh = _case(rows, dim, hidden, kind, rows % 2 == 0, rows + dim)
+    args[0] = args[0] * 2 ** -3   # (keeps fp16's sums over thousands of rows in range)
+    want, tol = _reference(*(None if t is None else t.to(cuda) for t in args), dh.to(cuda), "silu", TYPES[kind])
+    for name, got, v, t in zip(NAMES, _run(cuda, args, dh, "silu"), want, tol):
+        _check(got, v.cpu(), t.cpu(), f"{name} {rows}x{dim}->{hidden} {kind}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_large_views(cuda, kind):
+    """Large rows at odd addresses and inside wider buffers of NaN: nothing outside is read into a result."""
+    from gsr.layers import gated_linear
+    (x, wg, wu, _, _), dh = _case(4100, 72, 1032, kind, False, 8)
+    leaves = [t.to(cuda).requires_grad_(True) for t in (x, wg, wu)]
+    h = gated_linear(*leaves)
+    want = [h, *torch.autograd.grad(h, leaves, dh.to(cuda))]
+    for left, right in ((0, 8), (8, 0), (1, 2)):
+        def inside(t):
+            wide = torch.full((t.shape[0] + 1, left + t.shape[1] + right), float("nan"), device=cuda, dtype=t.dtype)
+            wide[:-1, left:left + t.shape[1]] = t.to(cuda)
+            return wide[:-1, left:left + t.shape[1]]
+        leaves = [t.detach().requires_grad_(True) for t in (inside(x), leaves[1], leaves[2])]
+        h = gated_linear(*leaves)
+        got = [h, *torch.autograd.grad(h, leaves, inside(dh))]
+        assert all(torch.equal(a, b) for a, b in zip(want, got)), (left, right)
+
+
 @pytest.mark.gpu
 def test_gradient_against_differences(cuda):
     """Central differences (h = 2^-5, arguments of size 1): curvature leaves h^2/6 of third derivatives of
@@ -166,7 +202,7 @@ def test_gradient_against_differences(cuda):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", list(TYPES))
-@pytest.mark.parametrize("rows,dim,hidden", [(70, 40, 72), (3, 64, 96), (300, 128, 300)])
+@pytest.mark.parametrize("rows,dim,hidden", [(70, 40, 72), (3, 64, 96), (300, 128, 300), (4096, 72, 1024)])
 def test_bad_rows_stay_alone(cuda, kind, rows, dim, hidden):
     """A NaN or infinite row reaches its own outputs and input gradient, and no other row's."""
     args, dh = _case(rows, dim, hidden, kind, False, 9)
@@ -194,7 +230,8 @@ def test_no_rows(cuda, kind):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,dim,hidden,kind", [(600, 200, 136, "bf16"), (2000, 8, 128, "f32"), (1, 512, 640, "bf16"),
-                                                  (1024, 512, 512, "bf16"), (1024, 256, 512, "f32")])
+                                                  (1024, 512, 512, "bf16"), (1024, 256, 512, "f32"),
+                                                  (4200, 136, 1000, "bf16"), (4100, 65, 1030, "f16")])
 def test_same_bits_streams_and_graph(cuda, rows, dim, hidden, kind):
     """Repeated calls, a call on another stream and a captured pass replayed with new inputs give the same bits."""
     from gsr.layers import gated_linear
@@ -340,7 +377,7 @@ def test_refusals():
         gated_linear(f(1, 1).expand(1 << 27, 1), f(1, 1), f(1, 1))
     L = _lib.lib()
     fwd = lambda rows=4, dim=8, stride=8, t=0, hidden=6, act=0: L.gsr_gated_fwd(  # noqa: E731
-        None, rows, dim, stride, t, None, None, hidden, None, None, act, None, None)
+        None, rows, dim, stride, t, None, None, hidden, None, None, act, None, None, 0, None)
     for kw, msg in [(dict(rows=-1), b"bad rows"), (dict(dim=0), b"bad dim"), (dict(hidden=0), b"bad dim"),
                     (dict(stride=7), b"row stride"), (dict(t=3), b"bad type"), (dict(act=4), b"bad activation"),
                     ({}, b"null pointer"), (dict(hidden=1 << 21), b"bad dim")]:
@@ -349,4 +386,5 @@ def test_refusals():
                                               None)
     assert bwd(1, 16) == -1 and b"workspace" in L.gsr_last_error()
     assert bwd(1, 1 << 20, dh=None) == -1 and b"null" in L.gsr_last_error()
-    assert L.gsr_gated_bwd_workspace(4, 8, 6, 0) >= 4 * 128 * 4 and L.gsr_gated_bwd_workspace(4, 8, 6, 7) == 0
+    assert L.gsr_gated_workspace(4, 8, 6, 0, 1) >= 4 * 128 * 4 and L.gsr_gated_workspace(4, 8, 6, 7, 1) == 0
+    assert L.gsr_gated_workspace(4, 8, 6, 1, 0) == 0
