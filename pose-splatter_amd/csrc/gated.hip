@@ -16,7 +16,12 @@
 // ones for fp32 (exact fp32 products), bf16/fp16 ones with fp32 sums.  A weight gradient's sum
 // over rows is split over workgroups where there are few tiles; the parts are joined in order.
 #include "gated.h"
+#include "gated_skinny.h"
 #include "gated_wide.h"
+
+#ifndef GSR_SIDE_RULE
+#define GSR_SIDE_RULE 1
+#endif
 
 namespace gsr {
 
@@ -108,7 +113,7 @@ __device__ __forceinline__ void tile_product(Operand<T> a, int64_t m0, int64_t M
 #pragma unroll
     for (int q = 0; q < NB; ++q) {
       const auto o = b_at(q, k);
-      tile_fetch<T, BKC>(o.op, n0, N, o.k, o.kend < k1 ? o.kend : k1, bv[q]);
+      tile_fetch<T, BKC>(o.op, n0, N, o.k, o.kend, bv[q]);
     }
   };
   if (k0 < k1) fetch(k0);
@@ -212,17 +217,20 @@ __global__ __launch_bounds__(256) void k_tile_gated(const T* x, int64_t x_stride
   }
 }
 
-// dx = [dg | du] [Wg; Wu]
+// dx = [dg | du] [Wg; Wu] over the columns of share blockIdx.z.  One share: into dx; more: fp32 parts
+// [share][rows][dim].
 template <typename T>
-__global__ __launch_bounds__(256) void k_tile_dx(const T* dgu, const T* wg, const T* wu, GatedShape s, T* dx) {
+__global__ __launch_bounds__(256) void k_tile_dx(const T* dgu, const T* wg, const T* wu, GatedShape s, int64_t share, T* dx,
+                                                 float* parts) {
   const int64_t m0 = (int64_t)blockIdx.x * 64, n0 = (int64_t)blockIdx.y * 64, pad = gated_pad(s.hidden);
+  const int64_t k0 = blockIdx.z * share, k1 = k0 + share < 2 * pad ? k0 + share : 2 * pad;
   v4f acc[1][2][2];
   tile_product<T, 1, true, false>(
       Operand<T>{dgu, 2 * pad}, m0, s.rows,
       [&](int, int64_t k) {
         return k < pad ? OperandAt<T>{Operand<T>{wg, s.dim}, k, s.hidden} : OperandAt<T>{Operand<T>{wu, s.dim}, k - pad, s.hidden};
       },
-      n0, s.dim, 0, 2 * pad, acc);
+      n0, s.dim, k0, k1, acc);
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
 #pragma unroll
   for (int nb = 0; nb < 2; ++nb)
@@ -232,7 +240,12 @@ __global__ __launch_bounds__(256) void k_tile_dx(const T* dgu, const T* wg, cons
       float v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = acc[0][nb][mb][i];
-      if (m < s.rows) store_upto(dx + m * s.dim + n, s.dim - n, v);
+      if (m >= s.rows) continue;
+      if (parts) {
+        store_upto(parts + (blockIdx.z * s.rows + m) * s.dim + n, s.dim - n, v);
+      } else {
+        store_upto(dx + m * s.dim + n, s.dim - n, v);
+      }
     }
 }
 
@@ -246,7 +259,7 @@ __global__ __launch_bounds__(256) void k_tile_dw(const T* dgu, const T* x, int64
   v4f acc[1][2][2];
   tile_product<T, 1, false, false>(
       Operand<T>{dgu, 2 * pad}, m0, 2 * pad,
-      [&](int, int64_t k) { return OperandAt<T>{Operand<T>{x, x_stride}, k, s.rows}; }, n0, s.dim, k0, k1, acc);
+      [&](int, int64_t k) { return OperandAt<T>{Operand<T>{x, x_stride}, k, k1}; }, n0, s.dim, k0, k1, acc);
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
 #pragma unroll
   for (int nb = 0; nb < 2; ++nb)
@@ -267,61 +280,77 @@ __global__ __launch_bounds__(256) void k_tile_dw(const T* dgu, const T* x, int64
     }
 }
 
-// a, b [n each] = the sum over `count` rows of parts [count][2][n], in order.
+// [a | b], a the first `split` of n values, = the sum over `count` rows of parts [count][n], in order.
 template <typename T>
-__global__ __launch_bounds__(256) void k_gated_join(const float* parts, int64_t count, int64_t n, T* a, T* b) {
+__global__ __launch_bounds__(256) void k_gated_join(const float* parts, int64_t count, int64_t n, int64_t split, T* a, T* b) {
   __shared__ float sum[4][64];
   const int lane = threadIdx.x % 64, grp = threadIdx.x / 64;
   const int64_t c = (int64_t)blockIdx.x * 64 + lane;
   float s = 0.f;
-  if (c < 2 * n)
-    for (int64_t r = grp; r < count; r += 4) s += parts[r * 2 * n + c];
+  if (c < n)
+    for (int64_t r = grp; r < count; r += 4) s += parts[r * n + c];
   sum[grp][lane] = s;
   __syncthreads();
-  if (grp == 0 && c < 2 * n) {
+  if (grp == 0 && c < n) {
     s = (sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane]);
-    if (c < n) {
+    if (c < split) {
       if (a) a[c] = from_f<T>(s);
     } else if (b) {
-      b[c - n] = from_f<T>(s);
+      b[c - split] = from_f<T>(s);
     }
   }
 }
 
-// Shares of the rows in a weight gradient of `tile` x `tile` tiles: enough workgroups for two 64 x 64
-// (one 256 x 256) tiles a CU, each share at least four tiles of rows, the parts at most 64 MB.
-static int64_t gated_shares(GatedShape s, int64_t tile) {
-  const int64_t tiles = ceil_div64(2 * gated_pad(s.hidden), tile) * ceil_div64(s.dim, tile);
-  int64_t n = (tile == 64 ? 512 : 256) / tiles;
-  n = n < s.rows / (4 * tile) ? n : s.rows / (4 * tile);
-  const int64_t most = (64 << 20) / (2 * s.hidden * s.dim * 4);
+template <typename T>
+static void gated_join(const float* parts, int64_t count, int64_t n, int64_t split, void* a, void* b, hipStream_t st) {
+  k_gated_join<T><<<(unsigned)ceil_div64(n, 64), 256, 0, st>>>(parts, count, n, split, (T*)a, (T*)b);
+}
+
+// Shares of K in a product of `tiles` tiles of side `tile`: enough workgroups for two a CU (one of side
+// 256), each share at least eight steps of 64, the fp32 parts of `values` results at most 64 MB.
+static int64_t gated_shares(int64_t tiles, int64_t tile, int64_t k, int64_t values) {
+  int64_t n = (tile == 256 ? 256 : 512) / tiles;
+  n = n < k / 512 ? n : k / 512;
+  const int64_t most = (64 << 20) / 4 / values;
   n = n < most ? n : most;
   return n < 1 ? 1 : n;
 }
 
-// to [rows][kdim] = p [rows][dim] (row stride `stride`) and zeros: rows that start at 16 bytes and
-// whose length is whole 16-byte pieces.
+// Padded copies of up to three matrices: to [rows][kdim] = p [rows][dim] (row stride `stride`) and
+// zeros, rows that start at 16 bytes and are whole 16-byte pieces.
 template <typename T>
-__global__ __launch_bounds__(256) void k_gated_pad(const T* p, int64_t rows, int64_t dim, int64_t stride, int64_t kdim, T* to) {
-  const int64_t per = kdim / 8, n = rows * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per, c = i % per * 8;
-    float v[8];
-    load_upto(p + r * stride + c, dim - c, v);
-    store_vec(to + r * kdim + c, v);
+struct GatedPads {
+  const T* p[3];
+  T* to[3];
+  int64_t rows[3], stride[3];   // rows 0: none
+  int64_t dim, kdim;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_pad(GatedPads<T> a) {
+  const int64_t per = a.kdim / 8;
+  int64_t first = 0;
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {   // one run of pieces through all three
+    const int64_t n = a.rows[q] * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < first + n; i += (int64_t)gridDim.x * 256) {
+      if (i < first) continue;
+      const int64_t r = (i - first) / per, c = (i - first) % per * 8;
+      float v[8];
+      load_upto(a.p[q] + r * a.stride[q] + c, a.dim - c, v);
+      store_vec(a.to[q] + r * a.kdim + c, v);
+    }
+    first += n;
   }
 }
 
-template <typename T>
-static const T* gated_padded(const T* p, int64_t rows, int64_t dim, int64_t stride, int64_t kdim, char* to, hipStream_t st) {
-  const int64_t blocks = ceil_div64(rows * (kdim / 8), 256);
-  k_gated_pad<T><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(p, rows, dim, stride, kdim, (T*)to);
-  return (const T*)to;
-}
-
-// Whether a case runs on the 256 x 256 tiles.
-static bool gated_is_wide(GatedShape s, int type) {
-  return type != GSR_F32 && ceil_div64(s.rows, 256) * ceil_div64(s.hidden, 128) >= 128 && s.dim >= 64;
+// Tile side of a 16-bit product of `rows` x `cols` outputs: 256 where its tiles fill most CUs, 128
+// where two a CU would be filled to half by the shares of K, 64 (any alignment, no padded copies) below.
+static int gated_side(int type, int64_t rows, int64_t cols, int64_t k, GatedShape s) {
+  if (type == GSR_F32 || s.dim < 64 || s.rows <= kSkinnyRows) return 64;
+  const int64_t wide = ceil_div64(rows, 256) * ceil_div64(cols, 256);
+  if (wide >= 192) return 256;
+  return GSR_SIDE_RULE ? 128 : 64;
 }
 
 // What a wide case's operands need: rows of whole 16-byte pieces at 16-byte addresses, 256 of them
@@ -330,116 +359,140 @@ static bool gated_aligned(const void* p, int64_t dim, int64_t stride) {
   return (uintptr_t)p % 16 == 0 && dim % 8 == 0 && stride % 8 == 0 && stride <= 1 << 21;
 }
 
-// Workspace of a pass, as byte offsets.  Padded copies only where a wide case's inputs need them
-// (an odd dim; a caller whose rows or addresses are odd is told by `copy_x`, `copy_w`).
-struct GatedSpace {
-  int64_t x, wg, wu, dgu, bias, shares, total;
-  int64_t kdim, n_shares;
+// How a pass is laid out: each product's tile side and shares of K, and its workspace (byte
+// offsets).  There is room for padded copies wherever a wide product may need them: an odd dim, rows
+// or addresses that are not multiples of 16 bytes.
+struct GatedPlan {
+  int fwd, dx, dw;               // tile sides
+  int64_t n_dx, n_dw;            // shares
+  int64_t kdim;                  // dim in whole 16-byte pieces
+  int64_t x, wg, wu, dgu, bias, bias_rows, dx_parts, dw_parts, total;
 };
 
-static GatedSpace gated_space(GatedShape s, int type, bool backward) {
-  const auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-  const bool wide = gated_is_wide(s, type);
-  GatedSpace w;
+static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
+  GatedPlan w;
+  const int64_t pad = gated_pad(s.hidden);
+  w.fwd = gated_side(type, s.rows, 2 * pad, s.dim, s);
+  w.dx = gated_side(type, s.rows, s.dim, 2 * pad, s);
+  w.dw = gated_side(type, 2 * pad, s.dim, s.rows, s);
   w.kdim = (s.dim + 7) / 8 * 8;
+  const auto tiles = [](int side, int64_t r, int64_t c) { return ceil_div64(r, side) * ceil_div64(c, side); };
+  w.n_dx = gated_shares(tiles(w.dx, s.rows, s.dim), w.dx, 2 * pad, s.rows * s.dim);
+  w.n_dw = gated_shares(tiles(w.dw, 2 * pad, s.dim), w.dw, s.rows, 2 * s.hidden * s.dim);
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
     const int64_t here = at;
-    at += up(bytes);
+    at += (bytes + 255) / 256 * 256;
     return here;
   };
-  w.x = take(wide ? s.rows * w.kdim * 2 : 0);
-  w.wg = take(wide ? s.hidden * w.kdim * 2 : 0);
-  w.wu = take(wide ? s.hidden * w.kdim * 2 : 0);
-  w.dgu = w.bias = w.shares = at;
-  w.n_shares = 1;
-  if (backward) {
-    w.dgu = take(s.rows * 2 * gated_pad(s.hidden) * (int64_t)type_size(type));
-    w.bias = take(wide ? ceil_div64(s.rows, 256) * 4 * s.hidden * 4 : ceil_div64(s.rows, 64) * 2 * s.hidden * 4);
-    w.n_shares = gated_shares(s, wide ? 256 : 64);
-    w.shares = take(w.n_shares > 1 ? w.n_shares * 2 * s.hidden * s.dim * 4 : 0);
-  }
+  const bool xw = w.fwd > 64 || (backward && w.dw > 64), ww = w.fwd > 64 || (backward && w.dx > 64);
+  w.x = take(xw ? s.rows * w.kdim * 2 : 0);
+  w.wg = take(ww ? s.hidden * w.kdim * 2 : 0);
+  w.wu = take(ww ? s.hidden * w.kdim * 2 : 0);
+  w.bias_rows = s.rows <= kSkinnyRows ? 1 : w.fwd > 64 ? ceil_div64(s.rows, w.fwd) * 2 : ceil_div64(s.rows, 64);
+  w.dgu = take(backward ? s.rows * 2 * pad * (int64_t)type_size(type) : 0);
+  w.bias = take(backward ? w.bias_rows * 2 * s.hidden * 4 : 0);
+  w.dx_parts = take(backward && w.n_dx > 1 ? w.n_dx * s.rows * s.dim * 4 : 0);
+  w.dw_parts = take(backward && w.n_dw > 1 ? w.n_dw * 2 * s.hidden * s.dim * 4 : 0);
   w.total = at;
   return w;
 }
 
+// The wide products' operands, copied into whole 16-byte pieces where they are not.
 template <typename T>
-static GatedWide gated_wide_args(const void* x, int64_t x_stride, const void* wg, const void* wu, const void* bg,
-                                 const void* bu, int act, GatedShape s, const GatedSpace& w, char* ws, hipStream_t st) {
+static GatedWide gated_wide_args(const T* x, int64_t x_stride, const T* wg, const T* wu, const void* bg, const void* bu, int act,
+                                 GatedShape s, const GatedPlan& w, bool use_x, bool use_w, char* ws, hipStream_t st) {
   GatedWide a{};
   a.s = s;
-  a.kdim = s.dim, a.x_stride = x_stride, a.w_stride = s.dim;
+  a.kdim = w.kdim, a.x_stride = x_stride, a.w_stride = s.dim;
   a.x = x, a.wg = wg, a.wu = wu, a.bg = bg, a.bu = bu, a.act = act;
-  if (!gated_aligned(x, s.dim, x_stride)) {
-    a.x = gated_padded((const T*)x, s.rows, s.dim, x_stride, w.kdim, ws + w.x, st);
-    a.x_stride = w.kdim;
+  GatedPads<T> p{};
+  p.dim = s.dim, p.kdim = w.kdim;
+  if (use_x && !gated_aligned(x, s.dim, x_stride)) {
+    p.p[0] = x, p.to[0] = (T*)(ws + w.x), p.rows[0] = s.rows, p.stride[0] = x_stride;
+    a.x = p.to[0], a.x_stride = w.kdim;
   }
-  if (!gated_aligned(wg, s.dim, s.dim) || !gated_aligned(wu, s.dim, s.dim)) {
-    a.wg = gated_padded((const T*)wg, s.hidden, s.dim, s.dim, w.kdim, ws + w.wg, st);
-    a.wu = gated_padded((const T*)wu, s.hidden, s.dim, s.dim, w.kdim, ws + w.wu, st);
-    a.w_stride = w.kdim;
+  if (use_w && !(gated_aligned(wg, s.dim, s.dim) && gated_aligned(wu, s.dim, s.dim))) {
+    p.p[1] = wg, p.to[1] = (T*)(ws + w.wg), p.rows[1] = s.hidden, p.stride[1] = s.dim;
+    p.p[2] = wu, p.to[2] = (T*)(ws + w.wu), p.rows[2] = s.hidden, p.stride[2] = s.dim;
+    a.wg = p.to[1], a.wu = p.to[2], a.w_stride = w.kdim;
   }
-  if (s.dim % 8) a.kdim = w.kdim;   // (then both were copied)
+  const int64_t pieces = (p.rows[0] + p.rows[1] + p.rows[2]) * (w.kdim / 8), blocks = ceil_div64(pieces, 256);
+  if (pieces) k_gated_pad<T><<<(unsigned)(blocks < 8192 ? blocks : 8192), 256, 0, st>>>(p);
   return a;
 }
 
 template <typename T>
-static void gated_fwd(const void* x, int64_t x_stride, const void* wg, const void* wu, const void* bg, const void* bu, int act,
-                      GatedShape s, void* h, char* ws, hipStream_t st) {
-  const int type = __is_same(T, float) ? GSR_F32 : __is_same(T, bf16) ? GSR_BF16 : GSR_F16;
-  if (gated_is_wide(s, type)) {
-    GatedWide a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, gated_space(s, type, false), ws, st);
-    a.h = h;
-    gated_wide(type, kWideFwd, a, 1, st);
-    return;
-  }
-  const dim3 grid((unsigned)ceil_div64(s.rows, 64), (unsigned)ceil_div64(s.hidden, 64));
-  k_tile_gated<T><<<grid, 256, 0, st>>>((const T*)x, x_stride, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, act, s,
-                                        (T*)h, nullptr, 0, nullptr, nullptr);
+static constexpr int type_of() {
+  return __is_same(T, float) ? GSR_F32 : __is_same(T, bf16) ? GSR_BF16 : GSR_F16;
 }
 
 template <typename T>
-static void gated_bwd(const void* x, int64_t x_stride, const void* wg, const void* wu, const void* bg, const void* bu, int act,
-                      GatedShape s, const void* dh, int64_t dh_stride, void* dx, void* dwg, void* dwu, void* dbg, void* dbu,
-                      char* ws, hipStream_t st) {
-  const int type = __is_same(T, float) ? GSR_F32 : __is_same(T, bf16) ? GSR_BF16 : GSR_F16;
-  const GatedSpace w = gated_space(s, type, true);
-  const bool wide = gated_is_wide(s, type);
-  const int64_t rb = ceil_div64(s.rows, 64), pad = gated_pad(s.hidden), n = w.n_shares;
+static void gated_fwd(const T* x, int64_t x_stride, const T* wg, const T* wu, const T* bg, const T* bu, int act, GatedShape s,
+                      T* h, char* ws, hipStream_t st) {
+  const int type = type_of<T>();
+  if (s.rows <= kSkinnyRows) {
+    gated_skinny(type, GatedSkinny{s, x, wg, wu, bg, bu, nullptr, x_stride, 0, h, nullptr, nullptr, act}, st);
+    return;
+  }
+  const GatedPlan w = gated_plan(s, type, false);
+  if (w.fwd > 64) {
+    GatedWide a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, true, true, ws, st);
+    a.h = h;
+    gated_wide(type, kWideFwd, w.fwd, a, 1, st);
+    return;
+  }
+  const dim3 grid((unsigned)ceil_div64(s.rows, 64), (unsigned)ceil_div64(s.hidden, 64));
+  k_tile_gated<T><<<grid, 256, 0, st>>>(x, x_stride, wg, wu, bg, bu, act, s, h, nullptr, 0, nullptr, nullptr);
+}
+
+template <typename T>
+static void gated_bwd(const T* x, int64_t x_stride, const T* wg, const T* wu, const T* bg, const T* bu, int act, GatedShape s,
+                      const T* dh, int64_t dh_stride, T* dx, T* dwg, T* dwu, T* dbg, T* dbu, char* ws, hipStream_t st) {
+  const int type = type_of<T>();
+  const GatedPlan w = gated_plan(s, type, true);
+  const int64_t rb = ceil_div64(s.rows, 64), db = ceil_div64(s.dim, 64), pad = gated_pad(s.hidden);
+  const bool weights = dwg || dwu, few = s.rows <= kSkinnyRows;
   T* dgu = (T*)(ws + w.dgu);
   float* bias = dbg || dbu ? (float*)(ws + w.bias) : nullptr;
-  float* parts = n > 1 ? (float*)(ws + w.shares) : nullptr;
   GatedWide a{};
-  if (wide) {
-    a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, ws, st);
-    a.dh = dh, a.dh_stride = dh_stride, a.dgu = dgu, a.dx = dx, a.dwg = dwg, a.dwu = dwu, a.parts = bias;
-    gated_wide(type, kWideGrad, a, 1, st);
+  if (w.fwd > 64 || w.dx > 64 || w.dw > 64) {
+    a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, w.fwd > 64 || (weights && w.dw > 64),
+                           w.fwd > 64 || (dx && w.dx > 64), ws, st);
+    a.dh = dh, a.dh_stride = dh_stride, a.dgu = dgu, a.dx = dx, a.dwg = dwg, a.dwu = dwu;
+  }
+  if (few) {
+    gated_skinny(type, GatedSkinny{s, x, wg, wu, bg, bu, dh, x_stride, dh_stride, nullptr, dgu, bias, act}, st);
+  } else if (w.fwd > 64) {
+    a.parts = bias;
+    gated_wide(type, kWideGrad, w.fwd, a, 1, st);
   } else {
-    k_tile_gated<T><<<dim3((unsigned)rb, (unsigned)(pad / 64)), 256, 0, st>>>(
-        (const T*)x, x_stride, (const T*)wg, (const T*)wu, (const T*)bg, (const T*)bu, act, s, nullptr, (const T*)dh,
-        dh_stride, dgu, bias);
+    k_tile_gated<T><<<dim3((unsigned)rb, (unsigned)(pad / 64)), 256, 0, st>>>(x, x_stride, wg, wu, bg, bu, act, s, nullptr, dh,
+                                                                            dh_stride, dgu, bias);
   }
-  if (bias)
-    k_gated_join<T><<<(unsigned)ceil_div64(2 * s.hidden, 64), 256, 0, st>>>(bias, wide ? ceil_div64(s.rows, 256) * 2 : rb,
-                                                                          s.hidden, (T*)dbg, (T*)dbu);
-  if (dx && wide) {
-    gated_wide(type, kWideDx, a, 1, st);
-  } else if (dx) {
-    k_tile_dx<T><<<dim3((unsigned)rb, (unsigned)ceil_div64(s.dim, 64)), 256, 0, st>>>(dgu, (const T*)wg, (const T*)wu, s,
-                                                                                      (T*)dx);
-  }
-  if (dwg || dwu) {
-    const int64_t share = ceil_div64(ceil_div64(s.rows, n), 64) * 64;
-    if (wide) {
+  if (bias) gated_join<T>(bias, w.bias_rows, 2 * s.hidden, s.hidden, dbg, dbu, st);
+  if (dx) {
+    const int64_t n = w.n_dx, share = ceil_div64(ceil_div64(2 * pad, n), 64) * 64;
+    float* parts = n > 1 ? (float*)(ws + w.dx_parts) : nullptr;
+    if (w.dx > 64) {
       a.share = share, a.parts = parts;
-      gated_wide(type, kWideDw, a, (int)n, st);
+      gated_wide(type, kWideDx, w.dx, a, (int)n, st);
     } else {
-      const dim3 grid((unsigned)(2 * pad / 64), (unsigned)ceil_div64(s.dim, 64), (unsigned)n);
-      k_tile_dw<T><<<grid, 256, 0, st>>>(dgu, (const T*)x, x_stride, s, share, (T*)dwg, (T*)dwu, parts);
+      k_tile_dx<T><<<dim3((unsigned)rb, (unsigned)db, (unsigned)n), 256, 0, st>>>(dgu, wg, wu, s, share, dx, parts);
     }
-    if (parts)
-      k_gated_join<T><<<(unsigned)ceil_div64(2 * s.hidden * s.dim, 64), 256, 0, st>>>(parts, n, s.hidden * s.dim, (T*)dwg,
-                                                                                    (T*)dwu);
+    if (parts) gated_join<T>(parts, n, s.rows * s.dim, s.rows * s.dim, dx, nullptr, st);
+  }
+  if (weights) {
+    const int64_t n = w.n_dw, share = ceil_div64(ceil_div64(s.rows, n), 64) * 64;
+    float* parts = n > 1 ? (float*)(ws + w.dw_parts) : nullptr;
+    if (w.dw > 64) {
+      a.share = share, a.parts = parts;
+      gated_wide(type, kWideDw, w.dw, a, (int)n, st);
+    } else {
+      k_tile_dw<T><<<dim3((unsigned)(2 * pad / 64), (unsigned)db, (unsigned)n), 256, 0, st>>>(dgu, x, x_stride, s, share, dwg,
+                                                                                              dwu, parts);
+    }
+    if (parts) gated_join<T>(parts, n, 2 * s.hidden * s.dim, s.hidden * s.dim, dwg, dwu, st);
   }
 }
 
@@ -460,8 +513,8 @@ using namespace gsr;
 
 extern "C" size_t gsr_gated_workspace(int64_t rows, int64_t dim, int64_t hidden, int32_t type, int32_t backward) {
   const GatedShape s{rows, dim, hidden};
-  if (gated_check("gsr_gated_workspace", s, dim, type, GSR_ACT_SILU)) return 0;
-  return (size_t)gated_space(s, type, backward != 0).total;
+  if (gated_check("gsr_gated_workspace", s, dim, type, GSR_ACT_SILU) || rows == 0) return 0;
+  return (size_t)gated_plan(s, type, backward != 0).total;
 }
 
 extern "C" int gsr_gated_fwd(const void* x, int64_t rows, int64_t dim, int64_t x_stride, int32_t type, const void* wg,
@@ -476,11 +529,11 @@ extern "C" int gsr_gated_fwd(const void* x, int64_t rows, int64_t dim, int64_t x
   char* ws = (char*)workspace;
   const auto st = (hipStream_t)stream;
   if (type == GSR_F32) {
-    gated_fwd<float>(x, x_stride, wg, wu, bg, bu, act, s, h, ws, st);
+    gated_fwd((const float*)x, x_stride, (const float*)wg, (const float*)wu, (const float*)bg, (const float*)bu, act, s, (float*)h, ws, st);
   } else if (type == GSR_BF16) {
-    gated_fwd<bf16>(x, x_stride, wg, wu, bg, bu, act, s, h, ws, st);
+    gated_fwd((const bf16*)x, x_stride, (const bf16*)wg, (const bf16*)wu, (const bf16*)bg, (const bf16*)bu, act, s, (bf16*)h, ws, st);
   } else {
-    gated_fwd<f16>(x, x_stride, wg, wu, bg, bu, act, s, h, ws, st);
+    gated_fwd((const f16*)x, x_stride, (const f16*)wg, (const f16*)wu, (const f16*)bg, (const f16*)bu, act, s, (f16*)h, ws, st);
   }
   GSR_LAUNCH_CHECK("gsr_gated_fwd");
   return 0;
@@ -500,7 +553,7 @@ extern "C" int gsr_gated_bwd(const void* x, int64_t rows, int64_t dim, int64_t x
   char* ws = (char*)workspace;
   if (rows == 0) {   // sums over no rows
     const auto zero = [&](void* p, int64_t n) {
-      if (p) k_gated_join<bf16><<<(unsigned)ceil_div64(2 * n, 64), 256, 0, st>>>(nullptr, 0, n, (bf16*)p, nullptr);
+      if (p) gated_join<bf16>(nullptr, 0, n, n, p, nullptr, st);
     };
     const int64_t each = type == GSR_F32 ? 2 : 1;   // zeros of any type, 16 bits at a time
     zero(dwg, hidden * dim * each);
@@ -508,11 +561,14 @@ extern "C" int gsr_gated_bwd(const void* x, int64_t rows, int64_t dim, int64_t x
     zero(dbg, hidden * each);
     zero(dbu, hidden * each);
   } else if (type == GSR_F32) {
-    gated_bwd<float>(x, x_stride, wg, wu, bg, bu, act, s, dh, dh_stride, dx, dwg, dwu, dbg, dbu, ws, st);
+    gated_bwd((const float*)x, x_stride, (const float*)wg, (const float*)wu, (const float*)bg, (const float*)bu, act, s, (const float*)dh,
+              dh_stride, (float*)dx, (float*)dwg, (float*)dwu, (float*)dbg, (float*)dbu, ws, st);
   } else if (type == GSR_BF16) {
-    gated_bwd<bf16>(x, x_stride, wg, wu, bg, bu, act, s, dh, dh_stride, dx, dwg, dwu, dbg, dbu, ws, st);
+    gated_bwd((const bf16*)x, x_stride, (const bf16*)wg, (const bf16*)wu, (const bf16*)bg, (const bf16*)bu, act, s, (const bf16*)dh,
+              dh_stride, (bf16*)dx, (bf16*)dwg, (bf16*)dwu, (bf16*)dbg, (bf16*)dbu, ws, st);
   } else {
-    gated_bwd<f16>(x, x_stride, wg, wu, bg, bu, act, s, dh, dh_stride, dx, dwg, dwu, dbg, dbu, ws, st);
+    gated_bwd((const f16*)x, x_stride, (const f16*)wg, (const f16*)wu, (const f16*)bg, (const f16*)bu, act, s, (const f16*)dh,
+              dh_stride, (f16*)dx, (f16*)dwg, (f16*)dwu, (f16*)dbg, (f16*)dbu, ws, st);
   }
   GSR_LAUNCH_CHECK("gsr_gated_bwd");
   return 0;

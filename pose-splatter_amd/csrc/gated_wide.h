@@ -1,4 +1,4 @@
-// Launch of the gated block's 256 x 256 products (gated_wide.hip).
+// Launch of the gated block's products on square tiles of 256 or 128 (gated_wide.hip).
 #pragma once
 
 #include "gated.h"
@@ -14,11 +14,12 @@ struct GatedWide {
   int64_t kdim, x_stride, w_stride, dh_stride;
   const void *x, *wg, *wu, *bg, *bu, *dh;
   void *h, *dgu, *dx, *dwg, *dwu;
-  float* parts;    // gradients: column sums [ceil(rows / 256) * 2][2][hidden]; dW: [share][2][hidden][dim]; or NULL
-  int64_t share;   // dW: rows of x a share, a multiple of 64
+  float* parts;    // gradients: column sums [ceil(rows / side) * 2][2][hidden]; dx: [share][rows][dim]; dW:
+                   // [share][2][hidden][dim]; or NULL
+  int64_t share;   // dx: columns of dgu a share; dW: rows of x a share; multiples of 64
   int act, mt, nt;
 };
 
-void gated_wide(int type, int mode, GatedWide a, int shares, hipStream_t st);
+void gated_wide(int type, int mode, int side, GatedWide a, int shares, hipStream_t st);
 
 }  // namespace gsr

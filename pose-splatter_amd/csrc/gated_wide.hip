@@ -1,8 +1,8 @@
-// The gated block's products in 16 bits with 256 x 256 tiles (wide.h has the main loop's layout).
+// The gated block's products in 16 bits with square tiles of 256 or 128 (wide.h has the layout).
 //
-//   forward, gradients  a tile is 256 rows by 128 columns of g and the same 128 of u (shared memory
-//                       rows 0..127 from Wg, 128..255 from Wu), so a wave holds both projections of
-//                       its outputs and the activation joins them in registers
+//   forward, gradients  a tile is 256 (128) rows by half as many columns of g and the same columns of u
+//                       (the first half of its shared memory's rows from Wg, the second from Wu), so
+//                       a wave holds both projections of its outputs and the activation joins them
 //   dx                  K runs through [dg | du], its other operand through Wg, then Wu
 //   dWg, dWu            rows are the columns of [dg | du], K the rows of x
 #include "gated_wide.h"
@@ -11,20 +11,21 @@
 
 namespace gsr {
 
-template <typename T, int MODE>
-__global__ __launch_bounds__(kWideThreads, 1) void k_wide(GatedWide a) {
+template <typename T, int MODE, int SIDE>
+__global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(GatedWide a) {
   constexpr bool DUAL = MODE == kWideFwd || MODE == kWideGrad, AKC = MODE != kWideDw, BKC = DUAL;
-  __shared__ __attribute__((aligned(1024))) char lds[2][2][32768];   // [buffer][operand]
+  constexpr int NB = SIDE / 64, HALF = SIDE / 2, BYTES = SIDE * kWideK * 2;   // blocks a wave and side; its rows
+  __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];   // [buffer][operand]
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wm = wave % 2, wn = wave / 2;
   const GatedShape s = a.s;
   const int64_t pad = gated_pad(s.hidden);
   int tm, tn;
   wide_tile_of(blockIdx.x, a.mt, a.nt, &tm, &tn);
-  const int64_t m0 = (int64_t)tm * 256, n0 = (int64_t)tn * (DUAL ? 128 : 256);
+  const int64_t m0 = (int64_t)tm * SIDE, n0 = (int64_t)tn * (DUAL ? HALF : SIDE);
 
   // K of this workgroup, and the operands' first bytes
   int64_t k0 = 0, k1 = DUAL ? a.kdim : MODE == kWideDx ? 2 * pad : s.rows;
-  if constexpr (MODE == kWideDw) {
+  if constexpr (!DUAL) {
     k0 = blockIdx.z * a.share;
     k1 = k0 + a.share < k1 ? k0 + a.share : k1;
   }
@@ -40,8 +41,9 @@ __global__ __launch_bounds__(kWideThreads, 1) void k_wide(GatedWide a) {
     a_step = b_step = kWideK * 2;
   } else if constexpr (MODE == kWideDx) {
     a_stride = 2 * pad, b_stride = a.w_stride;
-    sa = from(a.dgu, m0 * a_stride, s.rows * a_stride);
-    sb = from(a.wg, n0, (s.hidden - 1) * b_stride + a.kdim);
+    sa = from(a.dgu, m0 * a_stride + k0, s.rows * a_stride);
+    const int64_t kw = k0 < pad ? k0 : k0 - pad;   // (pad is whole steps: none straddles Wg and Wu)
+    sb = from(k0 < pad ? a.wg : a.wu, kw * b_stride + n0, (s.hidden - 1) * b_stride + a.kdim);
     sb2 = from(a.wu, n0, (s.hidden - 1) * b_stride + a.kdim);
     a_step = kWideK * 2, b_step = kWideK * b_stride * 2;
   } else {
@@ -50,10 +52,10 @@ __global__ __launch_bounds__(kWideThreads, 1) void k_wide(GatedWide a) {
     sb = from(a.x, k0 * b_stride + n0, (k1 - 1) * b_stride + a.kdim);
     a_step = kWideK * a_stride * 2, b_step = kWideK * b_stride * 2;
   }
-  WideTile<AKC> ta;
-  WideTile<BKC> tb;
-  ta.init(a_stride * 2, wm * 128);
-  tb.init(b_stride * 2, DUAL ? wn * 64 : wn * 128);
+  WideTile<AKC, SIDE> ta;
+  WideTile<BKC, SIDE> tb;
+  ta.init(a_stride * 2, wm * HALF);
+  tb.init(b_stride * 2, DUAL ? wn * (HALF / 2) : wn * HALF);
 
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0][0];
   int64_t left = k1 - k0;   // K left at the next tile's start
@@ -64,14 +66,15 @@ __global__ __launch_bounds__(kWideThreads, 1) void k_wide(GatedWide a) {
     db = sb.descriptor(next < steps);
     if constexpr (DUAL) db2 = sb2.descriptor(next < steps);
   };
-  const auto load = [&](int i, int buf) {   // one of 16
-    const uint32_t to = lds0 + buf * 65536;
-    if (i < 8) {
+  constexpr int LOADS = SIDE / 32;
+  const auto load = [&](int i, int buf) {   // one of 2 LOADS
+    const uint32_t to = lds0 + buf * 2 * BYTES;
+    if (i < LOADS) {
       ta.load(da, to, i, i, left);
-    } else if (DUAL && i >= 12) {
-      tb.load(db2, to + 32768, i - 8, i - 12, left);
+    } else if (DUAL && i >= LOADS * 3 / 2) {
+      tb.load(db2, to + BYTES, i - LOADS, i - LOADS * 3 / 2, left);
     } else {
-      tb.load(db, to + 32768, i - 8, i - 8, left);
+      tb.load(db, to + BYTES, i - LOADS, i - LOADS, left);
     }
   };
   const auto end = [&]() {
@@ -81,31 +84,31 @@ __global__ __launch_bounds__(kWideThreads, 1) void k_wide(GatedWide a) {
     left -= kWideK;
     ++next;
     if constexpr (MODE == kWideDx)
-      if (next == pad / kWideK) sb = sb2;
+      if (k0 + (int64_t)next * kWideK == pad) sb = sb2;
   };
 
-  v16f acc[4][4];   // [n block][m block]
+  v16f acc[NB][NB];   // [n block][m block]
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
+  for (int i = 0; i < NB * NB; ++i)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) acc[i / 4][i % 4][j] = 0.f;
-  v8s fa[2][4], fb[2][4];
+    for (int j = 0; j < 16; ++j) acc[i / NB][i % NB][j] = 0.f;
+  v8s fa[2][NB], fb[2][NB];
   const auto operands = [&](int buf, int kk, int set) {
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
+    for (int b = 0; b < NB; ++b) {
       fa[set][b] = ta.operand(lds[buf][0], b * 32, kk);
-      fb[set][b] = tb.operand(lds[buf][1], DUAL && b >= 2 ? 64 + b * 32 : b * 32, kk);
+      fb[set][b] = tb.operand(lds[buf][1], DUAL && b >= NB / 2 ? HALF + (b - NB / 2) * 32 : b * 32, kk);
     }
   };
   const auto mma = [&](int set, int i) {
-    acc[i / 4][i % 4] = wide_mma<T>(fb[set][i / 4], fa[set][i % 4], acc[i / 4][i % 4]);
+    acc[i / NB][i % NB] = wide_mma<T>(fb[set][i / NB], fa[set][i % NB], acc[i / NB][i % NB]);
   };
 
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
     begin();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) load(i, b);
+    for (int i = 0; i < 2 * LOADS; ++i) load(i, b);
     end();
   }
   wide_wait();
@@ -118,7 +121,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void k_wide(GatedWide a) {
       operands(buf, kk + 1, (kk + 1) & 1);   // in flight over the products (the scheduler would sink them)
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mma(kk & 1, i);
+      for (int i = 0; i < NB * NB; ++i) mma(kk & 1, i);
     }
     // The last operands of this buffer are in registers and the next buffer's loads, a step old,
     // have landed: for every wave, after the barrier.
@@ -128,39 +131,41 @@ __global__ __launch_bounds__(kWideThreads, 1) void k_wide(GatedWide a) {
     operands(buf ^ 1, 0, 0);
     begin();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {   // a load behind each product, rather than sixteen in a row
+    for (int i = 0; i < NB * NB; ++i) {   // loads between the products, rather than all in a row
       __builtin_amdgcn_sched_barrier(0);
-      load(i, buf);
+#pragma unroll
+      for (int j = 0; j < 2 * LOADS / (NB * NB); ++j) load(i * (2 * LOADS / (NB * NB)) + j, buf);
       mma(1, i);
     }
     end();
   }
 
-  // Each wave passes its sums, 32 rows of 128 at a time, through its own quarter of the shared memory
+  // Each wave passes its sums, 32 rows of a block row at a time, through its own part of the shared memory
   // (no wave reads a tile any more after the barrier): there a lane takes eight neighbouring columns,
   // so that rows are read and written in whole lines.
   wide_wait();   // (the loads past K's end write zeros)
   __syncthreads();
-  float* mine = (float*)&lds[0][0][0] + wave * 8192;
-  constexpr int LD = 132;   // floats a row: 128 and 4 to spread the banks
-  constexpr int LANES = DUAL ? 8 : 16, ROWS = 64 / LANES;   // lanes a row, rows a pass
+  constexpr int LD = HALF + 4;   // floats a row: a wave's columns and 4 to spread the banks
+  static_assert(4 * 32 * LD * sizeof(float) <= sizeof(lds), "the waves' rows fit the tiles' memory");
+  float* mine = (float*)&lds[0][0][0] + wave * 32 * LD;
+  constexpr int COLS = DUAL ? HALF / 2 : HALF, LANES = COLS / 8, ROWS = 64 / LANES;   // lanes a row, rows a pass
   const int c = lane % LANES * 8;
-  const int64_t n = n0 + (DUAL ? wn * 64 : wn * 128) + c, left_n = (DUAL ? s.hidden : s.dim) - n;
+  const int64_t n = n0 + wn * COLS + c, left_n = (DUAL ? s.hidden : s.dim) - n;
   float gb[8] = {}, ub[8] = {}, sg[8] = {}, su[8] = {};
   if constexpr (DUAL) {
     load_upto((const T*)a.bg + n, a.bg ? left_n : 0, gb);
     load_upto((const T*)a.bu + n, a.bu ? left_n : 0, ub);
   }
 #pragma unroll
-  for (int mb = 0; mb < 4; ++mb) {
+  for (int mb = 0; mb < NB; ++mb) {
 #pragma unroll
-    for (int nb = 0; nb < 4; ++nb)   // a lane holds row lane % 32, columns 8 q + 4 (lane / 32) + 0..3 of a block
+    for (int nb = 0; nb < NB; ++nb)   // a lane holds row lane % 32, columns 8 q + 4 (lane / 32) + 0..3 of a block
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         *(v4f*)(mine + lane % 32 * LD + nb * 32 + q * 8 + lane / 32 * 4) =
             v4f{acc[nb][mb][q * 4], acc[nb][mb][q * 4 + 1], acc[nb][mb][q * 4 + 2], acc[nb][mb][q * 4 + 3]};
     wide_fence();
-    const int64_t first = m0 + wm * 128 + mb * 32;
+    const int64_t first = m0 + wm * HALF + mb * 32;
 #pragma unroll 1
     for (int r = lane / LANES; r < 32; r += ROWS) {
       const int64_t m = first + r;
@@ -169,7 +174,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void k_wide(GatedWide a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         g[i] = mine[r * LD + c + i];
-        if constexpr (DUAL) u[i] = mine[r * LD + 64 + c + i];
+        if constexpr (DUAL) u[i] = mine[r * LD + COLS + c + i];
       }
       if constexpr (DUAL) {
         if constexpr (MODE == kWideGrad) load_upto((const T*)a.dh + m * a.dh_stride + n, left_n, d);
@@ -197,7 +202,11 @@ __global__ __launch_bounds__(kWideThreads, 1) void k_wide(GatedWide a) {
           store_vec((T*)a.dgu + m * 2 * pad + pad + n, u);
         }
       } else if constexpr (MODE == kWideDx) {
-        store_upto((T*)a.dx + m * s.dim + n, left_n, g);
+        if (a.parts) {
+          store_upto(a.parts + (blockIdx.z * s.rows + m) * s.dim + n, left_n, g);
+        } else {
+          store_upto((T*)a.dx + m * s.dim + n, left_n, g);
+        }
       } else {
         const int which = m >= pad;
         const int64_t row = m - which * pad;
@@ -212,15 +221,15 @@ __global__ __launch_bounds__(kWideThreads, 1) void k_wide(GatedWide a) {
     }
     wide_fence();
   }
-  if (MODE == kWideGrad && a.parts) {   // column sums of the wave's 128 rows
+  if (MODE == kWideGrad && a.parts) {   // column sums of the wave's rows
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
 #pragma unroll
-      for (int d = 8; d < 64; d <<= 1) {
+      for (int d = LANES; d < 64; d <<= 1) {
         sg[i] += __shfl_xor(sg[i], d);
         su[i] += __shfl_xor(su[i], d);
       }
-      if (lane < 8 && i < left_n) {
+      if (lane < LANES && i < left_n) {
         float* to = a.parts + (int64_t)(tm * 2 + wm) * 2 * s.hidden + n + i;
         to[0] = sg[i];
         to[s.hidden] = su[i];
@@ -229,28 +238,32 @@ __global__ __launch_bounds__(kWideThreads, 1) void k_wide(GatedWide a) {
   }
 }
 
-template <typename T>
+template <typename T, int SIDE>
 static void wide_launch(int mode, const GatedWide& a, int shares, hipStream_t st) {
   const dim3 grid((unsigned)(a.mt * a.nt), 1, (unsigned)shares);
   if (mode == kWideFwd) {
-    k_wide<T, kWideFwd><<<grid, kWideThreads, 0, st>>>(a);
+    k_wide<T, kWideFwd, SIDE><<<grid, kWideThreads, 0, st>>>(a);
   } else if (mode == kWideGrad) {
-    k_wide<T, kWideGrad><<<grid, kWideThreads, 0, st>>>(a);
+    k_wide<T, kWideGrad, SIDE><<<grid, kWideThreads, 0, st>>>(a);
   } else if (mode == kWideDx) {
-    k_wide<T, kWideDx><<<grid, kWideThreads, 0, st>>>(a);
+    k_wide<T, kWideDx, SIDE><<<grid, kWideThreads, 0, st>>>(a);
   } else {
-    k_wide<T, kWideDw><<<grid, kWideThreads, 0, st>>>(a);
+    k_wide<T, kWideDw, SIDE><<<grid, kWideThreads, 0, st>>>(a);
   }
 }
 
-void gated_wide(int type, int mode, GatedWide a, int shares, hipStream_t st) {
+void gated_wide(int type, int mode, int side, GatedWide a, int shares, hipStream_t st) {
   const int64_t pad = gated_pad(a.s.hidden);
-  a.mt = ceil_div(mode == kWideDw ? 2 * pad : a.s.rows, 256);
-  a.nt = mode <= kWideGrad ? ceil_div(pad, 128) : ceil_div(a.s.dim, 256);
-  if (type == GSR_BF16) {
-    wide_launch<bf16>(mode, a, shares, st);
+  a.mt = ceil_div(mode == kWideDw ? 2 * pad : a.s.rows, side);
+  a.nt = mode <= kWideGrad ? ceil_div(pad, side / 2) : ceil_div(a.s.dim, side);
+  if (type == GSR_BF16 && side == 256) {
+    wide_launch<bf16, 256>(mode, a, shares, st);
+  } else if (type == GSR_BF16) {
+    wide_launch<bf16, 128>(mode, a, shares, st);
+  } else if (side == 256) {
+    wide_launch<f16, 256>(mode, a, shares, st);
   } else {
-    wide_launch<f16>(mode, a, shares, st);
+    wide_launch<f16, 128>(mode, a, shares, st);
   }
 }
 

@@ -1,17 +1,19 @@
-// 256 x 256 products of 16-bit matrices with fp32 sums: the main loop of the gated block's large cases.
+// Products of 16-bit matrices with fp32 sums in square tiles of 256 or 128: the parts of the gated
+// block's main loop.
 //
 // A workgroup of four waves owns a 256 x 256 tile, each wave a 128 x 128 quarter of 4 x 4 blocks
 // of 32x32x16 matrix instructions: 256 accumulators a lane.  K advances 64 at a time through two
 // buffers of shared memory (2 x 64 KB).  A quarter that large reads 2 x 128 x 64 elements for
 // 128 x 128 x 64 multiply-adds, 64 bytes of shared memory a cycle and CU at full matrix rate
 // where 128 are available; eight waves of 128 x 64 would need 96 and leave none for the stores.
+// 128 x 128 tiles (2 x 2 blocks a wave, two workgroups a CU) are for products of fewer tiles than CUs.
 //
 // Tiles come straight from global memory into shared memory (16 bytes a lane, no registers).  Each
 // operand is read in the order it lies in memory:
 //   K contiguous     rows of 64 K (128 bytes); 16-byte chunk c of row r sits in slot c ^ (r % 8),
 //                    so the 16-byte reads of eight neighbouring rows hit different banks
-//   K across rows    rows of 256 columns (512 bytes) a K; chunk c of row k sits in slot
-//                    c ^ (2 (k % 4) + 8 (k / 8 % 4)); ds_read_b64_tr_b16 turns 4 K x 16 columns
+//   K across rows    rows of 256 (128) columns a K; chunk c of row k sits in slot
+//                    c ^ (2 (k % 4) + 8 (k / 8 % 4 (% 2))); ds_read_b64_tr_b16 turns 4 K x 16 columns
 //                    into the instruction's K-contiguous operand on the way out
 // The pattern is made by choosing what each lane loads: shared memory itself is filled in lane
 // order.  Loads past an operand's end return zeros (the buffer descriptor's bound), so no tile
@@ -22,7 +24,7 @@
 
 namespace gsr {
 
-constexpr int kWideTile = 256, kWideK = 64, kWideThreads = 256;
+constexpr int kWideK = 64, kWideThreads = 256;
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -74,56 +76,62 @@ __device__ __forceinline__ void wide_fence() {
 
 constexpr uint32_t kWideNowhere = 0x80000000u;   // past every descriptor's end
 
-// One operand's tile: this lane's places in it.
-template <bool KC>
+// One operand's tile of SIDE rows (KC) or columns: this lane's places in it.
+template <bool KC, int SIDE>
 struct WideTile {
-  uint32_t at[8];       // byte offsets of the lane's eight loads from the tile's corner
+  static constexpr int LOADS = SIDE / 32, BYTES = SIDE * kWideK * 2, BLOCKS = SIDE / 64;
+  static constexpr int ROW = SIDE * 2;   // bytes of a K row (K across rows)
+  uint32_t at[LOADS];   // byte offsets of the lane's loads from the tile's corner
   int k;                // KC: the loads' first K
-  uint32_t read[KC ? 4 : 8];   // byte offsets of its reads: per 16 K (KC), or per block and K parity
+  uint32_t read[KC ? 4 : 2 * BLOCKS];   // byte offsets of its reads: per 16 K (KC), or per K parity and block
 
-  // origin: the wave's first row (KC) or column of the tile's 256
+  // origin: the wave's first row (KC) or column of the tile's
   __device__ __forceinline__ void init(int64_t stride_bytes, int origin) {
     const int t = threadIdx.x, l = t % 64;
     if constexpr (KC) {
       const int c = t % 8 ^ (t / 8 & 7);
       k = c * 8;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) at[j] = (uint32_t)((j * 32 + t / 8) * stride_bytes + c * 16);
+      for (int j = 0; j < LOADS; ++j) at[j] = (uint32_t)((j * 32 + t / 8) * stride_bytes + c * 16);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) read[kk] = (origin + l % 32) * 128 + ((kk * 2 + l / 32) ^ (l & 7)) * 16;
     } else {
+      constexpr int SLOTS = ROW / 16, EACH = 256 / SLOTS;   // 16-byte slots a K row, K rows a load
+      constexpr int MASK = SIDE == 256 ? 3 : 1;
       k = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        at[j] = (uint32_t)((j * 8 + t / 32) * stride_bytes + (t % 32 ^ (t / 32 & 3) * 2 ^ (j & 3) * 8) * 16);
+      for (int j = 0; j < LOADS; ++j) {
+        const int kr = j * EACH + t / SLOTS;
+        at[j] = (uint32_t)(kr * stride_bytes + (t % SLOTS ^ (kr & 3) * 2 ^ (kr >> 3 & MASK) * 8) * 16);
+      }
       const int g = l / 16, row = l % 16 / 4;   // K row of the lane's 4 x 16 piece
 #pragma unroll
       for (int p = 0; p < 2; ++p)
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < BLOCKS; ++b) {
           const int c = origin / 8 + b * 4 + g % 2 * 2 + l % 4 / 2;
-          read[p * 4 + b] = (g / 2 * 8 + row) * 512 + (c ^ row * 2 ^ (p * 2 + g / 2) * 8) * 16 + l % 2 * 8;
+          read[p * BLOCKS + b] = (g / 2 * 8 + row) * ROW + (c ^ row * 2 ^ (p * 2 + g / 2 & MASK) * 8) * 16 + l % 2 * 8;
         }
     }
   }
 
-  // One of the eight loads that fill the 32 KB at `lds` (j: 4 KB of it), from the lane's j_from-th
+  // One of the loads that fill the tile at `lds` (j: 4 KB of it), from the lane's j_from-th
   // place; limit: K left in the source's rows (KC).
   __device__ __forceinline__ void load(const v4i& d, uint32_t lds, int j, int j_from, int64_t limit) const {
     wide_load(d, !KC || k < limit ? at[j_from] : kWideNowhere,
               __builtin_amdgcn_readfirstlane(lds + threadIdx.x / 64 * 1024 + j * 4096));
   }
 
-  // The operand of the 32 rows from the wave's origin + `off` (a multiple of 32, below 128 where K
-  // runs across rows) and K kk * 16 .. + 15.
+  // The operand of the 32 rows from the wave's origin + `off` (a multiple of 32, below SIDE / 2 where
+  // K runs across rows) and K kk * 16 .. + 15.
   __device__ __forceinline__ v8s operand(const char* lds, int off, int kk) const {
     if constexpr (KC) {
       return *(const v8s*)(lds + read[kk] + off * 128);
     } else {
       typedef __attribute__((address_space(3))) v4s lds_v4s;
-      const char* p = lds + read[kk % 2 * 4 + off / 32] + kk * 8192;
+      const char* p = lds + read[kk % 2 * BLOCKS + off / 32] + kk * 16 * ROW;
       const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p);
-      const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 2048));
+      const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 4 * ROW));
       return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }

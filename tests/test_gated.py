@@ -387,4 +387,4 @@ def test_refusals():
     assert bwd(1, 16) == -1 and b"workspace" in L.gsr_last_error()
     assert bwd(1, 1 << 20, dh=None) == -1 and b"null" in L.gsr_last_error()
     assert L.gsr_gated_workspace(4, 8, 6, 0, 1) >= 4 * 128 * 4 and L.gsr_gated_workspace(4, 8, 6, 7, 1) == 0
-    assert L.gsr_gated_workspace(4, 8, 6, 1, 0) == 0
+    assert L.gsr_gated_workspace(4, 8, 6, 1, 0) == 0 and L.gsr_gated_workspace(0, 8, 6, 1, 1) == 0
