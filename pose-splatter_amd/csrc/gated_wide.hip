@@ -15,7 +15,7 @@ template <typename T, int MODE, int SIDE>
 __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(GatedWide a) {
   constexpr bool DUAL = MODE == kWideFwd || MODE == kWideGrad, AKC = MODE != kWideDw, BKC = DUAL;
   constexpr int NB = SIDE / 64, HALF = SIDE / 2, BYTES = SIDE * kWideK * 2;   // blocks a wave and side; its rows
-  __shared__ __attribute__((aligned(1024))) char lds[2][2][BYTES];   // [buffer][operand]
+  __shared__ __attribute__((aligned(1024))) char lds[kWideStages][2][BYTES];   // [stage][operand]
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wm = wave % 2, wn = wave / 2;
   const GatedShape s = a.s;
   const int64_t pad = gated_pad(s.hidden);
@@ -23,68 +23,88 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
   wide_tile_of(blockIdx.x, a.mt, a.nt, &tm, &tn);
   const int64_t m0 = (int64_t)tm * SIDE, n0 = (int64_t)tn * (DUAL ? HALF : SIDE);
 
-  // K of this workgroup, and the operands' first bytes
+  // K of this workgroup, and the operands' corners.  Where K is contiguous the descriptor holds the
+  // tile's rows of one step; where it runs across rows, a step's rows up to K's end (the last step
+  // may be short: `short_bytes`).
   int64_t k0 = 0, k1 = DUAL ? a.kdim : MODE == kWideDx ? 2 * pad : s.rows;
   if constexpr (!DUAL) {
     k0 = blockIdx.z * a.share;
     k1 = k0 + a.share < k1 ? k0 + a.share : k1;
   }
   const int steps = (int)((k1 - k0 + kWideK - 1) / kWideK);
+  const auto at = [](const void* p, int64_t i) { return (const char*)p + i * 2; };
+  const auto rows_of = [&](int64_t rows, int64_t first, int64_t stride) {   // K contiguous: rows first .. of `rows`
+    const int64_t n = rows - first < SIDE ? rows - first : SIDE;
+    return n <= 0 ? 0 : ((n - 1) * stride + kWideK) * 2;
+  };
+  const auto ks_of = [](int64_t n, int64_t stride, int64_t left) {   // K across rows: n K, `left` columns to the row's end
+    return n <= 0 ? 0 : ((n < kWideK ? n : kWideK) - 1) * stride * 2 + left * 2;
+  };
   WideSource sa, sb, sb2;
-  int64_t a_step, b_step, a_stride, b_stride;
-  const auto from = [](const void* p, int64_t at, int64_t end) { return WideSource{(const char*)p + at * 2, (end - at) * 2}; };
+  uint32_t a_step, b_step, a_short = 0, b_short = 0;
+  int64_t a_stride, b_stride;
+  int shorts = steps, turn = -1;   // steps from `shorts` on are short; at step `turn` the second matrix begins
   if constexpr (DUAL) {
     a_stride = a.x_stride, b_stride = a.w_stride;
-    sa = from(a.x, m0 * a_stride, (s.rows - 1) * a_stride + a.kdim);
-    sb = from(a.wg, n0 * b_stride, (s.hidden - 1) * b_stride + a.kdim);
-    sb2 = from(a.wu, n0 * b_stride, (s.hidden - 1) * b_stride + a.kdim);
+    sa = WideSource(at(a.x, m0 * a_stride), rows_of(s.rows, m0, a_stride));
+    const int64_t n = s.hidden - n0 < HALF ? s.hidden - n0 : HALF, bytes = n <= 0 ? 0 : ((n - 1) * b_stride + kWideK) * 2;
+    sb = WideSource(at(a.wg, n0 * b_stride), bytes);
+    sb2 = WideSource(at(a.wu, n0 * b_stride), bytes);
     a_step = b_step = kWideK * 2;
   } else if constexpr (MODE == kWideDx) {
     a_stride = 2 * pad, b_stride = a.w_stride;
-    sa = from(a.dgu, m0 * a_stride + k0, s.rows * a_stride);
-    const int64_t kw = k0 < pad ? k0 : k0 - pad;   // (pad is whole steps: none straddles Wg and Wu)
-    sb = from(k0 < pad ? a.wg : a.wu, kw * b_stride + n0, (s.hidden - 1) * b_stride + a.kdim);
-    sb2 = from(a.wu, n0, (s.hidden - 1) * b_stride + a.kdim);
-    a_step = kWideK * 2, b_step = kWideK * b_stride * 2;
+    sa = WideSource(at(a.dgu, m0 * a_stride + k0), rows_of(s.rows, m0, a_stride));
+    // K rows of Wg, then of Wu, each followed by up to pad - hidden < 64 rows of nothing
+    const int64_t kw = k0 < pad ? k0 : k0 - pad;   // (pad is whole steps: none straddles the matrices)
+    sb = WideSource(at(k0 < pad ? a.wg : a.wu, kw * b_stride + n0), ks_of(kWideK, b_stride, a.kdim - n0));
+    sb2 = WideSource(at(a.wu, n0), 0);
+    a_step = kWideK * 2, b_step = (uint32_t)(kWideK * b_stride * 2);
+    turn = k0 < pad ? (int)((pad - k0) / kWideK) : -1;
   } else {
     a_stride = 2 * pad, b_stride = a.x_stride;
-    sa = from(a.dgu, k0 * a_stride + m0, k1 * a_stride);
-    sb = from(a.x, k0 * b_stride + n0, (k1 - 1) * b_stride + a.kdim);
-    a_step = kWideK * a_stride * 2, b_step = kWideK * b_stride * 2;
+    sa = WideSource(at(a.dgu, k0 * a_stride + m0), ks_of(k1 - k0, a_stride, a_stride - m0));
+    sb = WideSource(at(a.x, k0 * b_stride + n0), ks_of(k1 - k0, b_stride, a.kdim - n0));
+    a_step = (uint32_t)(kWideK * a_stride * 2), b_step = (uint32_t)(kWideK * b_stride * 2);
+    a_short = (uint32_t)ks_of((k1 - k0) % kWideK, a_stride, a_stride - m0);
+    b_short = (uint32_t)ks_of((k1 - k0) % kWideK, b_stride, a.kdim - n0);
+    shorts = (int)((k1 - k0) / kWideK);
   }
   WideTile<AKC, SIDE> ta;
   WideTile<BKC, SIDE> tb;
   ta.init(a_stride * 2, wm * HALF);
   tb.init(b_stride * 2, DUAL ? wn * (HALF / 2) : wn * HALF);
 
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0][0];
-  int64_t left = k1 - k0;   // K left at the next tile's start
-  int next = 0;             // the next tile to load
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0][0] + wave * 1024);
+  int next = 0;   // the next step to load
   v4i da, db, db2;
-  const auto begin = [&]() {   // (a tile past K's end is nothing: descriptors of no length)
+  const auto begin = [&]() {   // (a step past K's end is nothing: descriptors of no length)
+    if constexpr (MODE == kWideDx) {
+      if (next == turn) sb.lo = sb2.lo, sb.hi = sb2.hi;
+      // the rows left of this matrix
+      const int64_t k = k0 + (int64_t)next * kWideK, n = s.hidden - (k < pad ? k : k - pad);
+      sb.bytes = (uint32_t)ks_of(n, b_stride, a.kdim - n0);
+    }
+    if constexpr (MODE == kWideDw) {
+      if (next == shorts) sa.bytes = a_short, sb.bytes = b_short;
+    }
     da = sa.descriptor(next < steps);
     db = sb.descriptor(next < steps);
     if constexpr (DUAL) db2 = sb2.descriptor(next < steps);
-  };
-  constexpr int LOADS = SIDE / 32;
-  const auto load = [&](int i, int buf) {   // one of 2 LOADS
-    const uint32_t to = lds0 + buf * 2 * BYTES;
-    if (i < LOADS) {
-      ta.load(da, to, i, i, left);
-    } else if (DUAL && i >= LOADS * 3 / 2) {
-      tb.load(db2, to + BYTES, i - LOADS, i - LOADS * 3 / 2, left);
-    } else {
-      tb.load(db, to + BYTES, i - LOADS, i - LOADS, left);
-    }
-  };
-  const auto end = [&]() {
     sa.advance(a_step);
     sb.advance(b_step);
     if constexpr (DUAL) sb2.advance(b_step);
-    left -= kWideK;
     ++next;
-    if constexpr (MODE == kWideDx)
-      if (k0 + (int64_t)next * kWideK == pad) sb = sb2;
+  };
+  constexpr int LOADS = BYTES / 4096;
+  const auto load = [&](int i, uint32_t to) {   // one of 2 LOADS into the stage at `to`
+    if (i < LOADS) {
+      wide_load(da, ta.at[i % LOADS], to, i * 4096);
+    } else if (DUAL && i >= LOADS * 3 / 2) {
+      wide_load(db2, tb.at[i - LOADS * 3 / 2], to, i * 4096);
+    } else {
+      wide_load(db, tb.at[i - LOADS], to, i * 4096);
+    }
   };
 
   v16f acc[NB][NB];   // [n block][m block]
@@ -93,57 +113,61 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[i / NB][i % NB][j] = 0.f;
   v8s fa[2][NB], fb[2][NB];
-  const auto operands = [&](int buf, int kk, int set) {
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      fa[set][b] = ta.operand(lds[buf][0], b * 32, kk);
-      fb[set][b] = tb.operand(lds[buf][1], DUAL && b >= NB / 2 ? HALF + (b - NB / 2) * 32 : b * 32, kk);
+  const char* base = &lds[0][0][0];
+  const auto operand = [&](int stage, int kk, int i) {   // one of 2 NB
+    const char* p = base + stage * 2 * BYTES;
+    if (i < NB) {
+      fa[kk][i % NB] = ta.operand(p, i * 32, kk);
+    } else {
+      const int b = i % NB;
+      fb[kk][b] = tb.operand(p + BYTES, DUAL && b >= NB / 2 ? HALF + (b - NB / 2) * 32 : b * 32, kk);
     }
   };
-  const auto mma = [&](int set, int i) {
-    acc[i / NB][i % NB] = wide_mma<T>(fb[set][i / NB], fa[set][i % NB], acc[i / NB][i % NB]);
-  };
-
+  // Half a step: the products of kk, and between them the reads of the next half's operands, then half
+  // of a stage's loads.  One wave a SIMD issues all of it, so every other instruction sits in a
+  // product's shadow (32 cycles, six or so instructions); the order is as written.
+  const auto half_step = [&](int kk, int from, uint32_t to) {
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
+    for (int i = 0; i < NB * NB; ++i) {
+      acc[i / NB][i % NB] = wide_mma<T>(fb[kk][i / NB], fa[kk][i % NB], acc[i / NB][i % NB]);
+      constexpr int EVERY = NB * NB / LOADS, READS = 4 / NB;   // reads a product: 1 of 16, 2 of 4
+#pragma unroll
+      for (int j = 0; j < READS; ++j)
+        if (i * READS + j < 2 * NB) operand(from, kk ^ 1, i * READS + j);
+      if (i % EVERY == EVERY - 1) load(kk * LOADS + i / EVERY, to);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  constexpr int AHEAD = kWideStages - 1, FLIGHT = (AHEAD - 2) * 2 * LOADS + LOADS;
+#pragma unroll
+  for (int b = 0; b < AHEAD; ++b) {
     begin();
 #pragma unroll
-    for (int i = 0; i < 2 * LOADS; ++i) load(i, b);
-    end();
+    for (int i = 0; i < 2 * LOADS; ++i) load(i, lds0 + b * 2 * BYTES);
   }
-  wide_wait();
+  wide_wait<(AHEAD - 1) * 2 * LOADS>();
   __syncthreads();
-  operands(0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < 2 * NB; ++i) operand(0, 0, i);
+  int stage = 0;
   for (int st = 0; st < steps; ++st) {
-    const int buf = st & 1;
-#pragma unroll
-    for (int kk = 0; kk < 3; ++kk) {
-      operands(buf, kk + 1, (kk + 1) & 1);   // in flight over the products (the scheduler would sink them)
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < NB * NB; ++i) mma(kk & 1, i);
-    }
-    // The last operands of this buffer are in registers and the next buffer's loads, a step old,
-    // have landed: for every wave, after the barrier.
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    const int after = stage == AHEAD ? 0 : stage + 1;
+    const uint32_t to = lds0 + (stage == 0 ? AHEAD : stage - 1) * 2 * BYTES;   // the step before's stage: read by all
+    begin();
+    half_step(0, stage, to);
+    // This stage's last operands are in registers, and the next stage has landed: for every wave,
+    // after the barrier.
+    wide_wait<FLIGHT>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    operands(buf ^ 1, 0, 0);
-    begin();
-#pragma unroll
-    for (int i = 0; i < NB * NB; ++i) {   // loads between the products, rather than all in a row
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int j = 0; j < 2 * LOADS / (NB * NB); ++j) load(i * (2 * LOADS / (NB * NB)) + j, buf);
-      mma(1, i);
-    }
-    end();
+    half_step(1, after, to);
+    stage = after;
   }
 
   // Each wave passes its sums, 32 rows of a block row at a time, through its own part of the shared memory
   // (no wave reads a tile any more after the barrier): there a lane takes eight neighbouring columns,
   // so that rows are read and written in whole lines.
-  wide_wait();   // (the loads past K's end write zeros)
+  wide_wait<0>();   // (the loads past K's end write zeros)
   __syncthreads();
   constexpr int LD = HALF + 4;   // floats a row: a wave's columns and 4 to spread the banks
   static_assert(4 * 32 * LD * sizeof(float) <= sizeof(lds), "the waves' rows fit the tiles' memory");
