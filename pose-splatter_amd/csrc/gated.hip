@@ -317,7 +317,7 @@ static int64_t gated_shares(int64_t tiles, int64_t tile, int64_t k, int64_t valu
 }
 
 // Padded copies of up to three matrices: to [rows][kdim] = p [rows][dim] (row stride `stride`) and
-// zeros, rows that start at 16 bytes and are whole steps of K.
+// zeros, rows that start at 16 bytes and are whole 16-byte pieces.
 template <typename T>
 struct GatedPads {
   const T* p[3];
@@ -353,19 +353,19 @@ static int gated_side(int type, int64_t rows, int64_t cols, int64_t k, GatedShap
   return GSR_SIDE_RULE ? 128 : 64;
 }
 
-// What a wide case's operands need: rows of whole steps of K at 16-byte addresses, 256 of them
+// What a wide case's operands need: rows of whole 16-byte pieces at 16-byte addresses, 256 of them
 // within 31 bits.
 static bool gated_aligned(const void* p, int64_t dim, int64_t stride) {
-  return (uintptr_t)p % 16 == 0 && dim % 32 == 0 && stride % 8 == 0 && stride <= 1 << 21;
+  return (uintptr_t)p % 16 == 0 && dim % 8 == 0 && stride % 8 == 0 && stride <= 1 << 21;
 }
 
 // How a pass is laid out: each product's tile side and shares of K, and its workspace (byte
-// offsets).  There is room for padded copies wherever a wide product may need them: a dim that is not
-// whole steps of K, rows or addresses that are not multiples of 16 bytes.
+// offsets).  There is room for padded copies wherever a wide product may need them: an odd dim, rows
+// or addresses that are not multiples of 16 bytes.
 struct GatedPlan {
   int fwd, dx, dw;               // tile sides
   int64_t n_dx, n_dw;            // shares
-  int64_t kdim;                  // dim in whole steps of 32
+  int64_t kdim;                  // dim in whole 16-byte pieces
   int64_t x, wg, wu, dgu, bias, bias_rows, dx_parts, dw_parts, total;
 };
 
@@ -375,7 +375,7 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
   w.fwd = gated_side(type, s.rows, 2 * pad, s.dim, s);
   w.dx = gated_side(type, s.rows, s.dim, 2 * pad, s);
   w.dw = gated_side(type, 2 * pad, s.dim, s.rows, s);
-  w.kdim = (s.dim + 31) / 32 * 32;
+  w.kdim = (s.dim + 7) / 8 * 8;
   const auto tiles = [](int side, int64_t r, int64_t c) { return ceil_div64(r, side) * ceil_div64(c, side); };
   w.n_dx = gated_shares(tiles(w.dx, s.rows, s.dim), w.dx, 2 * pad, s.rows * s.dim);
   w.n_dw = gated_shares(tiles(w.dw, 2 * pad, s.dim), w.dw, s.rows, 2 * s.hidden * s.dim);
@@ -398,7 +398,7 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
   return w;
 }
 
-// The wide products' operands, copied into rows of whole steps where they are not.
+// The wide products' operands, copied into whole 16-byte pieces where they are not.
 template <typename T>
 static GatedWide gated_wide_args(const T* x, int64_t x_stride, const T* wg, const T* wu, const void* bg, const void* bu, int act,
                                  GatedShape s, const GatedPlan& w, bool use_x, bool use_w, char* ws, hipStream_t st) {

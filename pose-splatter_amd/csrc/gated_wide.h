@@ -8,8 +8,7 @@ namespace gsr {
 enum { kWideFwd, kWideGrad, kWideDx, kWideDw };
 
 // The tensors of one product, 16-bit, x, wg and wu 16-byte aligned with strides (in elements) that are
-// multiples of 8, and kdim, the length of their rows, a multiple of 32: the block's dim, or it padded
-// with zeros.
+// multiples of 8, and kdim, the length of their rows, too: the block's dim, or it padded with zeros.
 struct GatedWide {
   GatedShape s;
   int64_t kdim, x_stride, w_stride, dh_stride;

@@ -11,11 +11,16 @@
 
 namespace gsr {
 
+template <int N>
+struct Count {
+  static constexpr int value = N;
+};
+
 template <typename T, int MODE, int SIDE>
 __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(GatedWide a) {
   constexpr bool DUAL = MODE == kWideFwd || MODE == kWideGrad, AKC = MODE != kWideDw, BKC = DUAL;
   constexpr int NB = SIDE / 64, HALF = SIDE / 2, BYTES = SIDE * kWideK * 2;   // blocks a wave and side; its rows
-  __shared__ __attribute__((aligned(1024))) char lds[kWideStages][2][BYTES];   // [stage][operand]
+  __shared__ __attribute__((aligned(1024))) char lds[kWideSlots][BYTES];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wm = wave % 2, wn = wave / 2;
   const GatedShape s = a.s;
   const int64_t pad = gated_pad(s.hidden);
@@ -75,35 +80,41 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
   tb.init(b_stride * 2, DUAL ? wn * (HALF / 2) : wn * HALF);
 
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
-      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0][0] + wave * 1024);
-  int next = 0;   // the next step to load
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0] + wave * 1024);
+  // A step's operand tiles are loaded one after the other, A then B; next_*: the step whose tile is next.
+  // (A step past K's end is nothing: descriptors of no length.)
+  int next_a = 0, next_b = 0, left_a = (int)(k1 - k0), left_b = left_a;
   v4i da, db, db2;
-  const auto begin = [&]() {   // (a step past K's end is nothing: descriptors of no length)
+  const auto begin_a = [&]() {
+    if constexpr (MODE == kWideDw)
+      if (next_a == shorts) sa.bytes = a_short;
+    da = sa.descriptor(next_a < steps);
+    sa.advance(a_step);
+    left_a = (int)(k1 - k0) - next_a * kWideK;
+    ++next_a;
+  };
+  const auto begin_b = [&]() {
     if constexpr (MODE == kWideDx) {
-      if (next == turn) sb.lo = sb2.lo, sb.hi = sb2.hi;
-      // the rows left of this matrix
-      const int64_t k = k0 + (int64_t)next * kWideK, n = s.hidden - (k < pad ? k : k - pad);
+      if (next_b == turn) sb.lo = sb2.lo, sb.hi = sb2.hi;
+      const int64_t k = k0 + (int64_t)next_b * kWideK, n = s.hidden - (k < pad ? k : k - pad);   // rows left in the matrix
       sb.bytes = (uint32_t)ks_of(n, b_stride, a.kdim - n0);
     }
-    if constexpr (MODE == kWideDw) {
-      if (next == shorts) sa.bytes = a_short, sb.bytes = b_short;
-    }
-    da = sa.descriptor(next < steps);
-    db = sb.descriptor(next < steps);
-    if constexpr (DUAL) db2 = sb2.descriptor(next < steps);
-    sa.advance(a_step);
+    if constexpr (MODE == kWideDw)
+      if (next_b == shorts) sb.bytes = b_short;
+    db = sb.descriptor(next_b < steps);
+    if constexpr (DUAL) db2 = sb2.descriptor(next_b < steps);
     sb.advance(b_step);
     if constexpr (DUAL) sb2.advance(b_step);
-    ++next;
+    left_b = (int)(k1 - k0) - next_b * kWideK;
+    ++next_b;
   };
   constexpr int LOADS = BYTES / 4096;
-  const auto load = [&](int i, uint32_t to) {   // one of 2 LOADS into the stage at `to`
-    if (i < LOADS) {
-      wide_load(da, ta.at[i % LOADS], to, i * 4096);
-    } else if (DUAL && i >= LOADS * 3 / 2) {
-      wide_load(db2, tb.at[i - LOADS * 3 / 2], to, i * 4096);
+  const auto load_a = [&](int i, int slot) { wide_load(da, ta.offset(i, left_a), lds0 + slot * BYTES, i * 4096); };
+  const auto load_b = [&](int i, int slot) {
+    if (DUAL && i >= LOADS / 2) {
+      wide_load(db2, tb.offset(i - LOADS / 2, left_b), lds0 + slot * BYTES, i * 4096);
     } else {
-      wide_load(db, tb.at[i - LOADS], to, i * 4096);
+      wide_load(db, tb.offset(i, left_b), lds0 + slot * BYTES, i * 4096);
     }
   };
 
@@ -113,55 +124,66 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[i / NB][i % NB][j] = 0.f;
   v8s fa[2][NB], fb[2][NB];
-  const char* base = &lds[0][0][0];
-  const auto operand = [&](int stage, int kk, int i) {   // one of 2 NB
-    const char* p = base + stage * 2 * BYTES;
+  const auto operand = [&](int slot_a, int slot_b, int kk, int i) {   // one of 2 NB
     if (i < NB) {
-      fa[kk][i % NB] = ta.operand(p, i * 32, kk);
+      fa[kk & 1][i % NB] = ta.operand(&lds[slot_a][0], i * 32, kk);
     } else {
       const int b = i % NB;
-      fb[kk][b] = tb.operand(p + BYTES, DUAL && b >= NB / 2 ? HALF + (b - NB / 2) * 32 : b * 32, kk);
+      fb[kk & 1][b] = tb.operand(&lds[slot_b][0], DUAL && b >= NB / 2 ? HALF + (b - NB / 2) * 32 : b * 32, kk);
     }
   };
-  // Half a step: the products of kk, and between them the reads of the next half's operands, then half
-  // of a stage's loads.  One wave a SIMD issues all of it, so every other instruction sits in a
-  // product's shadow (32 cycles, six or so instructions); the order is as written.
-  const auto half_step = [&](int kk, int from, uint32_t to) {
+  // A quarter of a step: the products of 16 K, and between them the reads of the next quarter's operands
+  // (of kk `read` in the slots given), then `loads` of the LOADS loads that `load` issues.  One wave a
+  // SIMD issues all of it, so every other instruction sits in a product's shadow (32 cycles, six
+  // or so instructions); the order is as written.
+  const auto quarter = [&](int kk, int slot_a, int slot_b, int read, auto loads, auto load) {
 #pragma unroll
     for (int i = 0; i < NB * NB; ++i) {
-      acc[i / NB][i % NB] = wide_mma<T>(fb[kk][i / NB], fa[kk][i % NB], acc[i / NB][i % NB]);
-      constexpr int EVERY = NB * NB / LOADS, READS = 4 / NB;   // reads a product: 1 of 16, 2 of 4
+      acc[i / NB][i % NB] = wide_mma<T>(fb[kk & 1][i / NB], fa[kk & 1][i % NB], acc[i / NB][i % NB]);
+      constexpr int READS = 4 / NB;   // reads a product: 1 of 16, 2 of 4
 #pragma unroll
       for (int j = 0; j < READS; ++j)
-        if (i * READS + j < 2 * NB) operand(from, kk ^ 1, i * READS + j);
-      if (i % EVERY == EVERY - 1) load(kk * LOADS + i / EVERY, to);
+        if (i * READS + j < 2 * NB) operand(slot_a, slot_b, read, i * READS + j);
+      constexpr int N = decltype(loads)::value;
+      if constexpr (N > 0) {
+        constexpr int EVERY = NB * NB / N;
+        if (i % EVERY == EVERY - 1) load(i / EVERY);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  constexpr int AHEAD = kWideStages - 1, FLIGHT = (AHEAD - 2) * 2 * LOADS + LOADS;
+  const auto nothing = [](int) {};
+
 #pragma unroll
-  for (int b = 0; b < AHEAD; ++b) {
-    begin();
+  for (int b = 0; b < 2; ++b) {
+    begin_a();
 #pragma unroll
-    for (int i = 0; i < 2 * LOADS; ++i) load(i, lds0 + b * 2 * BYTES);
+    for (int i = 0; i < LOADS; ++i) load_a(i, 2 * b);
+    begin_b();
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load_b(i, 2 * b + 1);
   }
-  wide_wait<(AHEAD - 1) * 2 * LOADS>();
+  wide_wait<2 * LOADS>();
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 2 * NB; ++i) operand(0, 0, i);
-  int stage = 0;
+  for (int i = 0; i < 2 * NB; ++i) operand(0, 1, 0, i);
+  const auto plus = [](int slot, int n) { return slot + n < kWideSlots ? slot + n : slot + n - kWideSlots; };
+  int slot_a = 0, slot_b = 1;   // of this step; the next step's are two on, the one after's four
   for (int st = 0; st < steps; ++st) {
-    const int after = stage == AHEAD ? 0 : stage + 1;
-    const uint32_t to = lds0 + (stage == 0 ? AHEAD : stage - 1) * 2 * BYTES;   // the step before's stage: read by all
-    begin();
-    half_step(0, stage, to);
-    // This stage's last operands are in registers, and the next stage has landed: for every wave,
-    // after the barrier.
-    wide_wait<FLIGHT>();
+    const int into_a = plus(slot_a, 4), next_slot_a = plus(slot_a, 2), next_slot_b = plus(slot_b, 2);
+    begin_a();   // A of the step after the next, into the slot of B of the step before
+    quarter(0, slot_a, slot_b, 1, Count<LOADS / 2>{}, [&](int i) { load_a(i, into_a); });
+    quarter(1, slot_a, slot_b, 2, Count<LOADS / 2>{}, [&](int i) { load_a(LOADS / 2 + i, into_a); });
+    quarter(2, slot_a, slot_b, 3, Count<0>{}, nothing);
+    // This step's last operands are in registers and the next step's tiles have landed (only the A
+    // above may be in flight): for every wave, after the barrier.
+    wide_wait<LOADS>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    half_step(1, after, to);
-    stage = after;
+    begin_b();   // B of the step after the next, into this step's slot of A
+    quarter(3, next_slot_a, next_slot_b, 0, Count<LOADS>{}, [&](int i) { load_b(i, slot_a); });
+    slot_a = next_slot_a;
+    slot_b = next_slot_b;
   }
 
   // Each wave passes its sums, 32 rows of a block row at a time, through its own part of the shared memory
@@ -171,7 +193,7 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
   __syncthreads();
   constexpr int LD = HALF + 4;   // floats a row: a wave's columns and 4 to spread the banks
   static_assert(4 * 32 * LD * sizeof(float) <= sizeof(lds), "the waves' rows fit the tiles' memory");
-  float* mine = (float*)&lds[0][0][0] + wave * 32 * LD;
+  float* mine = (float*)&lds[0][0] + wave * 32 * LD;
   constexpr int COLS = DUAL ? HALF / 2 : HALF, LANES = COLS / 8, ROWS = 64 / LANES;   // lanes a row, rows a pass
   const int c = lane % LANES * 8;
   const int64_t n = n0 + wn * COLS + c, left_n = (DUAL ? s.hidden : s.dim) - n;

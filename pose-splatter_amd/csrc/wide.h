@@ -2,30 +2,32 @@
 // block's main loop.
 //
 // A workgroup of four waves owns a 256 x 256 tile, each wave a 128 x 128 quarter of 4 x 4 blocks
-// of 32x32x16 matrix instructions: 256 accumulators a lane.  K advances 32 at a time through a ring
-// of five stages in shared memory (32 KB each, all of it), so a stage's loads have three and a half
-// steps to land.  A quarter that large reads 2 x 128 x 64 elements for 128 x 128 x 64
-// multiply-adds, 64 bytes of shared memory a cycle and CU at full matrix rate where 128 are
-// available; eight waves of 128 x 64 would need 96 and leave none for the stores.  128 x 128 tiles
-// (2 x 2 blocks a wave, two workgroups a CU) are for products of fewer tiles than CUs.
+// of 32x32x16 matrix instructions: 256 accumulators a lane.  K advances 64 at a time; shared memory
+// is a ring of five operand tiles (32 KB each, all of it): the two in use and three on their way,
+// so a tile's loads have one to one and three quarters of a step to land.  A quarter that large reads
+// 2 x 128 x 64 elements for 128 x 128 x 64 multiply-adds, 64 bytes of shared memory a cycle and
+// CU at full matrix rate where 128 are available; eight waves of 128 x 64 would need 96 and leave
+// none for the stores.  128 x 128 tiles (2 x 2 blocks a wave, two workgroups a CU) are for products
+// of fewer tiles than CUs.
 //
 // Tiles come straight from global memory into shared memory (16 bytes a lane, no registers).  Each
 // operand is read in the order it lies in memory:
-//   K contiguous     rows of 32 K (64 bytes); 16-byte chunk c of row r sits in slot c ^ (r / 4 % 4),
-//                    so the 16-byte reads of eight neighbouring rows hit different banks
+//   K contiguous     rows of 64 K (128 bytes, a cache line); 16-byte chunk c of row r sits in slot
+//                    c ^ (r % 8), so the 16-byte reads of eight neighbouring rows hit different banks
 //   K across rows    rows of 256 (128) columns a K; chunk c of row k sits in slot
 //                    c ^ (2 (k % 4) + 8 (k / 8 % 4 (% 2))); ds_read_b64_tr_b16 turns 4 K x 16 columns
 //                    into the instruction's K-contiguous operand on the way out
 // The pattern is made by choosing what each lane loads: shared memory itself is filled in lane
 // order.  Loads past an operand's end return zeros (the buffer descriptor's bound), so no tile
-// needs a special case; a row of contiguous K is whole steps long (padded with zeros where it is not).
+// needs a special case; only K's own end inside a row is checked lane by lane.
 #pragma once
 
 #include "types.h"
 
 namespace gsr {
 
-constexpr int kWideK = 32, kWideStages = 5, kWideThreads = 256;
+constexpr int kWideK = 64, kWideSlots = 5, kWideThreads = 256;
+constexpr uint32_t kWideNowhere = 0x80000000u;   // past every descriptor's end
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
@@ -90,17 +92,19 @@ struct WideTile {
   static constexpr int BYTES = SIDE * kWideK * 2, LOADS = BYTES / 4096, BLOCKS = SIDE / 64;
   static constexpr int ROW = SIDE * 2;   // bytes of a K row (K across rows)
   uint32_t at[LOADS];   // byte offsets of the lane's loads from the tile's corner
-  uint32_t read[KC ? 2 : 2 * BLOCKS];   // byte offsets of its reads: per 16 K (KC), or per K parity and block
+  int k;                // KC: the loads' first K
+  uint32_t read[KC ? 4 : 2 * BLOCKS];   // byte offsets of its reads: per 16 K (KC), or per K parity and block
 
   // origin: the wave's first row (KC) or column of the tile's
   __device__ __forceinline__ void init(int64_t stride_bytes, int origin) {
     const int t = threadIdx.x, l = t % 64;
     if constexpr (KC) {
-      const int c = t % 4 ^ (t / 16 & 3);
+      const int c = t % 8 ^ (t / 8 & 7);
+      k = c * 8;
 #pragma unroll
-      for (int j = 0; j < LOADS; ++j) at[j] = (uint32_t)((j * 64 + t / 4) * stride_bytes + c * 16);
+      for (int j = 0; j < LOADS; ++j) at[j] = (uint32_t)((j * 32 + t / 8) * stride_bytes + c * 16);
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) read[kk] = (origin + l % 32) * 64 + ((kk * 2 + l / 32) ^ (l >> 2 & 3)) * 16;
+      for (int kk = 0; kk < 4; ++kk) read[kk] = (origin + l % 32) * 128 + ((kk * 2 + l / 32) ^ (l & 7)) * 16;
     } else {
       constexpr int SLOTS = ROW / 16, EACH = 256 / SLOTS;   // 16-byte slots a K row, K rows a load
       constexpr int MASK = SIDE == 256 ? 3 : 1;
@@ -120,14 +124,17 @@ struct WideTile {
     }
   }
 
+  // The lane's j-th load's offset, where `left` K are left at the tile's start.
+  __device__ __forceinline__ uint32_t offset(int j, int left) const { return !KC || k < left ? at[j] : kWideNowhere; }
+
   // The operand of the 32 rows from the wave's origin + `off` (a multiple of 32, below SIDE / 2 where
   // K runs across rows) and K kk * 16 .. + 15.
   __device__ __forceinline__ v8s operand(const char* lds, int off, int kk) const {
     if constexpr (KC) {
-      return *(const v8s*)(lds + read[kk] + off * 64);
+      return *(const v8s*)(lds + read[kk] + off * 128);
     } else {
       typedef __attribute__((address_space(3))) v4s lds_v4s;
-      const char* p = lds + read[kk * BLOCKS + off / 32] + kk * 16 * ROW;
+      const char* p = lds + read[kk % 2 * BLOCKS + off / 32] + kk * 16 * ROW;
       const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p);
       const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 4 * ROW));
       return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
