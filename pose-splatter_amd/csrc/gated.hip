@@ -10,7 +10,8 @@
 // kept from the forward and moved twice), then takes dx from K = [dg | du] and both weight
 // gradients from M = [dg | du].
 //
-// Large 16-bit cases run on 256 x 256 tiles (gated_wide.hip); here is what serves all others:
+// Most cases run on square tiles of 256 or 128 (gated_wide.hip), up to 64 rows on gated_skinny.hip's kernel;
+// here is what serves the others:
 //
 // k_tile: 64 x 64 tiles of any shape, stride and alignment, with 16x16 matrix instructions: fp32
 // ones for fp32 (exact fp32 products), bf16/fp16 ones with fp32 sums.  A weight gradient's sum
@@ -18,10 +19,6 @@
 #include "gated.h"
 #include "gated_skinny.h"
 #include "gated_wide.h"
-
-#ifndef GSR_SIDE_RULE
-#define GSR_SIDE_RULE 1
-#endif
 
 namespace gsr {
 
@@ -280,19 +277,23 @@ __global__ __launch_bounds__(256) void k_tile_dw(const T* dgu, const T* x, int64
     }
 }
 
-// [a | b], a the first `split` of n values, = the sum over `count` rows of parts [count][n], in order.
+// [a | b], a the first `split` of n values, = the sum over `count` rows of parts [count][n]: sixteen
+// lanes a value, each a fixed share of the rows with four loads in flight, then the sixteen in order.
 template <typename T>
-__global__ __launch_bounds__(256) void k_gated_join(const float* parts, int64_t count, int64_t n, int64_t split, T* a, T* b) {
-  __shared__ float sum[4][64];
+__global__ __launch_bounds__(1024) void k_gated_join(const float* parts, int64_t count, int64_t n, int64_t split, T* a, T* b) {
+  __shared__ float sum[16][65];
   const int lane = threadIdx.x % 64, grp = threadIdx.x / 64;
   const int64_t c = (int64_t)blockIdx.x * 64 + lane;
   float s = 0.f;
-  if (c < n)
-    for (int64_t r = grp; r < count; r += 4) s += parts[r * n + c];
+  if (c < n) {
+#pragma unroll 4
+    for (int64_t r = grp; r < count; r += 16) s += parts[r * n + c];
+  }
   sum[grp][lane] = s;
   __syncthreads();
   if (grp == 0 && c < n) {
-    s = (sum[0][lane] + sum[1][lane]) + (sum[2][lane] + sum[3][lane]);
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += sum[k][lane];
     if (c < split) {
       if (a) a[c] = from_f<T>(s);
     } else if (b) {
@@ -303,14 +304,14 @@ __global__ __launch_bounds__(256) void k_gated_join(const float* parts, int64_t 
 
 template <typename T>
 static void gated_join(const float* parts, int64_t count, int64_t n, int64_t split, void* a, void* b, hipStream_t st) {
-  k_gated_join<T><<<(unsigned)ceil_div64(n, 64), 256, 0, st>>>(parts, count, n, split, (T*)a, (T*)b);
+  k_gated_join<T><<<(unsigned)ceil_div64(n, 64), 1024, 0, st>>>(parts, count, n, split, (T*)a, (T*)b);
 }
 
-// Shares of K in a product of `tiles` tiles of side `tile`: enough workgroups for two a CU (one of side
-// 256), each share at least eight steps of 64, the fp32 parts of `values` results at most 64 MB.
-static int64_t gated_shares(int64_t tiles, int64_t tile, int64_t k, int64_t values) {
-  int64_t n = (tile == 256 ? 256 : 512) / tiles;
-  n = n < k / 512 ? n : k / 512;
+// Shares of K in a product of `tiles` 64 x 64 tiles: enough workgroups for two a CU, each share at
+// least 128 of K, the fp32 parts of `values` results at most 64 MB.
+static int64_t gated_shares(int64_t tiles, int64_t k, int64_t values) {
+  int64_t n = 512 / tiles;
+  n = n < k / 128 ? n : k / 128;
   const int64_t most = (64 << 20) / 4 / values;
   n = n < most ? n : most;
   return n < 1 ? 1 : n;
@@ -328,15 +329,16 @@ struct GatedPads {
 
 template <typename T>
 __global__ __launch_bounds__(256) void k_gated_pad(GatedPads<T> a) {
-  const int64_t per = a.kdim / 8;
+  constexpr int V = 16 / sizeof(T);
+  const int64_t per = a.kdim / V;
   int64_t first = 0;
 #pragma unroll
   for (int q = 0; q < 3; ++q) {   // one run of pieces through all three
     const int64_t n = a.rows[q] * per;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < first + n; i += (int64_t)gridDim.x * 256) {
       if (i < first) continue;
-      const int64_t r = (i - first) / per, c = (i - first) % per * 8;
-      float v[8];
+      const int64_t r = (i - first) / per, c = (i - first) % per * V;
+      float v[V];
       load_upto(a.p[q] + r * a.stride[q] + c, a.dim - c, v);
       store_vec(a.to[q] + r * a.kdim + c, v);
     }
@@ -344,22 +346,28 @@ __global__ __launch_bounds__(256) void k_gated_pad(GatedPads<T> a) {
   }
 }
 
-// Tile side of a 16-bit product of `rows` x `cols` outputs: 256 where its tiles fill most CUs, 128
-// where two a CU would be filled to half by the shares of K, 64 (any alignment, no padded copies) below.
+// Tile side of a product of rows x cols outputs over k.  256 (16 bits) where every CU gets at least 96
+// steps of K: 16384 x 2048 -> 5632, at 352 a CU, forward 660 us against 726 with 128, dW 593
+// against 877; at 88 the two are within 5 %; at 31 (16000 x 512 -> 2048) 111 us against 101.
+// 64 (any alignment, no padded copies) for dims whose K is hardly a step, and in fp32, whose products
+// are long enough to run side by side, where the 512 workgroups of 128 would get fewer than 8 steps
+// (256 x 1024 -> 2816, 5.5 steps: forward 56 us against 70; 16000 x 256 -> 512, 16: 84 against 77).
 static int gated_side(int type, int64_t rows, int64_t cols, int64_t k, GatedShape s) {
-  if (type == GSR_F32 || s.dim < 64 || s.rows <= kSkinnyRows) return 64;
-  const int64_t wide = ceil_div64(rows, 256) * ceil_div64(cols, 256);
-  if (wide >= 192) return 256;
-  return GSR_SIDE_RULE ? 128 : 64;
+  if (s.dim < 64 || s.rows <= kSkinnyRows) return 64;
+  const int64_t steps = gated_wide_steps(type, k);
+  if (type == GSR_F32) return ceil_div64(rows, 128) * ceil_div64(cols, 128) * steps >= 512 * 8 ? 128 : 64;
+  return ceil_div64(rows, 256) * ceil_div64(cols, 256) * steps >= 256 * 96 ? 256 : 128;
 }
 
 // What a wide case's operands need: rows of whole 16-byte pieces at 16-byte addresses, 256 of them
 // within 31 bits.
-static bool gated_aligned(const void* p, int64_t dim, int64_t stride) {
-  return (uintptr_t)p % 16 == 0 && dim % 8 == 0 && stride % 8 == 0 && stride <= 1 << 21;
+template <typename T>
+static bool gated_aligned(const T* p, int64_t dim, int64_t stride) {
+  constexpr int V = 16 / sizeof(T);
+  return (uintptr_t)p % 16 == 0 && dim % V == 0 && stride % V == 0 && stride <= 1 << 20;
 }
 
-// How a pass is laid out: each product's tile side and shares of K, and its workspace (byte
+// How a pass is laid out: each product's tile side, the 64 x 64 tiles' shares of K, and its workspace (byte
 // offsets).  There is room for padded copies wherever a wide product may need them: an odd dim, rows
 // or addresses that are not multiples of 16 bytes.
 struct GatedPlan {
@@ -375,10 +383,14 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
   w.fwd = gated_side(type, s.rows, 2 * pad, s.dim, s);
   w.dx = gated_side(type, s.rows, s.dim, 2 * pad, s);
   w.dw = gated_side(type, 2 * pad, s.dim, s.rows, s);
-  w.kdim = (s.dim + 7) / 8 * 8;
-  const auto tiles = [](int side, int64_t r, int64_t c) { return ceil_div64(r, side) * ceil_div64(c, side); };
-  w.n_dx = gated_shares(tiles(w.dx, s.rows, s.dim), w.dx, 2 * pad, s.rows * s.dim);
-  w.n_dw = gated_shares(tiles(w.dw, 2 * pad, s.dim), w.dw, s.rows, 2 * s.hidden * s.dim);
+  const int64_t es = (int64_t)type_size(type), piece = 16 / es;
+  w.kdim = (s.dim + piece - 1) / piece * piece;
+  const int64_t rb = ceil_div64(s.rows, 64), hb = 2 * pad / 64, db = ceil_div64(s.dim, 64);
+  w.n_dx = w.dx > 64 ? 1 : gated_shares(rb * db, 2 * pad, s.rows * s.dim);
+  w.n_dw = w.dw > 64 ? 1 : gated_shares(hb * db, s.rows, 2 * s.hidden * s.dim);
+  const auto cuts = [type](int side, int64_t r, int64_t c, int64_t k) {
+    return gated_wide_rounds(side, ceil_div64(r, side), ceil_div64(c, side), gated_wide_steps(type, k)).bytes(side);
+  };
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -386,14 +398,17 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
     return here;
   };
   const bool xw = w.fwd > 64 || (backward && w.dw > 64), ww = w.fwd > 64 || (backward && w.dx > 64);
-  w.x = take(xw ? s.rows * w.kdim * 2 : 0);
-  w.wg = take(ww ? s.hidden * w.kdim * 2 : 0);
-  w.wu = take(ww ? s.hidden * w.kdim * 2 : 0);
-  w.bias_rows = s.rows <= kSkinnyRows ? 1 : w.fwd > 64 ? ceil_div64(s.rows, w.fwd) * 2 : ceil_div64(s.rows, 64);
-  w.dgu = take(backward ? s.rows * 2 * pad * (int64_t)type_size(type) : 0);
+  w.x = take(xw ? s.rows * w.kdim * es : 0);
+  w.wg = take(ww ? s.hidden * w.kdim * es : 0);
+  w.wu = take(ww ? s.hidden * w.kdim * es : 0);
+  w.bias_rows = s.rows <= kSkinnyRows ? 1 : w.fwd > 64 ? ceil_div64(s.rows, w.fwd) * 2 : rb;
+  w.dgu = take(backward ? s.rows * 2 * pad * es : 0);
   w.bias = take(backward ? w.bias_rows * 2 * s.hidden * 4 : 0);
-  w.dx_parts = take(backward && w.n_dx > 1 ? w.n_dx * s.rows * s.dim * 4 : 0);
-  w.dw_parts = take(backward && w.n_dw > 1 ? w.n_dw * 2 * s.hidden * s.dim * 4 : 0);
+  w.dx_parts = take(!backward ? 0 : w.dx > 64 ? cuts(w.dx, s.rows, s.dim, 2 * pad) : w.n_dx > 1 ? w.n_dx * s.rows * s.dim * 4 : 0);
+  w.dw_parts = take(!backward  ? 0
+                    : w.dw > 64 ? cuts(w.dw, 2 * pad, s.dim, s.rows)
+                    : w.n_dw > 1 ? w.n_dw * 2 * s.hidden * s.dim * 4
+                                 : 0);
   w.total = at;
   return w;
 }
@@ -417,7 +432,7 @@ static GatedWide gated_wide_args(const T* x, int64_t x_stride, const T* wg, cons
     p.p[2] = wu, p.to[2] = (T*)(ws + w.wu), p.rows[2] = s.hidden, p.stride[2] = s.dim;
     a.wg = p.to[1], a.wu = p.to[2], a.w_stride = w.kdim;
   }
-  const int64_t pieces = (p.rows[0] + p.rows[1] + p.rows[2]) * (w.kdim / 8), blocks = ceil_div64(pieces, 256);
+  const int64_t pieces = (p.rows[0] + p.rows[1] + p.rows[2]) * (w.kdim / (16 / (int64_t)sizeof(T))), blocks = ceil_div64(pieces, 256);
   if (pieces) k_gated_pad<T><<<(unsigned)(blocks < 8192 ? blocks : 8192), 256, 0, st>>>(p);
   return a;
 }
@@ -439,7 +454,7 @@ static void gated_fwd(const T* x, int64_t x_stride, const T* wg, const T* wu, co
   if (w.fwd > 64) {
     GatedWide a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, true, true, ws, st);
     a.h = h;
-    gated_wide(type, kWideFwd, w.fwd, a, 1, st);
+    gated_wide(type, kWideFwd, w.fwd, a, st);
     return;
   }
   const dim3 grid((unsigned)ceil_div64(s.rows, 64), (unsigned)ceil_div64(s.hidden, 64));
@@ -465,7 +480,7 @@ static void gated_bwd(const T* x, int64_t x_stride, const T* wg, const T* wu, co
     gated_skinny(type, GatedSkinny{s, x, wg, wu, bg, bu, dh, x_stride, dh_stride, nullptr, dgu, bias, act}, st);
   } else if (w.fwd > 64) {
     a.parts = bias;
-    gated_wide(type, kWideGrad, w.fwd, a, 1, st);
+    gated_wide(type, kWideGrad, w.fwd, a, st);
   } else {
     k_tile_gated<T><<<dim3((unsigned)rb, (unsigned)(pad / 64)), 256, 0, st>>>(x, x_stride, wg, wu, bg, bu, act, s, nullptr, dh,
                                                                             dh_stride, dgu, bias);
@@ -475,8 +490,8 @@ static void gated_bwd(const T* x, int64_t x_stride, const T* wg, const T* wu, co
     const int64_t n = w.n_dx, share = ceil_div64(ceil_div64(2 * pad, n), 64) * 64;
     float* parts = n > 1 ? (float*)(ws + w.dx_parts) : nullptr;
     if (w.dx > 64) {
-      a.share = share, a.parts = parts;
-      gated_wide(type, kWideDx, w.dx, a, (int)n, st);
+      a.cuts = (float*)(ws + w.dx_parts);
+      gated_wide(type, kWideDx, w.dx, a, st);
     } else {
       k_tile_dx<T><<<dim3((unsigned)rb, (unsigned)db, (unsigned)n), 256, 0, st>>>(dgu, wg, wu, s, share, dx, parts);
     }
@@ -486,8 +501,8 @@ static void gated_bwd(const T* x, int64_t x_stride, const T* wg, const T* wu, co
     const int64_t n = w.n_dw, share = ceil_div64(ceil_div64(s.rows, n), 64) * 64;
     float* parts = n > 1 ? (float*)(ws + w.dw_parts) : nullptr;
     if (w.dw > 64) {
-      a.share = share, a.parts = parts;
-      gated_wide(type, kWideDw, w.dw, a, (int)n, st);
+      a.cuts = (float*)(ws + w.dw_parts);
+      gated_wide(type, kWideDw, w.dw, a, st);
     } else {
       k_tile_dw<T><<<dim3((unsigned)(2 * pad / 64), (unsigned)db, (unsigned)n), 256, 0, st>>>(dgu, x, x_stride, s, share, dwg,
                                                                                               dwu, parts);

@@ -7,19 +7,30 @@ namespace gsr {
 
 enum { kWideFwd, kWideGrad, kWideDx, kWideDw };
 
-// The tensors of one product, 16-bit, x, wg and wu 16-byte aligned with strides (in elements) that are
-// multiples of 8, and kdim, the length of their rows, too: the block's dim, or it padded with zeros.
+// The tensors of one product: x, wg and wu 16-byte aligned, with strides (in elements) and kdim, the length
+// of their rows, whole 16-byte pieces: the block's dim, or it padded with zeros.
 struct GatedWide {
   GatedShape s;
   int64_t kdim, x_stride, w_stride, dh_stride;
   const void *x, *wg, *wu, *bg, *bu, *dh;
   void *h, *dgu, *dx, *dwg, *dwu;
-  float* parts;    // gradients: column sums [ceil(rows / side) * 2][2][hidden]; dx: [share][rows][dim]; dW:
-                   // [share][2][hidden][dim]; or NULL
-  int64_t share;   // dx: columns of dgu a share; dW: rows of x a share; multiples of 64
-  int act, mt, nt;
+  float* parts;   // gradients: column sums [ceil(rows / side) * 2][2][hidden], or NULL
+  float* cuts;    // dx, dW: the cut tiles' sums [shares][cut][side][side]
+  int act;
+  int mt, nt, whole, cut, shares;   // set by the launch: tiles, and how they are cut (gated_wide_rounds)
 };
 
-void gated_wide(int type, int mode, int side, GatedWide a, int shares, hipStream_t st);
+// Tiles `whole` of a product are computed by one workgroup each, `cut` more by `shares` each.
+struct WideRounds {
+  int whole, cut, shares;
+  int64_t bytes(int side) const { return cut ? (int64_t)cut * shares * side * side * 4 : 0; }
+};
+WideRounds gated_wide_rounds(int side, int64_t mt, int64_t nt, int64_t steps);
+
+// Steps of 128 bytes of K.
+inline int64_t gated_wide_steps(int type, int64_t k) { return ceil_div64(k * (int64_t)type_size(type), 128); }
+
+// side 128, or 256 in 16 bits
+void gated_wide(int type, int mode, int side, GatedWide a, hipStream_t st);
 
 }  // namespace gsr

@@ -1,4 +1,4 @@
-// The gated block's products in 16 bits with square tiles of 256 or 128 (wide.h has the layout).
+// The gated block's products with square tiles of 256 (16 bits) or 128 (wide.h has the layout).
 //
 //   forward, gradients  a tile is 256 (128) rows by half as many columns of g and the same columns of u
 //                       (the first half of its shared memory's rows from Wg, the second from Wu), so
@@ -11,6 +11,21 @@
 
 namespace gsr {
 
+// Eight neighbouring results of dx, or of the weight gradients, whose rows are [dg | pad | du | pad]'s columns.
+template <typename T, int MODE>
+__device__ __forceinline__ void wide_store(const GatedWide& a, int64_t m, int64_t n, const float (&v)[8]) {
+  const GatedShape s = a.s;
+  if constexpr (MODE == kWideDx) {
+    if (m < s.rows) store_upto((T*)a.dx + m * s.dim + n, s.dim - n, v);
+  } else {
+    const int64_t pad = gated_pad(s.hidden);
+    const int which = m >= pad;
+    const int64_t row = m - which * pad;
+    T* to = (T*)(which ? a.dwu : a.dwg);
+    if (row < s.hidden && to) store_upto(to + row * s.dim + n, s.dim - n, v);
+  }
+}
+
 template <int N>
 struct Count {
   static constexpr int value = N;
@@ -19,13 +34,21 @@ struct Count {
 template <typename T, int MODE, int SIDE>
 __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(GatedWide a) {
   constexpr bool DUAL = MODE == kWideFwd || MODE == kWideGrad, AKC = MODE != kWideDw, BKC = DUAL;
-  constexpr int NB = SIDE / 64, HALF = SIDE / 2, BYTES = SIDE * kWideK * 2;   // blocks a wave and side; its rows
+  constexpr int NB = SIDE / 64, HALF = SIDE / 2, BYTES = SIDE * 128;   // blocks a wave and side; its rows
+  constexpr int ES = sizeof(T), K = kWideK<T>;
   __shared__ __attribute__((aligned(1024))) char lds[kWideSlots][BYTES];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wm = wave % 2, wn = wave / 2;
   const GatedShape s = a.s;
   const int64_t pad = gated_pad(s.hidden);
-  int tm, tn;
-  wide_tile_of(blockIdx.x, a.mt, a.nt, &tm, &tn);
+  // Whole tiles first; those that would leave CUs idle in the last round are cut into shares of K.
+  int tm, tn, id = blockIdx.x, share = -1;
+  if constexpr (!DUAL) {
+    if (id >= a.whole) {
+      share = (id - a.whole) / a.cut;
+      id = a.whole + (id - a.whole) % a.cut;
+    }
+  }
+  wide_tile_of(id, a.mt, a.nt, &tm, &tn);
   const int64_t m0 = (int64_t)tm * SIDE, n0 = (int64_t)tn * (DUAL ? HALF : SIDE);
 
   // K of this workgroup, and the operands' corners.  Where K is contiguous the descriptor holds the
@@ -33,17 +56,20 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
   // may be short: `short_bytes`).
   int64_t k0 = 0, k1 = DUAL ? a.kdim : MODE == kWideDx ? 2 * pad : s.rows;
   if constexpr (!DUAL) {
-    k0 = blockIdx.z * a.share;
-    k1 = k0 + a.share < k1 ? k0 + a.share : k1;
+    if (share >= 0) {
+      const int64_t all = (k1 + K - 1) / K;
+      k0 = all * share / a.shares * K;
+      if (share + 1 < a.shares) k1 = all * (share + 1) / a.shares * K;
+    }
   }
-  const int steps = (int)((k1 - k0 + kWideK - 1) / kWideK);
-  const auto at = [](const void* p, int64_t i) { return (const char*)p + i * 2; };
+  const int steps = (int)((k1 - k0 + K - 1) / K);
+  const auto at = [](const void* p, int64_t i) { return (const char*)p + i * ES; };
   const auto rows_of = [&](int64_t rows, int64_t first, int64_t stride) {   // K contiguous: rows first .. of `rows`
     const int64_t n = rows - first < SIDE ? rows - first : SIDE;
-    return n <= 0 ? 0 : ((n - 1) * stride + kWideK) * 2;
+    return n <= 0 ? 0 : ((n - 1) * stride + K) * ES;
   };
   const auto ks_of = [](int64_t n, int64_t stride, int64_t left) {   // K across rows: n K, `left` columns to the row's end
-    return n <= 0 ? 0 : ((n < kWideK ? n : kWideK) - 1) * stride * 2 + left * 2;
+    return n <= 0 ? 0 : ((n < K ? n : K) - 1) * stride * ES + left * ES;
   };
   WideSource sa, sb, sb2;
   uint32_t a_step, b_step, a_short = 0, b_short = 0;
@@ -52,32 +78,32 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
   if constexpr (DUAL) {
     a_stride = a.x_stride, b_stride = a.w_stride;
     sa = WideSource(at(a.x, m0 * a_stride), rows_of(s.rows, m0, a_stride));
-    const int64_t n = s.hidden - n0 < HALF ? s.hidden - n0 : HALF, bytes = n <= 0 ? 0 : ((n - 1) * b_stride + kWideK) * 2;
+    const int64_t n = s.hidden - n0 < HALF ? s.hidden - n0 : HALF, bytes = n <= 0 ? 0 : ((n - 1) * b_stride + K) * ES;
     sb = WideSource(at(a.wg, n0 * b_stride), bytes);
     sb2 = WideSource(at(a.wu, n0 * b_stride), bytes);
-    a_step = b_step = kWideK * 2;
+    a_step = b_step = K * ES;
   } else if constexpr (MODE == kWideDx) {
     a_stride = 2 * pad, b_stride = a.w_stride;
     sa = WideSource(at(a.dgu, m0 * a_stride + k0), rows_of(s.rows, m0, a_stride));
     // K rows of Wg, then of Wu, each followed by up to pad - hidden < 64 rows of nothing
     const int64_t kw = k0 < pad ? k0 : k0 - pad;   // (pad is whole steps: none straddles the matrices)
-    sb = WideSource(at(k0 < pad ? a.wg : a.wu, kw * b_stride + n0), ks_of(kWideK, b_stride, a.kdim - n0));
+    sb = WideSource(at(k0 < pad ? a.wg : a.wu, kw * b_stride + n0), ks_of(K, b_stride, a.kdim - n0));
     sb2 = WideSource(at(a.wu, n0), 0);
-    a_step = kWideK * 2, b_step = (uint32_t)(kWideK * b_stride * 2);
-    turn = k0 < pad ? (int)((pad - k0) / kWideK) : -1;
+    a_step = K * ES, b_step = (uint32_t)(K * b_stride * ES);
+    turn = k0 < pad ? (int)((pad - k0) / K) : -1;
   } else {
     a_stride = 2 * pad, b_stride = a.x_stride;
     sa = WideSource(at(a.dgu, k0 * a_stride + m0), ks_of(k1 - k0, a_stride, a_stride - m0));
     sb = WideSource(at(a.x, k0 * b_stride + n0), ks_of(k1 - k0, b_stride, a.kdim - n0));
-    a_step = (uint32_t)(kWideK * a_stride * 2), b_step = (uint32_t)(kWideK * b_stride * 2);
-    a_short = (uint32_t)ks_of((k1 - k0) % kWideK, a_stride, a_stride - m0);
-    b_short = (uint32_t)ks_of((k1 - k0) % kWideK, b_stride, a.kdim - n0);
-    shorts = (int)((k1 - k0) / kWideK);
+    a_step = (uint32_t)(K * a_stride * ES), b_step = (uint32_t)(K * b_stride * ES);
+    a_short = (uint32_t)ks_of((k1 - k0) % K, a_stride, a_stride - m0);
+    b_short = (uint32_t)ks_of((k1 - k0) % K, b_stride, a.kdim - n0);
+    shorts = (int)((k1 - k0) / K);
   }
-  WideTile<AKC, SIDE> ta;
-  WideTile<BKC, SIDE> tb;
-  ta.init(a_stride * 2, wm * HALF);
-  tb.init(b_stride * 2, DUAL ? wn * (HALF / 2) : wn * HALF);
+  WideTile<T, AKC, SIDE> ta;
+  WideTile<T, BKC, SIDE> tb;
+  ta.init(a_stride * ES, wm * HALF);
+  tb.init(b_stride * ES, DUAL ? wn * (HALF / 2) : wn * HALF);
 
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)&lds[0][0] + wave * 1024);
@@ -90,13 +116,13 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
       if (next_a == shorts) sa.bytes = a_short;
     da = sa.descriptor(next_a < steps);
     sa.advance(a_step);
-    left_a = (int)(k1 - k0) - next_a * kWideK;
+    left_a = (int)(k1 - k0) - next_a * K;
     ++next_a;
   };
   const auto begin_b = [&]() {
     if constexpr (MODE == kWideDx) {
       if (next_b == turn) sb.lo = sb2.lo, sb.hi = sb2.hi;
-      const int64_t k = k0 + (int64_t)next_b * kWideK, n = s.hidden - (k < pad ? k : k - pad);   // rows left in the matrix
+      const int64_t k = k0 + (int64_t)next_b * K, n = s.hidden - (k < pad ? k : k - pad);   // rows left in the matrix
       sb.bytes = (uint32_t)ks_of(n, b_stride, a.kdim - n0);
     }
     if constexpr (MODE == kWideDw)
@@ -105,7 +131,7 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
     if constexpr (DUAL) db2 = sb2.descriptor(next_b < steps);
     sb.advance(b_step);
     if constexpr (DUAL) sb2.advance(b_step);
-    left_b = (int)(k1 - k0) - next_b * kWideK;
+    left_b = (int)(k1 - k0) - next_b * K;
     ++next_b;
   };
   constexpr int LOADS = BYTES / 4096;
@@ -132,7 +158,7 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
       fb[kk & 1][b] = tb.operand(&lds[slot_b][0], DUAL && b >= NB / 2 ? HALF + (b - NB / 2) * 32 : b * 32, kk);
     }
   };
-  // A quarter of a step: the products of 16 K, and between them the reads of the next quarter's operands
+  // A quarter of a step: its products, and between them the reads of the next quarter's operands
   // (of kk `read` in the slots given), then `loads` of the LOADS loads that `load` issues.  One wave a
   // SIMD issues all of it, so every other instruction sits in a product's shadow (32 cycles, six
   // or so instructions); the order is as written.
@@ -215,15 +241,15 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
 #pragma unroll 1
     for (int r = lane / LANES; r < 32; r += ROWS) {
       const int64_t m = first + r;
-      if (m >= (MODE == kWideDw ? 2 * pad : s.rows)) break;
       float g[8], u[8], d[8];
+      if constexpr (MODE == kWideGrad) load_upto((const T*)a.dh + m * a.dh_stride + n, m < s.rows ? left_n : 0, d);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         g[i] = mine[r * LD + c + i];
         if constexpr (DUAL) u[i] = mine[r * LD + COLS + c + i];
       }
       if constexpr (DUAL) {
-        if constexpr (MODE == kWideGrad) load_upto((const T*)a.dh + m * a.dh_stride + n, left_n, d);
+        if (m >= s.rows) continue;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float act, slope;
@@ -247,22 +273,11 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
           store_vec((T*)a.dgu + m * 2 * pad + n, g);
           store_vec((T*)a.dgu + m * 2 * pad + pad + n, u);
         }
-      } else if constexpr (MODE == kWideDx) {
-        if (a.parts) {
-          store_upto(a.parts + (blockIdx.z * s.rows + m) * s.dim + n, left_n, g);
-        } else {
-          store_upto((T*)a.dx + m * s.dim + n, left_n, g);
-        }
+      } else if (share >= 0) {   // the whole tile, for wide_join
+        float* to = a.cuts + ((int64_t)share * a.cut + (id - a.whole)) * SIDE * SIDE;
+        store_vec(to + (m - m0) * SIDE + wn * COLS + c, g);
       } else {
-        const int which = m >= pad;
-        const int64_t row = m - which * pad;
-        if (row < s.hidden) {
-          if (a.parts) {
-            store_upto(a.parts + ((blockIdx.z * 2 + which) * s.hidden + row) * s.dim + n, left_n, g);
-          } else if (T* to = (T*)(which ? a.dwu : a.dwg)) {
-            store_upto(to + row * s.dim + n, left_n, g);
-          }
-        }
+        wide_store<T, MODE>(a, m, n, g);
       }
     }
     wide_fence();
@@ -284,32 +299,70 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
   }
 }
 
+// The cut tiles' results: the sums of their shares, in order.
+template <typename T, int MODE, int SIDE>
+__global__ __launch_bounds__(256) void k_wide_join(GatedWide a) {
+  constexpr int EACH = SIDE * SIDE / 8 / 256;   // workgroups a tile
+  const int tile = blockIdx.x / EACH, at = (blockIdx.x % EACH * 256 + threadIdx.x) * 8;
+  int tm, tn;
+  wide_tile_of(a.whole + tile, a.mt, a.nt, &tm, &tn);
+  const float* p = a.cuts + (int64_t)tile * SIDE * SIDE + at;
+  const int64_t each = (int64_t)a.cut * SIDE * SIDE;
+  float v[8] = {};
+#pragma unroll 4
+  for (int i = 0; i < a.shares; ++i) {
+    float w[8];
+    load_vec(p + i * each, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += w[j];
+  }
+  wide_store<T, MODE>(a, (int64_t)tm * SIDE + at / SIDE, (int64_t)tn * SIDE + at % SIDE, v);
+}
+
 template <typename T, int SIDE>
-static void wide_launch(int mode, const GatedWide& a, int shares, hipStream_t st) {
-  const dim3 grid((unsigned)(a.mt * a.nt), 1, (unsigned)shares);
+static void wide_launch(int mode, const GatedWide& a, hipStream_t st) {
+  const int join = a.cut * (SIDE * SIDE / 8 / 256);
   if (mode == kWideFwd) {
-    k_wide<T, kWideFwd, SIDE><<<grid, kWideThreads, 0, st>>>(a);
+    k_wide<T, kWideFwd, SIDE><<<a.mt * a.nt, kWideThreads, 0, st>>>(a);
   } else if (mode == kWideGrad) {
-    k_wide<T, kWideGrad, SIDE><<<grid, kWideThreads, 0, st>>>(a);
+    k_wide<T, kWideGrad, SIDE><<<a.mt * a.nt, kWideThreads, 0, st>>>(a);
   } else if (mode == kWideDx) {
-    k_wide<T, kWideDx, SIDE><<<grid, kWideThreads, 0, st>>>(a);
+    k_wide<T, kWideDx, SIDE><<<a.whole + a.cut * a.shares, kWideThreads, 0, st>>>(a);
+    if (join) k_wide_join<T, kWideDx, SIDE><<<join, 256, 0, st>>>(a);
   } else {
-    k_wide<T, kWideDw, SIDE><<<grid, kWideThreads, 0, st>>>(a);
+    k_wide<T, kWideDw, SIDE><<<a.whole + a.cut * a.shares, kWideThreads, 0, st>>>(a);
+    if (join) k_wide_join<T, kWideDw, SIDE><<<join, 256, 0, st>>>(a);
   }
 }
 
-void gated_wide(int type, int mode, int side, GatedWide a, int shares, hipStream_t st) {
+// The rounds of a product of mt x nt tiles: `slots` workgroups run at once, so the tiles of an
+// incomplete last round are cut along K into as many shares as fill it, each at least eight steps.
+WideRounds gated_wide_rounds(int side, int64_t mt, int64_t nt, int64_t steps) {
+  const int64_t slots = side == 256 ? 256 : 512, tiles = mt * nt;
+  WideRounds r{(int)tiles, 0, 1};
+  const int64_t cut = tiles % slots;
+  int64_t shares = cut ? slots / cut : 1;
+  shares = shares < steps / 8 ? shares : steps / 8;
+  if (shares > 1) r = WideRounds{(int)(tiles - cut), (int)cut, (int)shares};
+  return r;
+}
+
+void gated_wide(int type, int mode, int side, GatedWide a, hipStream_t st) {
   const int64_t pad = gated_pad(a.s.hidden);
   a.mt = ceil_div(mode == kWideDw ? 2 * pad : a.s.rows, side);
   a.nt = mode <= kWideGrad ? ceil_div(pad, side / 2) : ceil_div(a.s.dim, side);
-  if (type == GSR_BF16 && side == 256) {
-    wide_launch<bf16, 256>(mode, a, shares, st);
+  const WideRounds r = gated_wide_rounds(side, a.mt, a.nt, gated_wide_steps(type, mode == kWideDw ? a.s.rows : 2 * pad));
+  a.whole = r.whole, a.cut = r.cut, a.shares = r.shares;
+  if (type == GSR_F32) {
+    wide_launch<float, 128>(mode, a, st);
+  } else if (type == GSR_BF16 && side == 256) {
+    wide_launch<bf16, 256>(mode, a, st);
   } else if (type == GSR_BF16) {
-    wide_launch<bf16, 128>(mode, a, shares, st);
+    wide_launch<bf16, 128>(mode, a, st);
   } else if (side == 256) {
-    wide_launch<f16, 256>(mode, a, shares, st);
+    wide_launch<f16, 256>(mode, a, st);
   } else {
-    wide_launch<f16, 128>(mode, a, shares, st);
+    wide_launch<f16, 128>(mode, a, st);
   }
 }
 

@@ -1,5 +1,6 @@
-// Products of 16-bit matrices with fp32 sums in square tiles of 256 or 128: the parts of the gated
-// block's main loop.
+// Products with fp32 sums in square tiles of 256 or 128: the parts of the gated block's main loop.
+// Written for 16-bit matrices; fp32 ones (128 only) take 32 K a step in the place of 64 and
+// 32x32x2 matrix instructions, four to each 16 bytes of an operand, and need no transposed reads.
 //
 // A workgroup of four waves owns a 256 x 256 tile, each wave a 128 x 128 quarter of 4 x 4 blocks
 // of 32x32x16 matrix instructions: 256 accumulators a lane.  K advances 64 at a time; shared memory
@@ -26,7 +27,9 @@
 
 namespace gsr {
 
-constexpr int kWideK = 64, kWideSlots = 5, kWideThreads = 256;
+template <typename T>
+constexpr int kWideK = 128 / sizeof(T);   // K of a step: 128 bytes
+constexpr int kWideSlots = 5, kWideThreads = 256;
 constexpr uint32_t kWideNowhere = 0x80000000u;   // past every descriptor's end
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -37,12 +40,18 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef __bf16 wide_v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 wide_v8h __attribute__((ext_vector_type(8)));
 
+// c += a b over 8 (fp32) or 16 K: 16 bytes of K a lane, the lower 32 lanes' first.
 template <typename T>
 __device__ __forceinline__ v16f wide_mma(v8s a, v8s b, v16f c) {
   if constexpr (__is_same(T, bf16)) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(wide_v8bf, a), __builtin_bit_cast(wide_v8bf, b), c, 0, 0, 0);
-  } else {
+  } else if constexpr (__is_same(T, f16)) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(wide_v8h, a), __builtin_bit_cast(wide_v8h, b), c, 0, 0, 0);
+  } else {
+    const v4f x = __builtin_bit_cast(v4f, a), y = __builtin_bit_cast(v4f, b);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[s], y[s], c, 0, 0, 0);
+    return c;
   }
 }
 
@@ -87,40 +96,47 @@ __device__ __forceinline__ void wide_fence() {
 }
 
 // One operand's tile of SIDE rows (KC) or columns: this lane's places in it.
-template <bool KC, int SIDE>
+template <typename T, bool KC, int SIDE>
 struct WideTile {
-  static constexpr int BYTES = SIDE * kWideK * 2, LOADS = BYTES / 4096, BLOCKS = SIDE / 64;
-  static constexpr int ROW = SIDE * 2;   // bytes of a K row (K across rows)
+  static constexpr int BYTES = SIDE * 128, LOADS = BYTES / 4096, BLOCKS = SIDE / 64, ES = sizeof(T);
+  static constexpr int ROW = SIDE * ES;   // bytes of a K row (K across rows)
+  static constexpr int READS = KC ? 4 : ES == 4 ? BLOCKS : 2 * BLOCKS;
   uint32_t at[LOADS];   // byte offsets of the lane's loads from the tile's corner
   int k;                // KC: the loads' first K
-  uint32_t read[KC ? 4 : 2 * BLOCKS];   // byte offsets of its reads: per 16 K (KC), or per K parity and block
+  uint32_t read[READS];   // byte offsets of its reads: per quarter of a step (KC), or per (K parity and) block
 
   // origin: the wave's first row (KC) or column of the tile's
   __device__ __forceinline__ void init(int64_t stride_bytes, int origin) {
     const int t = threadIdx.x, l = t % 64;
     if constexpr (KC) {
       const int c = t % 8 ^ (t / 8 & 7);
-      k = c * 8;
+      k = c * (16 / ES);
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) at[j] = (uint32_t)((j * 32 + t / 8) * stride_bytes + c * 16);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) read[kk] = (origin + l % 32) * 128 + ((kk * 2 + l / 32) ^ (l & 7)) * 16;
     } else {
       constexpr int SLOTS = ROW / 16, EACH = 256 / SLOTS;   // 16-byte slots a K row, K rows a load
-      constexpr int MASK = SIDE == 256 ? 3 : 1;
+      constexpr int MASK = ES == 4 ? 0 : SIDE == 256 ? 3 : 1, MIX = ES == 4 ? 0 : 3;   // (fp32: chunks in order)
+      k = 0;
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) {
         const int kr = j * EACH + t / SLOTS;
-        at[j] = (uint32_t)(kr * stride_bytes + (t % SLOTS ^ (kr & 3) * 2 ^ (kr >> 3 & MASK) * 8) * 16);
+        at[j] = (uint32_t)(kr * stride_bytes + (t % SLOTS ^ (kr & MIX) * 2 ^ (kr >> 3 & MASK) * 8) * 16);
       }
-      const int g = l / 16, row = l % 16 / 4;   // K row of the lane's 4 x 16 piece
+      if constexpr (ES == 4) {
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
+        for (int b = 0; b < BLOCKS; ++b) read[b] = l / 32 * 4 * ROW + (origin + b * 32 + l % 32) * 4;
+      } else {
+        const int g = l / 16, row = l % 16 / 4;   // K row of the lane's 4 x 16 piece
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) {
-          const int c = origin / 8 + b * 4 + g % 2 * 2 + l % 4 / 2;
-          read[p * BLOCKS + b] = (g / 2 * 8 + row) * ROW + (c ^ row * 2 ^ (p * 2 + g / 2 & MASK) * 8) * 16 + l % 2 * 8;
-        }
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int b = 0; b < BLOCKS; ++b) {
+            const int c = origin / 8 + b * 4 + g % 2 * 2 + l % 4 / 2;
+            read[p * BLOCKS + b] = (g / 2 * 8 + row) * ROW + (c ^ row * 2 ^ (p * 2 + g / 2 & MASK) * 8) * 16 + l % 2 * 8;
+          }
+      }
     }
   }
 
@@ -128,10 +144,14 @@ struct WideTile {
   __device__ __forceinline__ uint32_t offset(int j, int left) const { return !KC || k < left ? at[j] : kWideNowhere; }
 
   // The operand of the 32 rows from the wave's origin + `off` (a multiple of 32, below SIDE / 2 where
-  // K runs across rows) and K kk * 16 .. + 15.
+  // K runs across rows) and quarter kk of the step's K.
   __device__ __forceinline__ v8s operand(const char* lds, int off, int kk) const {
     if constexpr (KC) {
       return *(const v8s*)(lds + read[kk] + off * 128);
+    } else if constexpr (ES == 4) {
+      const char* p = lds + read[off / 32] + kk * 8 * ROW;
+      return __builtin_bit_cast(v8s, v4f{*(const float*)p, *(const float*)(p + ROW), *(const float*)(p + 2 * ROW),
+                                         *(const float*)(p + 3 * ROW)});
     } else {
       typedef __attribute__((address_space(3))) v4s lds_v4s;
       const char* p = lds + read[kk % 2 * BLOCKS + off / 32] + kk * 16 * ROW;
