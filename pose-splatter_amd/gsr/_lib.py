@@ -10,7 +10,7 @@ import ctypes
 import os
 import threading
 
-__all__ = ["LIB_PATH", "GsrLibraryError", "lib", "check", "BinStats", "BinCaps", "LossTerms", "AdamwTensor",
+__all__ = ["LIB_PATH", "GsrLibraryError", "lib", "native", "check", "BinStats", "BinCaps", "LossTerms", "AdamwTensor",
            "AdamwArgs", "EXPORTS", "ABI_VERSION", "F32", "BF16", "F16", "ADAMW_BLOCK",
            "RADIUS_OPACITY_AABB", "RADIUS_ISOTROPIC_3SIGMA", "ORDER_DEPTH", "ORDER_INDEX", "TILE"]
 
@@ -222,6 +222,28 @@ def lib():
                                   f"{handle.gsr_last_error().decode(errors='replace')}")
         _lib = handle
         return _lib
+
+
+_native = None
+
+
+def native():
+    """The torch binding of libgsr's layer and optimizer calls (gsr/_torch.so, built beside
+    libgsr.so), bound to the library that lib() loaded; raises GsrLibraryError if unavailable."""
+    global _native
+    if _native is None:
+        lib()
+        try:
+            from . import _torch
+        except ImportError as e:
+            raise GsrLibraryError(f"gsr/_torch.so cannot be imported ({e}): build it with "
+                                  "`make -C pose-splatter_amd/csrc` (or __graft_entry__.build())") from e
+        if _torch.ABI_VERSION != ABI_VERSION:
+            raise GsrLibraryError(f"gsr/_torch.so was built for ABI revision {_torch.ABI_VERSION}, this binding expects "
+                                  f"{ABI_VERSION}: rebuild it")
+        _torch.bind(LIB_PATH)
+        _native = _torch
+    return _native
 
 
 def check(rc: int, name: str) -> None:

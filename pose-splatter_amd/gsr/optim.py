@@ -17,15 +17,11 @@ block are followed in steps.  No CPU path: the functions raise on CPU tensors.
 """
 from __future__ import annotations
 
-import array
-import ctypes
-
 import torch
 
 from . import _lib
-from ._lib import check, lib
-from .layers import _on, _raw_stream, _type
-from .render import _require_device
+from ._lib import check, lib, native
+from .render import _require_device, _stream
 
 __all__ = ["AdamW", "adamw_step", "decode_root"]
 
@@ -36,60 +32,6 @@ def _units(numel: int) -> int:
     return -(-numel // _BLOCK)
 
 
-def _dense(t: torch.Tensor) -> bool:
-    """Whether t's elements fill one stretch of memory, each once, in some order of its dimensions."""
-    if t.is_contiguous():
-        return True
-    n = 1
-    for stride, size in sorted((s, d) for s, d in zip(t.stride(), t.shape) if d != 1):
-        if stride != n:
-            return False
-        n *= size
-    return True
-
-
-def _layout(t: torch.Tensor):
-    """The strides that matter: those of dimensions of more than one element."""
-    return [s for s, d in zip(t.stride(), t.shape) if d != 1]
-
-
-def _check_layout(t: torch.Tensor, p: torch.Tensor, what: str) -> None:
-    if t.shape != p.shape or (_layout(t) != _layout(p) if t.numel() else False):
-        raise ValueError(f"adamw_step: {what} must have its parameter's shape and strides {tuple(p.shape)}, "
-                         f"{p.stride()}; got {tuple(t.shape)}, {t.stride()}")
-
-
-def _step_args(lr, betas, eps, weight_decay, step, bits):
-    args = _lib.AdamwArgs()
-    if isinstance(lr, torch.Tensor):
-        if lr.numel() != 1 or lr.dtype != torch.float32:
-            raise ValueError("adamw_step: a tensor lr must be one float32 value")
-        args.lr, args.lr_dev = 0.0, lr.data_ptr()
-    else:
-        if not lr >= 0:
-            raise ValueError(f"adamw_step: lr must not be negative, got {lr}")
-        args.lr, args.lr_dev = float(lr), None
-    b1, b2 = betas
-    if not (0 <= b1 < 1 and 0 <= b2 < 1):
-        raise ValueError(f"adamw_step: betas must be in [0, 1), got {betas}")
-    if not (eps >= 0 and weight_decay >= 0):
-        raise ValueError(f"adamw_step: eps and weight_decay must not be negative, got {eps}, {weight_decay}")
-    args.beta1, args.beta2, args.eps, args.weight_decay = float(b1), float(b2), float(eps), float(weight_decay)
-    args.step = 0 if isinstance(step, (torch.Tensor, list, tuple)) else int(step)
-    args.bits = bits
-    return args
-
-
-def _no_overlap(ranges) -> None:
-    ranges.sort()
-    end = 0
-    for a, b in ranges:
-        if a < end:
-            raise ValueError("adamw_step: a tensor is listed twice, or tensors to be written overlap")
-        end = b
-
-
-@torch.no_grad()
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 1e-2, step, exp_avg_units=None, exp_avg_root_units=None) -> None:
     """One AdamW step over lists of tensors, in place:
@@ -105,81 +47,12 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, lr=1e-3, betas=(0.9, 0.9
     zeros are zero moments.  lr: a number or one float32 value on the device.  step: the count of
     this step, 1 at first: a number, one int64 value on the device for all tensors, or a list of
     such values; the device forms are read by the kernel (a step captured in a HIP graph)."""
-    count = len(params)
-    bits = 32 if exp_avg_units is None else 8
-    if (exp_avg_units is None) != (exp_avg_root_units is None):
-        raise ValueError("adamw_step: exp_avg_units and exp_avg_root_units go together")
-    lists = [grads, exp_avgs, exp_avg_sqs] + ([exp_avg_units, exp_avg_root_units] if bits == 8 else [])
-    if any(len(x) != count for x in lists):
-        raise ValueError(f"adamw_step: {count} params, but lists of {[len(x) for x in lists]}")
-    args = _step_args(lr, betas, eps, weight_decay, step, bits)
+    lr_dev = lr if isinstance(lr, torch.Tensor) else None
     if isinstance(step, torch.Tensor):
-        step = [step] * count
-    steps = list(step) if isinstance(step, (list, tuple)) else None
-    if steps is None and args.step < 1:
-        raise ValueError(f"adamw_step: step must be at least 1, got {step}")
-    if steps is not None and len(steps) != count:
-        raise ValueError(f"adamw_step: {count} params, but {len(steps)} steps")
-    if count == 0:
-        return
-    dev = params[0].device
-    if args.lr_dev and lr.device != dev:
-        raise ValueError(f"adamw_step: lr is on {lr.device}, the parameters on {dev}")
-    if bits == 32:
-        m_type = v_type = torch.float32
-    else:
-        m_type, v_type = torch.float8_e4m3fn, torch.uint8
-    groups, ranges, kept = {}, [], []
-    m_size, v_size = m_type.itemsize, v_type.itemsize
-    for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
-        if not (p.device == g.device == m.device == v.device == dev):
-            raise ValueError(f"adamw_step: tensor {i}, its gradient and moments are on {p.device}, {g.device}, {m.device} "
-                             f"and {v.device}; the first tensor is on {dev}")
-        types = (p.dtype, g.dtype)
-        group = groups.get(types)
-        if group is None:
-            group = groups[types] = (_type(p, "adamw_step: a parameter"), _type(g, "adamw_step: a gradient"), [])
-        if m.dtype != m_type or v.dtype != v_type:
-            raise ValueError(f"adamw_step: exp_avg must be {m_type} and exp_avg_sq {v_type}, got {m.dtype} and {v.dtype}")
-        if g.layout != torch.strided or g.shape != p.shape:
-            raise ValueError(f"adamw_step: gradient {i} must be dense and {tuple(p.shape)}, got {tuple(g.shape)}")
-        if not (p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous()
-                and m.shape == p.shape and v.shape == p.shape):
-            if not _dense(p):
-                raise ValueError(f"adamw_step: parameter {i} does not fill its memory (strides {p.stride()})")
-            _check_layout(m, p, "exp_avg")
-            _check_layout(v, p, "exp_avg_sq")
-            if _layout(g) != _layout(p):   # (a gradient of another layout: copied into the parameter's)
-                g = torch.empty_strided(p.shape, p.stride(), dtype=g.dtype, device=dev).copy_(g)
-                kept.append(g)
-        n = p.numel()
-        if n == 0:
-            continue
-        pp, mp, vp, mu, vu, sp = p.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, 0
-        ranges += ((pp, pp + n * p.element_size()), (mp, mp + n * m_size), (vp, vp + n * v_size))
-        if bits == 8:
-            for u in (exp_avg_units[i], exp_avg_root_units[i]):
-                if u.dtype != torch.float32 or u.shape != (_units(n),) or not u.is_contiguous() or u.device != dev:
-                    raise ValueError(f"adamw_step: units {i} must be contiguous float32 [{_units(n)}] on {dev}, "
-                                     f"got {u.dtype} {tuple(u.shape)} on {u.device}")
-            mu, vu = exp_avg_units[i].data_ptr(), exp_avg_root_units[i].data_ptr()
-            ranges += ((mu, mu + 4 * _units(n)), (vu, vu + 4 * _units(n)))
-        if steps is not None:
-            s = steps[i]
-            if not isinstance(s, torch.Tensor) or s.numel() != 1 or s.dtype != torch.int64 or s.device != dev:
-                raise ValueError(f"adamw_step: step {i} must be one int64 value on {dev}")
-            sp = s.data_ptr()
-        group[2].extend((pp, g.data_ptr(), mp, vp, mu, vu, sp, n))
-    _no_overlap(ranges)
-    _require_device(params[0], "adamw_step")
-    L = lib()
-    with _on(dev):
-        stream = _raw_stream(dev)
-        for pt, gt, words in groups.values():
-            table = array.array("q", words)   # gsr_adamw_tensor: eight 64-bit fields
-            check(L.gsr_adamw_step(table.buffer_info()[0], len(words) // 8, pt, gt, ctypes.byref(args), stream),
-                  "gsr_adamw_step")
-    torch.autograd.graph.increment_version(list(params))
+        step = [step] * len(params)
+    steps = step if isinstance(step, (list, tuple)) else None
+    native().adamw_step(params, grads, exp_avgs, exp_avg_sqs, 0.0 if lr_dev is not None else lr, lr_dev, *betas, eps,
+                        weight_decay, 0 if steps is not None else step, steps, exp_avg_units, exp_avg_root_units)
 
 
 def decode_root(codes: torch.Tensor, units: torch.Tensor) -> torch.Tensor:
@@ -193,9 +66,9 @@ def decode_root(codes: torch.Tensor, units: torch.Tensor) -> torch.Tensor:
                          f"got {units.dtype} {tuple(units.shape)} on {units.device}")
     _require_device(codes, "decode_root")
     out = torch.empty(codes.shape, device=codes.device, dtype=torch.float32)
-    with _on(codes.device):
+    with torch.cuda.device(codes.device):
         check(lib().gsr_adamw_decode_root(codes.data_ptr(), units.data_ptr(), codes.numel(), out.data_ptr(),
-                                          _raw_stream(codes.device)), "gsr_adamw_decode_root")
+                                          _stream(codes.device)), "gsr_adamw_decode_root")
     return out
 
 
@@ -212,7 +85,7 @@ class AdamW(torch.optim.Optimizer):
                  moment_bits: int = 32, capturable: bool = False):
         if moment_bits not in (8, 32):
             raise ValueError(f"AdamW: moment_bits must be 8 or 32, got {moment_bits}")
-        _step_args(lr, betas, eps, weight_decay, 1, moment_bits)   # the same checks as every step's
+        adamw_step([], [], [], [], lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, step=1)   # checks them
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
                                       moment_bits=int(moment_bits), capturable=bool(capturable)))
 

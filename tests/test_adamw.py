@@ -396,3 +396,42 @@ def test_refusals():
     args.bits = 16
     assert call(t) == -1 and b"32 or 8" in L.gsr_last_error()
     assert L.gsr_adamw_decode_root(None, None, 4, None, None) == -1
+
+
+def test_struct_layouts_match_header(tmp_path):
+    """The ctypes mirrors of gsr_adamw_tensor and gsr_adamw_args have the C compiler's size and offsets."""
+    import ctypes
+    import os
+    import shutil
+    import subprocess
+    from gsr import _lib
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    structs = {"gsr_adamw_tensor": _lib.AdamwTensor, "gsr_adamw_args": _lib.AdamwArgs}
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "gsr.h"', "int main(void) {",
+             'printf("block %d\\n", GSR_ADAMW_BLOCK);']
+    for name, py in structs.items():
+        lines.append(f'printf("{name} size %zu\\n", sizeof({name}));')
+        lines += [f'printf("{name} {f} %zu\\n", offsetof({name}, {f}));' for f, _ in py._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text("\n".join([*lines, "return 0;", "}"]))
+    subprocess.run([cc, "-I", include, str(src), "-o", str(tmp_path / "layout")], check=True)
+    got = dict(x.rsplit(" ", 1) for x in subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True,
+                                                         text=True).stdout.splitlines())
+    assert int(got["block"]) == _lib.ADAMW_BLOCK
+    for name, py in structs.items():
+        assert int(got[f"{name} size"]) == ctypes.sizeof(py)
+        assert all(int(got[f"{name} {f}"]) == getattr(py, f).offset for f, _ in py._fields_)
+
+
+def test_binding_refuses_another_library(tmp_path):
+    """The torch binding fails loudly on a library that is missing or is not libgsr."""
+    from gsr import _lib
+    native = _lib.native()
+    with pytest.raises(RuntimeError, match="cannot load"):
+        native.bind(str(tmp_path / "nope.so"))
+    with pytest.raises(RuntimeError, match="has no gsr_"):
+        native.bind("libc.so.6")
+    native.bind(_lib.LIB_PATH)
