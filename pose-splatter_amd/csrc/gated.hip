@@ -277,34 +277,41 @@ __global__ __launch_bounds__(256) void k_tile_dw(const T* dgu, const T* x, int64
     }
 }
 
-// [a | b], a the first `split` of n values, = the sum over `count` rows of parts [count][n]: sixteen
-// lanes a value, each a fixed share of the rows with four loads in flight, then the sixteen in order.
-template <typename T>
-__global__ __launch_bounds__(1024) void k_gated_join(const float* parts, int64_t count, int64_t n, int64_t split, T* a, T* b) {
-  __shared__ float sum[16][65];
-  const int lane = threadIdx.x % 64, grp = threadIdx.x / 64;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+// [a | b], a the first `split` of n values, = the sum over `count` rows of parts [count][n]: GROUPS
+// lanes a value, each a fixed share of the rows with loads in flight, then the lanes in order.
+template <typename T, int GROUPS>
+__global__ __launch_bounds__(GROUPS == 1 ? 256 : GROUPS * 64) void k_gated_join(const float* parts, int64_t count, int64_t n,
+                                                                                int64_t split, T* a, T* b) {
+  constexpr int COLS = GROUPS == 1 ? 256 : 64;
+  __shared__ float sum[GROUPS][GROUPS == 1 ? 1 : 65];
+  const int lane = threadIdx.x % COLS, grp = threadIdx.x / COLS;
+  const int64_t c = (int64_t)blockIdx.x * COLS + lane;
   float s = 0.f;
   if (c < n) {
 #pragma unroll 4
-    for (int64_t r = grp; r < count; r += 16) s += parts[r * n + c];
+    for (int64_t r = grp; r < count; r += GROUPS) s += parts[r * n + c];
   }
-  sum[grp][lane] = s;
-  __syncthreads();
-  if (grp == 0 && c < n) {
+  if constexpr (GROUPS > 1) {
+    sum[grp][lane] = s;
+    __syncthreads();
+    if (grp) return;
 #pragma unroll
-    for (int k = 1; k < 16; ++k) s += sum[k][lane];
-    if (c < split) {
-      if (a) a[c] = from_f<T>(s);
-    } else if (b) {
-      b[c - split] = from_f<T>(s);
-    }
+    for (int k = 1; k < GROUPS; ++k) s += sum[k][lane];
+  }
+  if (c < split) {
+    if (a) a[c] = from_f<T>(s);
+  } else if (c < n && b) {
+    b[c - split] = from_f<T>(s);
   }
 }
 
 template <typename T>
 static void gated_join(const float* parts, int64_t count, int64_t n, int64_t split, void* a, void* b, hipStream_t st) {
-  k_gated_join<T><<<(unsigned)ceil_div64(n, 64), 1024, 0, st>>>(parts, count, n, split, (T*)a, (T*)b);
+  if (count < 16) {
+    k_gated_join<T, 1><<<(unsigned)ceil_div64(n, 256), 256, 0, st>>>(parts, count, n, split, (T*)a, (T*)b);
+  } else {
+    k_gated_join<T, 16><<<(unsigned)ceil_div64(n, 64), 1024, 0, st>>>(parts, count, n, split, (T*)a, (T*)b);
+  }
 }
 
 // Shares of K in a product of `tiles` 64 x 64 tiles: enough workgroups for two a CU, each share at

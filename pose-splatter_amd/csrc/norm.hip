@@ -6,15 +6,20 @@
 // Both passes are bound by memory: a row is read once and stays in registers while its mean,
 // then its variance about that mean (two sums, so no cancellation of E[x^2] - mean^2) are
 // reduced.  LANES lanes share a row -- part of a wave for short rows, a wave, or a whole
-// workgroup -- each holding NV vectors of V elements.  The backward's workgroups walk rows with
-// the grid's stride and keep dw and db of their columns in registers; each writes one row of
-// partial sums, which a second kernel adds in a fixed order: no atomics, the same bits every run.
+// workgroup -- each holding NV vectors of V elements.  Workgroups walk rows with the grid's stride,
+// keep the weights (and the backward's dw and db) of their columns in registers and load the next
+// row while they reduce this one.  Each backward workgroup writes one row of partial dw and db,
+// which a second kernel adds in a fixed order: no atomics, the same bits every run.
 // Sums, statistics and partials are fp32; only y, dx, dw and db are rounded to their types.
 #include "types.h"
 
 namespace gsr {
 
-constexpr int kNormParts = 512;   // partial rows of dw/db at most: two workgroups per CU
+// Workgroups of a backward at most, one partial row of dw and db each: those that run at once, three a
+// CU with up to two vectors a lane, two with four (32768 x 4096 bf16: 161 us at 768, 194 at 512, 191 at
+// 1024 where registers spill; 16384 x 8192: 171 at 512, 200 at 768).
+constexpr int norm_most_parts(int nv) { return nv <= 2 ? 768 : 512; }
+constexpr int kNormGrid = 2048;   // workgroups of a forward: up to eight a CU
 
 template <typename T>
 struct NormVec {
@@ -55,47 +60,68 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_norm_fwd(const T*
                                                                         const void* w, const void* b, int wtype, float eps,
                                                                         T* y, float2* stats) {
   constexpr int V = NormVec<T>::V, THREADS = LANES > 256 ? LANES : 256, RPB = THREADS / LANES;
+  constexpr bool HOLD = LANES <= 256;   // (1024 threads leave no registers for the weights)
   __shared__ float lds[LANES > 64 ? 2 * (LANES / 64) : 1];
   const int lane = threadIdx.x % LANES;
-  for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES; row < rows; row += (int64_t)gridDim.x * RPB) {
-  const T* xr = x + row * stride;
-  float v[NV][V];
-  float s[1] = {0.f};
+  float wv[HOLD ? NV : 1][V], bv[HOLD ? NV : 1][V];
+  if constexpr (HOLD)
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int64_t c = (int64_t)(k * LANES + lane) * V;
-    load_upto(xr + c, dim - c, v[k]);
-#pragma unroll
-    for (int i = 0; i < V; ++i) s[0] += v[k][i];
-  }
-  row_sum<LANES>(s, lds);
-  const float mean = s[0] / (float)dim;
-  s[0] = 0.f;
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int64_t c = (int64_t)(k * LANES + lane) * V;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      v[k][i] -= mean;
-      s[0] += c + i < dim ? v[k][i] * v[k][i] : 0.f;
+    for (int k = 0; k < NV; ++k) {
+      const int64_t c = (int64_t)(k * LANES + lane) * V;
+      load_param(w, wtype, c, dim - c, wv[k], 1.f);
+      load_param(b, wtype, c, dim - c, bv[k], 0.f);
     }
-  }
-  row_sum<LANES>(s, lds + (LANES > 64 ? LANES / 64 : 0));
-  const float rstd = 1.f / sqrtf(s[0] / (float)dim + eps);
-  if (stats && lane == 0) stats[row] = make_float2(mean, rstd);
-  T* yr = y + row * dim;
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES;
+  Raw<T> next[NV];
+  const auto fetch = [&](int64_t r) {
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int64_t c = (int64_t)(k * LANES + lane) * V;
-    if (c < dim) {
-      float wv[V], bv[V];
-      load_param(w, wtype, c, dim - c, wv, 1.f);
-      load_param(b, wtype, c, dim - c, bv, 0.f);
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[k][i] = v[k][i] * rstd * wv[i] + bv[i];
-      store_upto(yr + c, dim - c, v[k]);
+    for (int k = 0; k < NV; ++k) {
+      const int64_t c = (int64_t)(k * LANES + lane) * V;
+      next[k].load(x + r * stride + c, dim - c);
     }
-  }
+  };
+  if (row < rows) fetch(row);
+  for (; row < rows; row += step) {
+    float v[NV][V], s[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        v[k][i] = next[k].at(i);
+        s[0] += v[k][i];
+      }
+    if (row + step < rows) fetch(row + step);
+    row_sum<LANES>(s, lds);
+    const float mean = s[0] / (float)dim;
+    s[0] = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int64_t c = (int64_t)(k * LANES + lane) * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        v[k][i] -= mean;
+        s[0] += c + i < dim ? v[k][i] * v[k][i] : 0.f;
+      }
+    }
+    row_sum<LANES>(s, lds + (LANES > 64 ? LANES / 64 : 0));
+    const float rstd = 1.f / sqrtf(s[0] / (float)dim + eps);
+    if (stats && lane == 0) stats[row] = make_float2(mean, rstd);
+    T* yr = y + row * dim;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int64_t c = (int64_t)(k * LANES + lane) * V;
+      if (c < dim) {
+        const int h = HOLD ? k : 0;
+        if constexpr (!HOLD) {
+          load_param(w, wtype, c, dim - c, wv[0], 1.f);
+          load_param(b, wtype, c, dim - c, bv[0], 0.f);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[k][i] = v[k][i] * rstd * wv[h][i] + bv[h][i];
+        store_upto(yr + c, dim - c, v[k]);
+      }
+    }
   }
 }
 
@@ -138,44 +164,62 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(const T* x, int64_t rows
   }
 }
 
-// parts: [gridDim.x][2][dim] partial sums of dw and db (NULL: neither is wanted).
+// parts: [gridDim.x][2][dim] partial sums of dw and db (NULL: neither is wanted).  x and dy stay as they
+// were loaded (a row's two values of 16 bits in one register) and are widened again for dx: the
+// registers saved are waves that keep more loads in flight.
 template <typename T, int LANES, int NV>
-__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_norm_bwd(const T* x, const T* dy, int64_t rows, int64_t dim,
-                                                                        int64_t stride, int64_t dy_stride, const void* w,
-                                                                        int wtype, const float2* stats, T* dx, float* parts) {
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256, LANES > 256 ? 1 : NV <= 2 ? 3 : 2) void k_norm_bwd(
+    const T* x, const T* dy, int64_t rows, int64_t dim, int64_t stride, int64_t dy_stride, const void* w, int wtype,
+    const float2* stats, T* dx, float* parts) {
   constexpr int V = NormVec<T>::V, THREADS = LANES > 256 ? LANES : 256, RPB = THREADS / LANES;
   constexpr int W = LANES / 64;
+  constexpr bool HOLD = LANES <= 256;   // weights and the next row in registers (1024 threads have none left)
   __shared__ float lds[LANES > 64 ? 4 * W : 1];
   const int lane = threadIdx.x % LANES;
   const float inv = 1.f / (float)dim;
-  float wv[NV][V], aw[NV][V] = {}, ab[NV][V] = {};
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
+  float wv[HOLD ? NV : 1][V], aw[NV][V] = {}, ab[NV][V] = {};
+  const auto weights = [&](int k) {
     const int64_t c = (int64_t)(k * LANES + lane) * V;
-    load_param(w, wtype, c, dim - c, wv[k], 1.f);
-  }
+    load_param(w, wtype, c, dim - c, wv[HOLD ? k : 0], 1.f);
+  };
+  if constexpr (HOLD)
+#pragma unroll
+    for (int k = 0; k < NV; ++k) weights(k);
   int half = 0;
-  for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES; row < rows; row += (int64_t)gridDim.x * RPB) {
-    const float2 st = stats[row];
-    float xv[NV][V], g[NV][V], s[2] = {0.f, 0.f};
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES;
+  Raw<T> nx[NV], ng[NV];
+  float2 next_st;
+  const auto fetch = [&](int64_t r) {   // (columns past dim: dy is zero there, whatever xhat is)
+    next_st = stats[r];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int64_t c = (int64_t)(k * LANES + lane) * V;
-      load_upto(x + row * stride + c, dim - c, xv[k], st.x);
-      load_upto(dy + row * dy_stride + c, dim - c, g[k]);
+      nx[k].load(x + r * stride + c, dim - c);
+      ng[k].load(dy + r * dy_stride + c, dim - c);
     }
+  };
+  if (HOLD && row < rows) fetch(row);
+  for (; row < rows; row += step) {
+    if constexpr (!HOLD) fetch(row);
+    const float2 st = next_st;
+    Raw<T> cx[NV], cg[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) cx[k] = nx[k], cg[k] = ng[k];
+    if (HOLD && row + step < rows) fetch(row + step);
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if constexpr (!HOLD) weights(k);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float z = (xv[k][i] - st.x) * st.y;
-        xv[k][i] = z;
-        aw[k][i] += g[k][i] * z;
-        ab[k][i] += g[k][i];
-        g[k][i] *= wv[k][i];
-        s[0] += g[k][i];
-        s[1] += g[k][i] * z;
+        const float z = (cx[k].at(i) - st.x) * st.y, d = cg[k].at(i);
+        aw[k][i] += d * z;
+        ab[k][i] += d;
+        s[0] += d * wv[HOLD ? k : 0][i];
+        s[1] += d * wv[HOLD ? k : 0][i] * z;
       }
+    }
     row_sum<LANES>(s, lds + half * 2 * W);
     half ^= 1;
     if (dx) {
@@ -183,9 +227,14 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_norm_bwd(const T*
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int64_t c = (int64_t)(k * LANES + lane) * V;
+        if constexpr (!HOLD) weights(k);
+        float g[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) g[k][i] = (g[k][i] - m0 - xv[k][i] * m1) * st.y;
-        if (c < dim) store_upto(dx + row * dim + c, dim - c, g[k]);
+        for (int i = 0; i < V; ++i) {
+          const float z = (cx[k].at(i) - st.x) * st.y;
+          g[i] = (cg[k].at(i) * wv[HOLD ? k : 0][i] - m0 - z * m1) * st.y;
+        }
+        if (c < dim) store_upto(dx + row * dim + c, dim - c, g);
       }
     }
   }
@@ -295,8 +344,10 @@ __global__ __launch_bounds__(1024) void k_norm_join(const float* parts, int n, i
   const int col = threadIdx.x % 64, grp = threadIdx.x / 64;
   const int64_t c = (int64_t)blockIdx.x * 64 + col;
   float s = 0.f;
-  if (c < 2 * dim)
+  if (c < 2 * dim) {
+#pragma unroll 8
     for (int r = grp; r < n; r += 16) s += parts[(int64_t)r * 2 * dim + c];
+  }
   sum[grp][col] = s;
   __syncthreads();
   if (grp == 0 && c < 2 * dim) {
@@ -331,9 +382,7 @@ static void norm_layout(int64_t vecs, int* lanes, int* nv) {
   }
 }
 
-// Workgroups of a pass: one a row (or group of rows) up to 2^20, which then walk on by the grid's
-// stride (a launch may hold 2^32 threads).
-static unsigned norm_grid(int64_t blocks) { return (unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)); }
+static unsigned norm_grid(int64_t blocks) { return (unsigned)(blocks < kNormGrid ? blocks : kNormGrid); }
 
 #define GSR_NORM_DISPATCH(CALL)                 \
   switch (lanes * 8 + nv) {                     \
@@ -358,7 +407,9 @@ static int norm_parts(int64_t rows, int64_t dim, int xtype) {
   norm_layout(ceil_div64(dim, xtype == GSR_F32 ? 4 : 8), &lanes, &nv);
   const int rpb = lanes == 0 || lanes > 256 ? 1 : 256 / lanes;
   const int64_t blocks = ceil_div64(rows, rpb);
-  const int most = lanes == 0 ? 64 : kNormParts;
+  // enough rows a part that writing and joining it stays small beside reading them, but a part a CU
+  int64_t most = lanes == 0 ? 64 : blocks / 8 < 256 ? 256 : blocks / 8;
+  if (lanes && most > norm_most_parts(nv)) most = norm_most_parts(nv);
   return (int)(blocks < most ? blocks : most);
 }
 

@@ -72,6 +72,42 @@ __device__ __forceinline__ void store_upto(T* p, int64_t n, const float (&in)[V]
   }
 }
 
+// 16 bytes of T as they lie in memory, four registers (an array of 16-bit elements would take eight),
+// for loads that are to be in flight while others are worked on.  Elements from n on are zeros.
+template <typename T>
+struct Raw {
+  static constexpr int V = 16 / sizeof(T);
+  uint32_t w[4];
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else if constexpr (__is_same(T, bf16)) {
+      return __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    } else {
+      return (float)__builtin_bit_cast(_Float16, (uint16_t)(i % 2 ? w[i / 2] >> 16 : w[i / 2]));
+    }
+  }
+  __device__ __forceinline__ void load(const T* p, int64_t n) {
+    if (n >= V) {
+      const Pack<uint32_t, 4> k = *reinterpret_cast<const Pack<uint32_t, 4>*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = k.v[i];
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) {
+        if constexpr (sizeof(T) == 4) {
+          w[i] = __float_as_uint(p[i]);
+        } else {
+          w[i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[i]) << (16 * (i % 2));
+        }
+      }
+  }
+};
+
 // A parameter vector (weights, biases) of type `type`, or `fill` where there is none.
 template <int V>
 __device__ __forceinline__ void load_param(const void* p, int type, int64_t at, int64_t n, float (&out)[V], float fill) {
