@@ -703,18 +703,22 @@ int gsr_layer_norm_bwd(const void* x, const void* dy, int64_t rows, int64_t dim,
  * bwd: from dh [rows, hidden] (row stride dh_stride) the gradients dx [rows, dim], dwg, dwu
  * [hidden, dim], dbg, dbu [hidden] (each may be NULL), contiguous.  dg and du are rounded to the
  * type before the products that use them, as the projections' outputs' gradients would be.
+ * kept: device, 256-byte aligned, gsr_gated_kept bytes, or NULL: g and u as the forward leaves them
+ * for its backward.  Without it (where the bytes are 0, or by choice) the backward computes both
+ * projections again.
  * workspace: device, 256-byte aligned, gsr_gated_workspace bytes (0: NULL).  Fixed-order sums. */
 #define GSR_ACT_SILU 0
 #define GSR_ACT_GELU 1     /* g Phi(g), the error function's form */
 #define GSR_ACT_RELU 2
 #define GSR_ACT_SIGMOID 3
 int gsr_gated_fwd(const void* x, int64_t rows, int64_t dim, int64_t x_stride, int32_t type, const void* wg,
-                  const void* wu, int64_t hidden, const void* bg, const void* bu, int32_t act, void* h, void* workspace,
-                  size_t workspace_bytes, void* stream);
+                  const void* wu, int64_t hidden, const void* bg, const void* bu, int32_t act, void* h, void* kept,
+                  void* workspace, size_t workspace_bytes, void* stream);
+size_t gsr_gated_kept(int64_t rows, int64_t dim, int64_t hidden, int32_t type);
 size_t gsr_gated_workspace(int64_t rows, int64_t dim, int64_t hidden, int32_t type, int32_t backward);
 int gsr_gated_bwd(const void* x, int64_t rows, int64_t dim, int64_t x_stride, int32_t type, const void* wg,
                   const void* wu, int64_t hidden, const void* bg, const void* bu, int32_t act, const void* dh,
-                  int64_t dh_stride, void* dx, void* dwg, void* dwu, void* dbg, void* dbu, void* workspace,
+                  int64_t dh_stride, const void* kept, void* dx, void* dwg, void* dwu, void* dbg, void* dbu, void* workspace,
                   size_t workspace_bytes, void* stream);
 
 /* One AdamW step over `count` tensors (a HOST list) in place:

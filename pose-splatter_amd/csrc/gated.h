@@ -49,4 +49,55 @@ struct GatedShape {
   int64_t rows, dim, hidden;
 };
 
+// The projections g and u that a forward keeps for its backward, rows of gated_pad(hidden): fp32 as they
+// are; of 16-bit blocks the upper 24 bits of their fp32 sums, in a plane of g's and u's upper
+// halves and one of their next bytes (6 bytes an element; the truncation, 2^-16 at most, is a small
+// part of the types' own half steps, where rounding g and u to the type would add as much again).
+template <typename T>
+struct Kept {
+  uint32_t* hi;   // fp32: g
+  uint16_t* lo;   // fp32: unused
+  float* u;       // fp32: u
+  __host__ __device__ Kept(void* p, int64_t rows, int64_t hidden) {
+    const int64_t n = rows * gated_pad(hidden);
+    hi = (uint32_t*)p;
+    lo = (uint16_t*)(hi + n);
+    u = (float*)(hi + n);
+  }
+  static int64_t bytes(int64_t rows, int64_t hidden) { return rows * gated_pad(hidden) * (sizeof(T) == 4 ? 8 : 6); }
+  __device__ __forceinline__ void store(int64_t at, const float (&g)[8], const float (&v)[8]) const {   // at: a multiple of 8
+    if constexpr (sizeof(T) == 4) {
+      store_vec((float*)hi + at, g);
+      store_vec(u + at, v);
+    } else {
+      uint32_t h[8], l[4];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t a = __float_as_uint(g[i]), b = __float_as_uint(v[i]);
+        h[i] = a >> 16 | (b & 0xFFFF0000u);
+        const uint32_t next = (a >> 8 & 0xFFu) | (b & 0xFF00u);
+        l[i / 2] = i % 2 ? l[i / 2] | next << 16 : next;
+      }
+      *(uint4*)(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+      *(uint4*)(hi + at + 4) = make_uint4(h[4], h[5], h[6], h[7]);
+      *(uint4*)(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+  }
+  __device__ __forceinline__ void load(int64_t at, float (&g)[8], float (&v)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+      load_vec((const float*)hi + at, g);
+      load_vec(u + at, v);
+    } else {
+      const uint4 a = *(const uint4*)(hi + at), b = *(const uint4*)(hi + at + 4), c = *(const uint4*)(lo + at);
+      const uint32_t h[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, l[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t next = i % 2 ? l[i / 2] >> 16 : l[i / 2];
+        g[i] = __uint_as_float(h[i] << 16 | (next & 0xFFu) << 8);
+        v[i] = __uint_as_float((h[i] & 0xFFFF0000u) | (next & 0xFF00u));
+      }
+    }
+  }
+};
+
 }  // namespace gsr

@@ -5,10 +5,10 @@
 //   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dbg, dbu = column sums of dg, du
 //
 // Three products.  The forward's one launch computes both projections of a tile side by side, so
-// that g, u and the activation never leave registers; the backward computes them again with
-// the gradients as its epilogue (2 of its 6 product units, against 16 bytes an element of memory
-// kept from the forward and moved twice), then takes dx from K = [dg | du] and both weight
-// gradients from M = [dg | du].
+// that g, u and the activation never leave registers.  The backward needs g and u again: for long
+// K from the forward, which kept them (k_gated_slopes reads them), else by computing them again with
+// the gradients as the products' epilogue.  It then takes dx from K = [dg | du] and both
+// weight gradients from M = [dg | du].
 //
 // Most cases run on square tiles of 256 or 128 (gated_wide.hip), up to 64 rows on gated_skinny.hip's kernel;
 // here is what serves the others:
@@ -314,6 +314,56 @@ static void gated_join(const float* parts, int64_t count, int64_t n, int64_t spl
   }
 }
 
+// The gradients of the projections from what the forward kept: dgu, and parts [row blocks of 64][2][hidden]
+// of the column sums (NULL: not wanted).  Bound by memory: 12 bytes an element in 16 bits, 20 in fp32
+// (8 columns a lane, 256 a workgroup).
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_slopes(const void* saved, const T* dh, int64_t dh_stride, int act, GatedShape s,
+                                                      T* dgu, float* parts) {
+  const int64_t pad = gated_pad(s.hidden), n = (int64_t)blockIdx.x * 256 + threadIdx.x % 32 * 8, left = s.hidden - n;
+  const Kept<T> kept((void*)saved, s.rows, s.hidden);
+  const int64_t m0 = (int64_t)blockIdx.y * 64 + threadIdx.x / 32;
+  float sg[8] = {}, su[8] = {};
+  if (n < pad) {
+#pragma unroll 2
+    for (int r = 0; r < 64; r += 8) {
+      const int64_t m = m0 + r;
+      if (m >= s.rows) break;
+      float g[8], u[8], d[8];
+      kept.load(m * pad + n, g, u);
+      load_upto(dh + m * dh_stride + n, left, d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float a, slope;
+        activate<T>(act, g[i], a, slope);
+        g[i] = i < left ? d[i] * u[i] * slope : 0.f;   // (the padding holds zeros)
+        u[i] = i < left ? d[i] * a : 0.f;
+        sg[i] += g[i];
+        su[i] += u[i];
+      }
+      store_vec(dgu + m * 2 * pad + n, g);
+      store_vec(dgu + m * 2 * pad + pad + n, u);
+    }
+  }
+  if (!parts) return;
+  __shared__ float sum[8][2][256 + 8];
+  const int c = threadIdx.x % 32 * 8, rl = threadIdx.x / 32;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    sum[rl][0][c + i] = sg[i];
+    sum[rl][1][c + i] = su[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    float v = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v += sum[r][which][threadIdx.x];
+    if (col < s.hidden) parts[((int64_t)blockIdx.y * 2 + which) * s.hidden + col] = v;
+  }
+}
+
 // Shares of K in a product of `tiles` 64 x 64 tiles: enough workgroups for two a CU, each share at
 // least 128 of K, the fp32 parts of `values` results at most 64 MB.
 static int64_t gated_shares(int64_t tiles, int64_t k, int64_t values) {
@@ -356,13 +406,16 @@ __global__ __launch_bounds__(256) void k_gated_pad(GatedPads<T> a) {
 // Tile side of a product of rows x cols outputs over k.  256 (16 bits) where every CU gets at least 96
 // steps of K: 16384 x 2048 -> 5632, at 352 a CU, forward 660 us against 726 with 128, dW 593
 // against 877; at 88 the two are within 5 %; at 31 (16000 x 512 -> 2048) 111 us against 101.
-// 64 (any alignment, no padded copies) for dims whose K is hardly a step, and in fp32, whose products
-// are long enough to run side by side, where the 512 workgroups of 128 would get fewer than 8 steps
-// (256 x 1024 -> 2816, 5.5 steps: forward 56 us against 70; 16000 x 256 -> 512, 16: 84 against 77).
+// 64 (any alignment, no padded copies) for dims whose K is hardly a step; and where the 512 workgroups
+// of 128 would get fewer than 8 steps in fp32, whose products are long enough to run side by side
+// (256 x 1024 -> 2816, 5.5 steps: forward 56 us against 70; 16000 x 256 -> 512, 16: 84 against 77),
+// or with few rows (dx of 4 x 1024 -> 2816, 1.4: 10 us against 14; of 1 x 4096 -> 11264, 22: 106
+// against 40).
 static int gated_side(int type, int64_t rows, int64_t cols, int64_t k, GatedShape s) {
-  if (s.dim < 64 || s.rows <= kSkinnyRows) return 64;
+  const bool few = s.rows <= kSkinnyRows;
+  if (s.dim < 64 || (few && s.dim % 8)) return 64;
   const int64_t steps = gated_wide_steps(type, k);
-  if (type == GSR_F32) return ceil_div64(rows, 128) * ceil_div64(cols, 128) * steps >= 512 * 8 ? 128 : 64;
+  if (type == GSR_F32 || few) return ceil_div64(rows, 128) * ceil_div64(cols, 128) * steps >= 512 * 8 ? 128 : 64;
   return ceil_div64(rows, 256) * ceil_div64(cols, 256) * steps >= 256 * 96 ? 256 : 128;
 }
 
@@ -374,11 +427,19 @@ static bool gated_aligned(const T* p, int64_t dim, int64_t stride) {
   return (uintptr_t)p % 16 == 0 && dim % V == 0 && stride % V == 0 && stride <= 1 << 20;
 }
 
+// The least dim whose forward keeps its projections for the backward (on tiles of 128 and 256): what that
+// moves, 12 bytes an element (16 in fp32), does not grow with dim, what it saves does.  Forward and
+// gradients of the projections, kept against computed again: 16384 x 2048 -> 5632 bf16 915 us against
+// 1487, 4096 x 256 -> 2816 55 against 62, x 128 50 against 54 and not worth its memory; fp32 4096 x
+// 128 -> 2816 111 against 146.
+static bool gated_keeps(int type, int64_t dim) { return dim >= (type == GSR_F32 ? 128 : 256); }
+
 // How a pass is laid out: each product's tile side, the 64 x 64 tiles' shares of K, and its workspace (byte
 // offsets).  There is room for padded copies wherever a wide product may need them: an odd dim, rows
 // or addresses that are not multiples of 16 bytes.
 struct GatedPlan {
   int fwd, dx, dw;               // tile sides
+  bool keep;                     // the forward keeps its projections
   int64_t n_dx, n_dw;            // shares
   int64_t kdim;                  // dim in whole 16-byte pieces
   int64_t x, wg, wu, dgu, bias, bias_rows, dx_parts, dw_parts, total;
@@ -404,13 +465,15 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
     at += (bytes + 255) / 256 * 256;
     return here;
   };
+  if (s.rows <= kSkinnyRows) w.fwd = 64;   // (the kernel for few rows)
   const bool xw = w.fwd > 64 || (backward && w.dw > 64), ww = w.fwd > 64 || (backward && w.dx > 64);
   w.x = take(xw ? s.rows * w.kdim * es : 0);
   w.wg = take(ww ? s.hidden * w.kdim * es : 0);
   w.wu = take(ww ? s.hidden * w.kdim * es : 0);
+  w.keep = w.fwd > 64 && gated_keeps(type, s.dim);
   w.bias_rows = s.rows <= kSkinnyRows ? 1 : w.fwd > 64 ? ceil_div64(s.rows, w.fwd) * 2 : rb;
   w.dgu = take(backward ? s.rows * 2 * pad * es : 0);
-  w.bias = take(backward ? w.bias_rows * 2 * s.hidden * 4 : 0);
+  w.bias = take(backward ? (w.keep && rb > w.bias_rows ? rb : w.bias_rows) * 2 * s.hidden * 4 : 0);
   w.dx_parts = take(!backward ? 0 : w.dx > 64 ? cuts(w.dx, s.rows, s.dim, 2 * pad) : w.n_dx > 1 ? w.n_dx * s.rows * s.dim * 4 : 0);
   w.dw_parts = take(!backward  ? 0
                     : w.dw > 64 ? cuts(w.dw, 2 * pad, s.dim, s.rows)
@@ -451,7 +514,7 @@ static constexpr int type_of() {
 
 template <typename T>
 static void gated_fwd(const T* x, int64_t x_stride, const T* wg, const T* wu, const T* bg, const T* bu, int act, GatedShape s,
-                      T* h, char* ws, hipStream_t st) {
+                      T* h, void* kept, char* ws, hipStream_t st) {
   const int type = type_of<T>();
   if (s.rows <= kSkinnyRows) {
     gated_skinny(type, GatedSkinny{s, x, wg, wu, bg, bu, nullptr, x_stride, 0, h, nullptr, nullptr, act}, st);
@@ -460,7 +523,7 @@ static void gated_fwd(const T* x, int64_t x_stride, const T* wg, const T* wu, co
   const GatedPlan w = gated_plan(s, type, false);
   if (w.fwd > 64) {
     GatedWide a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, true, true, ws, st);
-    a.h = h;
+    a.h = h, a.kept = w.keep ? kept : nullptr;
     gated_wide(type, kWideFwd, w.fwd, a, st);
     return;
   }
@@ -470,20 +533,25 @@ static void gated_fwd(const T* x, int64_t x_stride, const T* wg, const T* wu, co
 
 template <typename T>
 static void gated_bwd(const T* x, int64_t x_stride, const T* wg, const T* wu, const T* bg, const T* bu, int act, GatedShape s,
-                      const T* dh, int64_t dh_stride, T* dx, T* dwg, T* dwu, T* dbg, T* dbu, char* ws, hipStream_t st) {
+                      const T* dh, int64_t dh_stride, const void* kept, T* dx, T* dwg, T* dwu, T* dbg, T* dbu, char* ws,
+                      hipStream_t st) {
   const int type = type_of<T>();
-  const GatedPlan w = gated_plan(s, type, true);
+  GatedPlan w = gated_plan(s, type, true);
   const int64_t rb = ceil_div64(s.rows, 64), db = ceil_div64(s.dim, 64), pad = gated_pad(s.hidden);
-  const bool weights = dwg || dwu, few = s.rows <= kSkinnyRows;
+  const bool weights = dwg || dwu, few = s.rows <= kSkinnyRows, keep = w.keep && kept;
+  if (keep) w.bias_rows = rb;
   T* dgu = (T*)(ws + w.dgu);
   float* bias = dbg || dbu ? (float*)(ws + w.bias) : nullptr;
   GatedWide a{};
   if (w.fwd > 64 || w.dx > 64 || w.dw > 64) {
-    a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, w.fwd > 64 || (weights && w.dw > 64),
-                           w.fwd > 64 || (dx && w.dx > 64), ws, st);
+    const bool again = w.fwd > 64 && !keep;   // both projections are computed again
+    a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, again || (weights && w.dw > 64), again || (dx && w.dx > 64), ws,
+                           st);
     a.dh = dh, a.dh_stride = dh_stride, a.dgu = dgu, a.dx = dx, a.dwg = dwg, a.dwu = dwu;
   }
-  if (few) {
+  if (keep) {
+    k_gated_slopes<T><<<dim3((unsigned)ceil_div64(pad, 256), (unsigned)rb), 256, 0, st>>>(kept, dh, dh_stride, act, s, dgu, bias);
+  } else if (few) {
     gated_skinny(type, GatedSkinny{s, x, wg, wu, bg, bu, dh, x_stride, dh_stride, nullptr, dgu, bias, act}, st);
   } else if (w.fwd > 64) {
     a.parts = bias;
@@ -539,9 +607,15 @@ extern "C" size_t gsr_gated_workspace(int64_t rows, int64_t dim, int64_t hidden,
   return (size_t)gated_plan(s, type, backward != 0).total;
 }
 
+extern "C" size_t gsr_gated_kept(int64_t rows, int64_t dim, int64_t hidden, int32_t type) {
+  const GatedShape s{rows, dim, hidden};
+  if (gated_check("gsr_gated_kept", s, dim, type, GSR_ACT_SILU) || rows == 0 || !gated_plan(s, type, false).keep) return 0;
+  return (size_t)(type == GSR_F32 ? Kept<float>::bytes(rows, hidden) : Kept<bf16>::bytes(rows, hidden));
+}
+
 extern "C" int gsr_gated_fwd(const void* x, int64_t rows, int64_t dim, int64_t x_stride, int32_t type, const void* wg,
                              const void* wu, int64_t hidden, const void* bg, const void* bu, int32_t act, void* h,
-                             void* workspace, size_t workspace_bytes, void* stream) {
+                             void* kept, void* workspace, size_t workspace_bytes, void* stream) {
   const GatedShape s{rows, dim, hidden};
   if (const int e = gated_check("gsr_gated_fwd", s, x_stride, type, act)) return e;
   if (rows == 0) return 0;
@@ -551,11 +625,11 @@ extern "C" int gsr_gated_fwd(const void* x, int64_t rows, int64_t dim, int64_t x
   char* ws = (char*)workspace;
   const auto st = (hipStream_t)stream;
   if (type == GSR_F32) {
-    gated_fwd((const float*)x, x_stride, (const float*)wg, (const float*)wu, (const float*)bg, (const float*)bu, act, s, (float*)h, ws, st);
+    gated_fwd((const float*)x, x_stride, (const float*)wg, (const float*)wu, (const float*)bg, (const float*)bu, act, s, (float*)h, kept, ws, st);
   } else if (type == GSR_BF16) {
-    gated_fwd((const bf16*)x, x_stride, (const bf16*)wg, (const bf16*)wu, (const bf16*)bg, (const bf16*)bu, act, s, (bf16*)h, ws, st);
+    gated_fwd((const bf16*)x, x_stride, (const bf16*)wg, (const bf16*)wu, (const bf16*)bg, (const bf16*)bu, act, s, (bf16*)h, kept, ws, st);
   } else {
-    gated_fwd((const f16*)x, x_stride, (const f16*)wg, (const f16*)wu, (const f16*)bg, (const f16*)bu, act, s, (f16*)h, ws, st);
+    gated_fwd((const f16*)x, x_stride, (const f16*)wg, (const f16*)wu, (const f16*)bg, (const f16*)bu, act, s, (f16*)h, kept, ws, st);
   }
   GSR_LAUNCH_CHECK("gsr_gated_fwd");
   return 0;
@@ -563,7 +637,7 @@ extern "C" int gsr_gated_fwd(const void* x, int64_t rows, int64_t dim, int64_t x
 
 extern "C" int gsr_gated_bwd(const void* x, int64_t rows, int64_t dim, int64_t x_stride, int32_t type, const void* wg,
                              const void* wu, int64_t hidden, const void* bg, const void* bu, int32_t act, const void* dh,
-                             int64_t dh_stride, void* dx, void* dwg, void* dwu, void* dbg, void* dbu, void* workspace,
+                             int64_t dh_stride, const void* kept, void* dx, void* dwg, void* dwu, void* dbg, void* dbu, void* workspace,
                              size_t workspace_bytes, void* stream) {
   const GatedShape s{rows, dim, hidden};
   if (const int e = gated_check("gsr_gated_bwd", s, x_stride, type, act)) return e;
@@ -584,13 +658,13 @@ extern "C" int gsr_gated_bwd(const void* x, int64_t rows, int64_t dim, int64_t x
     zero(dbu, hidden * each);
   } else if (type == GSR_F32) {
     gated_bwd((const float*)x, x_stride, (const float*)wg, (const float*)wu, (const float*)bg, (const float*)bu, act, s, (const float*)dh,
-              dh_stride, (float*)dx, (float*)dwg, (float*)dwu, (float*)dbg, (float*)dbu, ws, st);
+              dh_stride, kept, (float*)dx, (float*)dwg, (float*)dwu, (float*)dbg, (float*)dbu, ws, st);
   } else if (type == GSR_BF16) {
     gated_bwd((const bf16*)x, x_stride, (const bf16*)wg, (const bf16*)wu, (const bf16*)bg, (const bf16*)bu, act, s, (const bf16*)dh,
-              dh_stride, (bf16*)dx, (bf16*)dwg, (bf16*)dwu, (bf16*)dbg, (bf16*)dbu, ws, st);
+              dh_stride, kept, (bf16*)dx, (bf16*)dwg, (bf16*)dwu, (bf16*)dbg, (bf16*)dbu, ws, st);
   } else {
     gated_bwd((const f16*)x, x_stride, (const f16*)wg, (const f16*)wu, (const f16*)bg, (const f16*)bu, act, s, (const f16*)dh,
-              dh_stride, (f16*)dx, (f16*)dwg, (f16*)dwu, (f16*)dbg, (f16*)dbu, ws, st);
+              dh_stride, kept, (f16*)dx, (f16*)dwg, (f16*)dwu, (f16*)dbg, (f16*)dbu, ws, st);
   }
   GSR_LAUNCH_CHECK("gsr_gated_bwd");
   return 0;

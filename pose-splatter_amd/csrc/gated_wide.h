@@ -13,7 +13,7 @@ struct GatedWide {
   GatedShape s;
   int64_t kdim, x_stride, w_stride, dh_stride;
   const void *x, *wg, *wu, *bg, *bu, *dh;
-  void *h, *dgu, *dx, *dwg, *dwu;
+  void *h, *kept, *dgu, *dx, *dwg, *dwu;   // kept: NULL, or the forward's projections (Kept)
   float* parts;   // gradients: column sums [ceil(rows / side) * 2][2][hidden], or NULL
   float* cuts;    // dx, dW: the cut tiles' sums [shares][cut][side][side]
   int act;

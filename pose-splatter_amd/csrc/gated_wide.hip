@@ -252,9 +252,14 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
         if (m >= s.rows) continue;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          float act, slope;
           g[i] += gb[i];
           u[i] += ub[i];
+        }
+        if constexpr (MODE == kWideFwd)
+          if (a.kept && n < pad) Kept<T>(a.kept, s.rows, s.hidden).store(m * pad + n, g, u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float act, slope;
           activate<T>(a.act, g[i], act, slope);
           if constexpr (MODE == kWideFwd) {
             g[i] = act * u[i];

@@ -29,6 +29,7 @@ struct {
   decltype(&::gsr_layer_norm_workspace) layer_norm_workspace;
   decltype(&::gsr_layer_norm_bwd) layer_norm_bwd;
   decltype(&::gsr_gated_fwd) gated_fwd;
+  decltype(&::gsr_gated_kept) gated_kept;
   decltype(&::gsr_gated_workspace) gated_workspace;
   decltype(&::gsr_gated_bwd) gated_bwd;
   decltype(&::gsr_adamw_step) adamw_step;
@@ -46,6 +47,7 @@ void bind(const std::string& path) {
   take(gsr.layer_norm_workspace, "gsr_layer_norm_workspace");
   take(gsr.layer_norm_bwd, "gsr_layer_norm_bwd");
   take(gsr.gated_fwd, "gsr_gated_fwd");
+  take(gsr.gated_kept, "gsr_gated_kept");
   take(gsr.gated_workspace, "gsr_gated_workspace");
   take(gsr.gated_bwd, "gsr_gated_bwd");
   take(gsr.adamw_step, "gsr_adamw_step");
@@ -182,7 +184,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
 
 // ----------------------------------------------------------------- gated block
 Tensor gated_forward(const Rows& r, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& bg, const Tensor& bu,
-                     int64_t act) {
+                     int64_t act, const Tensor& kept) {
   const c10::OptionalDeviceGuard guard(x.device());
   const int type = type_of(x, "x");
   const int64_t dim = x.size(-1), hidden = wg.size(0);
@@ -192,7 +194,7 @@ Tensor gated_forward(const Rows& r, const Tensor& x, const Tensor& wg, const Ten
   const size_t bytes = gsr.gated_workspace(r.rows, dim, hidden, type, 0);
   if (bytes) ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
   check(gsr.gated_fwd(r.t.data_ptr(), r.rows, dim, r.stride, type, wg.data_ptr(), wu.data_ptr(), hidden, ptr(bg), ptr(bu), (int)act,
-                      h.data_ptr(), ptr(ws), bytes, stream_of(x.device())),
+                      h.data_ptr(), ptr(kept), ptr(ws), bytes, stream_of(x.device())),
         "gsr_gated_fwd");
   return h;
 }
@@ -202,15 +204,18 @@ struct Gated : torch::autograd::Function<Gated> {
                         const std::optional<Tensor>& b_gate, const std::optional<Tensor>& b_up, int64_t act) {
     const Tensor bg = or_none(b_gate), bu = or_none(b_up);
     const Rows r = rows_of(x, x.size(-1));
-    ctx->save_for_backward({r.t, wg, wu, bg, bu});
+    Tensor kept;
+    if (const size_t bytes = gsr.gated_kept(r.rows, x.size(-1), wg.size(0), type_of(x, "x")))
+      kept = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+    ctx->save_for_backward({r.t, wg, wu, bg, bu, kept});
     ctx->saved_data["shape"] = x.sizes();
     ctx->saved_data["act"] = act;
-    return gated_forward(r, x, wg, wu, bg, bu, act);
+    return gated_forward(r, x, wg, wu, bg, bu, act, kept);
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &bg = saved[3], &bu = saved[4];
+    const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &bg = saved[3], &bu = saved[4], &kept = saved[5];
     const int64_t rows = x.size(0), dim = x.size(1), stride = rows > 1 ? x.stride(0) : dim, hidden = wg.size(0);
     const int type = type_of(x, "x");
     Tensor d[5];
@@ -224,7 +229,7 @@ struct Gated : torch::autograd::Function<Gated> {
       const size_t bytes = gsr.gated_workspace(rows, dim, hidden, type, 1);
       const Tensor ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
       check(gsr.gated_bwd(x.data_ptr(), rows, dim, stride, type, wg.data_ptr(), wu.data_ptr(), hidden, ptr(bg), ptr(bu),
-                          (int)ctx->saved_data["act"].toInt(), g.t.data_ptr(), g.stride, ptr(d[0]), ptr(d[1]), ptr(d[2]), ptr(d[3]),
+                          (int)ctx->saved_data["act"].toInt(), g.t.data_ptr(), g.stride, ptr(kept), ptr(d[0]), ptr(d[1]), ptr(d[2]), ptr(d[3]),
                           ptr(d[4]), ws.data_ptr(), bytes, stream_of(x.device())),
             "gsr_gated_bwd");
     }
@@ -255,7 +260,7 @@ Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, c
   on_device(x, "gated_linear");
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(wg) || wants_grad(wu) || wants_grad(bg) || wants_grad(bu)))
     return Gated::apply(x, wg, wu, given(bg), given(bu), act);
-  return gated_forward(rows_of(x, dim), x, wg, wu, bg, bu, act);
+  return gated_forward(rows_of(x, dim), x, wg, wu, bg, bu, act, Tensor());
 }
 
 // ----------------------------------------------------------------- AdamW step

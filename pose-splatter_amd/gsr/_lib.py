@@ -170,9 +170,10 @@ EXPORTS = {
     "gsr_layer_norm_workspace": (_SZ, [_I64, _I64, _I32]),
     "gsr_layer_norm_bwd": (ctypes.c_int, [_P, _P, _I64, _I64, _I64, _I64, _I32, _P, _I32, _P, _P, _P, _P, _P, _SZ,
                                           _P]),
-    "gsr_gated_fwd": (ctypes.c_int, [_P, _I64, _I64, _I64, _I32, _P, _P, _I64, _P, _P, _I32, _P, _P, _SZ, _P]),
+    "gsr_gated_fwd": (ctypes.c_int, [_P, _I64, _I64, _I64, _I32, _P, _P, _I64, _P, _P, _I32, _P, _P, _P, _SZ, _P]),
+    "gsr_gated_kept": (_SZ, [_I64, _I64, _I64, _I32]),
     "gsr_gated_workspace": (_SZ, [_I64, _I64, _I64, _I32, _I32]),
-    "gsr_gated_bwd": (ctypes.c_int, [_P, _I64, _I64, _I64, _I32, _P, _P, _I64, _P, _P, _I32, _P, _I64, _P, _P, _P, _P,
+    "gsr_gated_bwd": (ctypes.c_int, [_P, _I64, _I64, _I64, _I32, _P, _P, _I64, _P, _P, _I32, _P, _I64, _P, _P, _P, _P, _P,
                                      _P, _P, _SZ, _P]),
     "gsr_adamw_step": (ctypes.c_int, [_P, _I32, _I32, _I32, ctypes.POINTER(AdamwArgs), _P]),
     "gsr_adamw_decode_root": (ctypes.c_int, [_P, _P, _I64, _P, _P]),

@@ -4,6 +4,8 @@ Tolerances (u = 2^-24; c(n) = (n + 16) u bounds an fp32 sum of n products, whate
 inputs are exact, 16-bit products are exact in fp32).
     eg = c(D) sum|x||wg| + 2u|g|,  eu alike
     h   |u| 1.13 eg + |a| eu + k |a u|,        k = (16 + |g|) u, + 2^-20 in 16 bits (v_exp, v_rcp)
+        (below, in 16 bits, eg + 2^-15 |g| and eu + 2^-15 |u|: a forward that keeps its projections
+        truncates them to 24 bits, of which 8 are exponent and sign and 16 mantissa's)
     dg  |dh| (|s| eu + |u| e_s),  e_s = eg + k (1 + |g|);  du  |dh| (1.13 eg + k |a|)
         (|act'| <= 1.13 and |act''| <= 1 for the smooth ones; relu's slope is open within eg of 0)
     then half a step of the type where dg, du are rounded for the products (not for the biases)
@@ -38,6 +40,9 @@ def _reference(x, wg, wu, bg, bu, dh, kind, dtype):
     eg = c(x.shape[1]) * (x.abs() @ wg.abs().T + bg.abs()) + 2 * U * g.abs()
     eu = c(x.shape[1]) * (x.abs() @ wu.abs().T + bu.abs()) + 2 * U * u.abs()
     k = (16 + g.abs()) * U + (2.0 ** -20 if short else 0)
+    th = u.abs() * 1.13 * eg + a.abs() * eu + k * (a * u).abs()
+    if short:
+        eg, eu = eg + 2.0 ** -15 * g.abs(), eu + 2.0 ** -15 * u.abs()
     es = (g.abs() <= eg).double() if kind == "relu" else eg + k * (1 + g.abs())
     dg, du = dh * u * s, dh * a
     tg, tu = dh.abs() * (s.abs() * eu + u.abs() * es) + 4 * U * dg.abs(), dh.abs() * (1.13 * eg + k * a.abs())
@@ -47,7 +52,7 @@ def _reference(x, wg, wu, bg, bu, dh, kind, dtype):
         rg, ru = rg + 2.0 ** -25, ru + 2.0 ** -25
     cr, ch = c(x.shape[0]), c(2 * wg.shape[0])
     values = [a * u, dg @ wg + du @ wu, dg.T @ x, du.T @ x, dg.sum(0), du.sum(0)]
-    tols = [u.abs() * 1.13 * eg + a.abs() * eu + k * (a * u).abs(),
+    tols = [th,
             (rg + ch * dg.abs()) @ wg.abs() + (ru + ch * du.abs()) @ wu.abs(),
             (rg + cr * dg.abs()).T @ x.abs(), (ru + cr * du.abs()).T @ x.abs(),
             (tg + cr * dg.abs()).sum(0), (tu + cr * du.abs()).sum(0)]
@@ -55,7 +60,7 @@ def _reference(x, wg, wu, bg, bu, dh, kind, dtype):
 
 
 def _check(got, want, tol, what):
-    got = got.detach().cpu()
+    got = got.detach().to(want.device)
     info = torch.finfo(got.dtype)
     limit = tol + info.eps / 2 * want.abs() * 1.01 + info.smallest_normal * info.eps
     err = (got.double() - want).abs()
@@ -143,7 +148,7 @@ def test_layouts(cuda, kind, layout):
         _check(got.reshape(v.shape), v, t, f"{name} {kind} {layout}")
 
 
-WIDE = [(3000, 1100, 4100), (4096, 64, 1024), (4100, 72, 1025), (4097, 65, 1100), (8192, 200, 600), (300, 130, 8256), (4864, 512, 1030),
+WIDE = [(3, 4096, 8200), (3000, 1100, 4100), (4096, 64, 1024), (4100, 72, 1025), (4097, 65, 1100), (8192, 200, 600), (300, 130, 8256), (4864, 512, 1030),
         (2049, 320, 2000)]
 
 
@@ -156,7 +161,33 @@ def test_large_cases(cuda, rows, dim, hidden, kind):
     args[0] = args[0] * 2 ** -3   # (keeps fp16's sums over thousands of rows in range)
     want, tol = _reference(*(None if t is None else t.to(cuda) for t in args), dh.to(cuda), "silu", TYPES[kind])
     for name, got, v, t in zip(NAMES, _run(cuda, args, dh, "silu"), want, tol):
-        _check(got, v.cpu(), t.cpu(), f"{name} {rows}x{dim}->{hidden} {kind}")
+        _check(got, v, t, f"{name} {rows}x{dim}->{hidden} {kind}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_largest_tiles(cuda, kind):
+    """Enough steps for tiles of 256 in all products, ragged ones, and a last round cut along K; and the same
+    backward without what the forward kept, which computes the projections again."""
+    from gsr import _lib
+    rows, dim, hidden = 8200, 2056, 4104
+    args, dh = _case(rows, dim, hidden, kind, True, 77)
+    args, dh = [t.to(cuda) for t in args], dh.to(cuda)
+    args[0] = args[0] * 2 ** -3
+    want, tol = _reference(*args, dh, "silu", TYPES[kind])
+    out = _run(cuda, args, dh, "silu")
+    for name, got, v, t in zip(NAMES, out, want, tol):
+        _check(got, v, t, f"{name} {kind}")
+    L, code = _lib.lib(), {"bf16": _lib.BF16, "f16": _lib.F16}[kind]
+    assert L.gsr_gated_kept(rows, dim, hidden, code) >= 6 * rows * hidden
+    grads = [torch.empty_like(t) for t in args]
+    ws = torch.empty(L.gsr_gated_workspace(rows, dim, hidden, code, 1), device=cuda, dtype=torch.uint8)
+    x, wg, wu, bg, bu = (t.data_ptr() for t in args)
+    _lib.check(L.gsr_gated_bwd(x, rows, dim, dim, code, wg, wu, hidden, bg, bu, 0, dh.data_ptr(), hidden, None,
+                               *(g.data_ptr() for g in grads), ws.data_ptr(), ws.numel(),
+                               torch.cuda.current_stream().cuda_stream), "gsr_gated_bwd")
+    for name, got, v, t in zip(NAMES[1:], grads, want[1:], tol[1:]):
+        _check(got, v, t, f"{name} {kind}, computed again")
 
 
 @pytest.mark.gpu
@@ -377,13 +408,13 @@ def test_refusals():
         gated_linear(f(1, 1).expand(1 << 27, 1), f(1, 1), f(1, 1))
     L = _lib.lib()
     fwd = lambda rows=4, dim=8, stride=8, t=0, hidden=6, act=0: L.gsr_gated_fwd(  # noqa: E731
-        None, rows, dim, stride, t, None, None, hidden, None, None, act, None, None, 0, None)
+        None, rows, dim, stride, t, None, None, hidden, None, None, act, None, None, None, 0, None)
     for kw, msg in [(dict(rows=-1), b"bad rows"), (dict(dim=0), b"bad dim"), (dict(hidden=0), b"bad dim"),
                     (dict(stride=7), b"row stride"), (dict(t=3), b"bad type"), (dict(act=4), b"bad activation"),
                     ({}, b"null pointer"), (dict(hidden=1 << 21), b"bad dim")]:
         assert fwd(**kw) == -1 and msg in L.gsr_last_error(), kw
-    bwd = lambda ws, n, dh=1: L.gsr_gated_bwd(1, 4, 8, 8, 0, 1, 1, 6, None, None, 0, dh, 6, 1, 1, 1, None, None, ws, n,  # noqa: E731
-                                              None)
+    bwd = lambda ws, n, dh=1: L.gsr_gated_bwd(1, 4, 8, 8, 0, 1, 1, 6, None, None, 0, dh, 6, None, 1, 1, 1, None, None, ws,  # noqa: E731
+                                              n, None)
     assert bwd(1, 16) == -1 and b"workspace" in L.gsr_last_error()
     assert bwd(1, 1 << 20, dh=None) == -1 and b"null" in L.gsr_last_error()
     assert L.gsr_gated_workspace(4, 8, 6, 0, 1) >= 4 * 128 * 4 and L.gsr_gated_workspace(4, 8, 6, 7, 1) == 0
