@@ -40,12 +40,12 @@ struct TileK {
   static constexpr int LD = BK + V;           // a row in shared memory, padded by 16 bytes
 };
 
-// 16 bytes of one operand's tile in flight, and where they go in shared memory.  KC: K is the
-// contiguous index.
-template <typename T, bool KC>
+// One lane's piece of an operand's tile in flight (16 bytes of the type M that is multiplied, loaded as
+// T), and where it goes in shared memory.  KC: K is the contiguous index.
+template <typename M, typename T, bool KC>
 __device__ __forceinline__ void tile_fetch(Operand<T> a, int64_t i0, int64_t rows, int64_t k0, int64_t k1,
-                                           float (&v)[TileK<T>::V]) {
-  constexpr int V = TileK<T>::V;
+                                           float (&v)[TileK<M>::V]) {
+  constexpr int V = TileK<M>::V;
   const int t = threadIdx.x;
   if constexpr (KC) {
     const int64_t i = i0 + t / 4, k = k0 + (t % 4) * V;
@@ -92,12 +92,13 @@ __device__ __forceinline__ v4f tile_mma<float>(const float* a, const float* b, v
 // acc[NB][nb][mb]: this wave's 32 x 32 of the tile (wave w: rows 32 (w % 2), columns 32 (w / 2)); a
 // lane holds row m = 16 mb + lane % 16 and columns n = 16 nb + 4 (lane / 16) + 0..3.
 // B(k): the operands for K step k0 (the gradient product changes matrices midway).
-template <typename T, int NB, bool AKC, bool BKC, typename FB>
-__device__ __forceinline__ void tile_product(Operand<T> a, int64_t m0, int64_t M, FB b_at, int64_t n0, int64_t N,
+// TA, TB: the operands' types, MT: the type they are multiplied in.
+template <typename MT, typename TA, typename TB, int NB, bool AKC, bool BKC, typename FB>
+__device__ __forceinline__ void tile_product(Operand<TA> a, int64_t m0, int64_t M, FB b_at, int64_t n0, int64_t N,
                                              int64_t k0, int64_t k1, v4f (&acc)[NB][2][2]) {
-  constexpr int V = TileK<T>::V, BK = TileK<T>::BK, LD = TileK<T>::LD;
-  __shared__ __attribute__((aligned(16))) T as[64 * LD];
-  __shared__ __attribute__((aligned(16))) T bs[NB][64 * LD];
+  constexpr int V = TileK<MT>::V, BK = TileK<MT>::BK, LD = TileK<MT>::LD;
+  __shared__ __attribute__((aligned(16))) MT as[64 * LD];
+  __shared__ __attribute__((aligned(16))) MT bs[NB][64 * LD];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int at = (lane % 16) * LD + (lane / 16) * V, wm = wave % 2 * 32, wn = wave / 2 * 32;
 #pragma unroll
@@ -106,19 +107,19 @@ __device__ __forceinline__ void tile_product(Operand<T> a, int64_t m0, int64_t M
     for (int i = 0; i < 4; ++i) acc[q][i / 2][i % 2] = v4f{0.f, 0.f, 0.f, 0.f};
   float av[V], bv[NB][V];
   const auto fetch = [&](int64_t k) {
-    tile_fetch<T, AKC>(a, m0, M, k, k1, av);
+    tile_fetch<MT, TA, AKC>(a, m0, M, k, k1, av);
 #pragma unroll
     for (int q = 0; q < NB; ++q) {
       const auto o = b_at(q, k);
-      tile_fetch<T, BKC>(o.op, n0, N, o.k, o.kend, bv[q]);
+      tile_fetch<MT, TB, BKC>(o.op, n0, N, o.k, o.kend, bv[q]);
     }
   };
   if (k0 < k1) fetch(k0);
   for (int64_t k = k0; k < k1; k += BK) {
     __syncthreads();
-    tile_keep<T, AKC>(as, av);
+    tile_keep<MT, AKC>(as, av);
 #pragma unroll
-    for (int q = 0; q < NB; ++q) tile_keep<T, BKC>(bs[q], bv[q]);
+    for (int q = 0; q < NB; ++q) tile_keep<MT, BKC>(bs[q], bv[q]);
     __syncthreads();
     if (k + BK < k1) fetch(k + BK);   // in flight over the products
 #pragma unroll
@@ -127,7 +128,7 @@ __device__ __forceinline__ void tile_product(Operand<T> a, int64_t m0, int64_t M
       for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
         for (int mb = 0; mb < 2; ++mb)
-          acc[q][nb][mb] = tile_mma<T>(bs[q] + (wn + nb * 16) * LD + at, as + (wm + mb * 16) * LD + at, acc[q][nb][mb]);
+          acc[q][nb][mb] = tile_mma<MT>(bs[q] + (wn + nb * 16) * LD + at, as + (wm + mb * 16) * LD + at, acc[q][nb][mb]);
   }
 }
 
@@ -139,13 +140,13 @@ struct OperandAt {
 
 // Forward (dgu NULL) or the gradients of the projections (h NULL): dgu [rows][2 gated_pad(hidden)],
 // parts [row blocks][2][hidden] the column sums of each block of 64 rows (NULL: not wanted).
-template <typename T>
+template <typename T, typename G>
 __global__ __launch_bounds__(256) void k_tile_gated(const T* x, int64_t x_stride, const T* wg, const T* wu, const T* bg,
                                                     const T* bu, int act, GatedShape s, T* h, const T* dh,
-                                                    int64_t dh_stride, T* dgu, float* parts) {
+                                                    int64_t dh_stride, G* dgu, float* parts) {
   const int64_t m0 = (int64_t)blockIdx.x * 64, n0 = (int64_t)blockIdx.y * 64;
   v4f acc[2][2][2];
-  tile_product<T, 2, true, true>(
+  tile_product<T, T, T, 2, true, true>(
       Operand<T>{x, x_stride}, m0, s.rows,
       [&](int q, int64_t k) { return OperandAt<T>{Operand<T>{q ? wu : wg, s.dim}, k, s.dim}; }, n0, s.hidden, 0, s.dim, acc);
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
@@ -216,14 +217,14 @@ __global__ __launch_bounds__(256) void k_tile_gated(const T* x, int64_t x_stride
 
 // dx = [dg | du] [Wg; Wu] over the columns of share blockIdx.z.  One share: into dx; more: fp32 parts
 // [share][rows][dim].
-template <typename T>
-__global__ __launch_bounds__(256) void k_tile_dx(const T* dgu, const T* wg, const T* wu, GatedShape s, int64_t share, T* dx,
+template <typename T, typename G>
+__global__ __launch_bounds__(256) void k_tile_dx(const G* dgu, const T* wg, const T* wu, GatedShape s, int64_t share, T* dx,
                                                  float* parts) {
   const int64_t m0 = (int64_t)blockIdx.x * 64, n0 = (int64_t)blockIdx.y * 64, pad = gated_pad(s.hidden);
   const int64_t k0 = blockIdx.z * share, k1 = k0 + share < 2 * pad ? k0 + share : 2 * pad;
   v4f acc[1][2][2];
-  tile_product<T, 1, true, false>(
-      Operand<T>{dgu, 2 * pad}, m0, s.rows,
+  tile_product<G, G, T, 1, true, false>(
+      Operand<G>{dgu, 2 * pad}, m0, s.rows,
       [&](int, int64_t k) {
         return k < pad ? OperandAt<T>{Operand<T>{wg, s.dim}, k, s.hidden} : OperandAt<T>{Operand<T>{wu, s.dim}, k - pad, s.hidden};
       },
@@ -248,14 +249,14 @@ __global__ __launch_bounds__(256) void k_tile_dx(const T* dgu, const T* wg, cons
 
 // [dWg; dWu] = [dg | du]^T x over the rows of share blockIdx.z.  One share: into dwg, dwu; more:
 // fp32 parts [share][2][hidden][dim].
-template <typename T>
-__global__ __launch_bounds__(256) void k_tile_dw(const T* dgu, const T* x, int64_t x_stride, GatedShape s, int64_t share,
+template <typename T, typename G>
+__global__ __launch_bounds__(256) void k_tile_dw(const G* dgu, const T* x, int64_t x_stride, GatedShape s, int64_t share,
                                                  T* dwg, T* dwu, float* parts) {
   const int64_t m0 = (int64_t)blockIdx.x * 64, n0 = (int64_t)blockIdx.y * 64, pad = gated_pad(s.hidden);
   const int64_t k0 = blockIdx.z * share, k1 = k0 + share < s.rows ? k0 + share : s.rows;
   v4f acc[1][2][2];
-  tile_product<T, 1, false, false>(
-      Operand<T>{dgu, 2 * pad}, m0, 2 * pad,
+  tile_product<G, G, T, 1, false, false>(
+      Operand<G>{dgu, 2 * pad}, m0, 2 * pad,
       [&](int, int64_t k) { return OperandAt<T>{Operand<T>{x, x_stride}, k, k1}; }, n0, s.dim, k0, k1, acc);
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
 #pragma unroll
@@ -317,9 +318,9 @@ static void gated_join(const float* parts, int64_t count, int64_t n, int64_t spl
 // The gradients of the projections from what the forward kept: dgu, and parts [row blocks of 64][2][hidden]
 // of the column sums (NULL: not wanted).  Bound by memory: 12 bytes an element in 16 bits, 20 in fp32
 // (8 columns a lane, 256 a workgroup).
-template <typename T>
+template <typename T, typename G>
 __global__ __launch_bounds__(256) void k_gated_slopes(const void* saved, const T* dh, int64_t dh_stride, int act, GatedShape s,
-                                                      T* dgu, float* parts) {
+                                                      G* dgu, float* parts) {
   const int64_t pad = gated_pad(s.hidden), n = (int64_t)blockIdx.x * 256 + threadIdx.x % 32 * 8, left = s.hidden - n;
   const Kept<T> kept((void*)saved, s.rows, s.hidden);
   const int64_t m0 = (int64_t)blockIdx.y * 64 + threadIdx.x / 32;
@@ -434,12 +435,24 @@ static bool gated_aligned(const T* p, int64_t dim, int64_t stride) {
 // 128 -> 2816 111 against 146.
 static bool gated_keeps(int type, int64_t dim) { return dim >= (type == GSR_F32 ? 128 : 256); }
 
+// Whether a 16-bit block's backward keeps the projections' gradients in fp32 and multiplies them so: where
+// products are short (in 64 x 64 tiles 2^24 products, a few us at the fp32 rate) or dx has few
+// values.  There one more rounding to 16 bits need not average out: the root mean square error of
+// a gradient grows by up to 2.1, that of larger ones by 1.4.  (65 x 256 -> 512 bf16: 30 us against 25;
+// 4096 x 256 -> 256, left in 16 bits, would take 66 against 33.)
+static bool gated_exact(int type, GatedShape s) {
+  if (type == GSR_F32) return false;
+  const int64_t r = s.rows < 64 ? 64 : s.rows, d = s.dim < 64 ? 64 : s.dim;
+  return r * d <= (1 << 24) / s.hidden || s.rows * s.dim <= 2048;
+}
+
 // How a pass is laid out: each product's tile side, the 64 x 64 tiles' shares of K, and its workspace (byte
 // offsets).  There is room for padded copies wherever a wide product may need them: an odd dim, rows
 // or addresses that are not multiples of 16 bytes.
 struct GatedPlan {
   int fwd, dx, dw;               // tile sides
   bool keep;                     // the forward keeps its projections
+  bool exact;                    // the backward's products take the projections' gradients in fp32
   int64_t n_dx, n_dw;            // shares
   int64_t kdim;                  // dim in whole 16-byte pieces
   int64_t x, wg, wu, dgu, bias, bias_rows, dx_parts, dw_parts, total;
@@ -449,8 +462,9 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
   GatedPlan w;
   const int64_t pad = gated_pad(s.hidden);
   w.fwd = gated_side(type, s.rows, 2 * pad, s.dim, s);
-  w.dx = gated_side(type, s.rows, s.dim, 2 * pad, s);
-  w.dw = gated_side(type, 2 * pad, s.dim, s.rows, s);
+  w.exact = gated_exact(type, s);
+  w.dx = w.exact ? 64 : gated_side(type, s.rows, s.dim, 2 * pad, s);
+  w.dw = w.exact ? 64 : gated_side(type, 2 * pad, s.dim, s.rows, s);
   const int64_t es = (int64_t)type_size(type), piece = 16 / es;
   w.kdim = (s.dim + piece - 1) / piece * piece;
   const int64_t rb = ceil_div64(s.rows, 64), hb = 2 * pad / 64, db = ceil_div64(s.dim, 64);
@@ -472,7 +486,7 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
   w.wu = take(ww ? s.hidden * w.kdim * es : 0);
   w.keep = w.fwd > 64 && gated_keeps(type, s.dim);
   w.bias_rows = s.rows <= kSkinnyRows ? 1 : w.fwd > 64 ? ceil_div64(s.rows, w.fwd) * 2 : rb;
-  w.dgu = take(backward ? s.rows * 2 * pad * es : 0);
+  w.dgu = take(backward ? s.rows * 2 * pad * (w.exact ? 4 : es) : 0);
   w.bias = take(backward ? (w.keep && rb > w.bias_rows ? rb : w.bias_rows) * 2 * s.hidden * 4 : 0);
   w.dx_parts = take(!backward ? 0 : w.dx > 64 ? cuts(w.dx, s.rows, s.dim, 2 * pad) : w.n_dx > 1 ? w.n_dx * s.rows * s.dim * 4 : 0);
   w.dw_parts = take(!backward  ? 0
@@ -517,7 +531,7 @@ static void gated_fwd(const T* x, int64_t x_stride, const T* wg, const T* wu, co
                       T* h, void* kept, char* ws, hipStream_t st) {
   const int type = type_of<T>();
   if (s.rows <= kSkinnyRows) {
-    gated_skinny(type, GatedSkinny{s, x, wg, wu, bg, bu, nullptr, x_stride, 0, h, nullptr, nullptr, act}, st);
+    gated_skinny(type, GatedSkinny{s, x, wg, wu, bg, bu, nullptr, x_stride, 0, h, nullptr, nullptr, act, false}, st);
     return;
   }
   const GatedPlan w = gated_plan(s, type, false);
@@ -528,11 +542,12 @@ static void gated_fwd(const T* x, int64_t x_stride, const T* wg, const T* wu, co
     return;
   }
   const dim3 grid((unsigned)ceil_div64(s.rows, 64), (unsigned)ceil_div64(s.hidden, 64));
-  k_tile_gated<T><<<grid, 256, 0, st>>>(x, x_stride, wg, wu, bg, bu, act, s, h, nullptr, 0, nullptr, nullptr);
+  k_tile_gated<T, T><<<grid, 256, 0, st>>>(x, x_stride, wg, wu, bg, bu, act, s, h, nullptr, 0, nullptr, nullptr);
 }
 
-template <typename T>
-static void gated_bwd(const T* x, int64_t x_stride, const T* wg, const T* wu, const T* bg, const T* bu, int act, GatedShape s,
+// G: the type that the projections' gradients are kept and multiplied in.
+template <typename T, typename G>
+static void gated_bwd_as(const T* x, int64_t x_stride, const T* wg, const T* wu, const T* bg, const T* bu, int act, GatedShape s,
                       const T* dh, int64_t dh_stride, const void* kept, T* dx, T* dwg, T* dwu, T* dbg, T* dbu, char* ws,
                       hipStream_t st) {
   const int type = type_of<T>();
@@ -540,24 +555,24 @@ static void gated_bwd(const T* x, int64_t x_stride, const T* wg, const T* wu, co
   const int64_t rb = ceil_div64(s.rows, 64), db = ceil_div64(s.dim, 64), pad = gated_pad(s.hidden);
   const bool weights = dwg || dwu, few = s.rows <= kSkinnyRows, keep = w.keep && kept;
   if (keep) w.bias_rows = rb;
-  T* dgu = (T*)(ws + w.dgu);
+  G* dgu = (G*)(ws + w.dgu);
   float* bias = dbg || dbu ? (float*)(ws + w.bias) : nullptr;
   GatedWide a{};
   if (w.fwd > 64 || w.dx > 64 || w.dw > 64) {
     const bool again = w.fwd > 64 && !keep;   // both projections are computed again
     a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, again || (weights && w.dw > 64), again || (dx && w.dx > 64), ws,
                            st);
-    a.dh = dh, a.dh_stride = dh_stride, a.dgu = dgu, a.dx = dx, a.dwg = dwg, a.dwu = dwu;
+    a.dh = dh, a.dh_stride = dh_stride, a.dgu = dgu, a.dgu32 = w.exact, a.dx = dx, a.dwg = dwg, a.dwu = dwu;
   }
   if (keep) {
-    k_gated_slopes<T><<<dim3((unsigned)ceil_div64(pad, 256), (unsigned)rb), 256, 0, st>>>(kept, dh, dh_stride, act, s, dgu, bias);
+    k_gated_slopes<T, G><<<dim3((unsigned)ceil_div64(pad, 256), (unsigned)rb), 256, 0, st>>>(kept, dh, dh_stride, act, s, dgu, bias);
   } else if (few) {
-    gated_skinny(type, GatedSkinny{s, x, wg, wu, bg, bu, dh, x_stride, dh_stride, nullptr, dgu, bias, act}, st);
+    gated_skinny(type, GatedSkinny{s, x, wg, wu, bg, bu, dh, x_stride, dh_stride, nullptr, dgu, bias, act, w.exact}, st);
   } else if (w.fwd > 64) {
     a.parts = bias;
     gated_wide(type, kWideGrad, w.fwd, a, st);
   } else {
-    k_tile_gated<T><<<dim3((unsigned)rb, (unsigned)(pad / 64)), 256, 0, st>>>(x, x_stride, wg, wu, bg, bu, act, s, nullptr, dh,
+    k_tile_gated<T, G><<<dim3((unsigned)rb, (unsigned)(pad / 64)), 256, 0, st>>>(x, x_stride, wg, wu, bg, bu, act, s, nullptr, dh,
                                                                             dh_stride, dgu, bias);
   }
   if (bias) gated_join<T>(bias, w.bias_rows, 2 * s.hidden, s.hidden, dbg, dbu, st);
@@ -568,7 +583,7 @@ static void gated_bwd(const T* x, int64_t x_stride, const T* wg, const T* wu, co
       a.cuts = (float*)(ws + w.dx_parts);
       gated_wide(type, kWideDx, w.dx, a, st);
     } else {
-      k_tile_dx<T><<<dim3((unsigned)rb, (unsigned)db, (unsigned)n), 256, 0, st>>>(dgu, wg, wu, s, share, dx, parts);
+      k_tile_dx<T, G><<<dim3((unsigned)rb, (unsigned)db, (unsigned)n), 256, 0, st>>>(dgu, wg, wu, s, share, dx, parts);
     }
     if (parts) gated_join<T>(parts, n, s.rows * s.dim, s.rows * s.dim, dx, nullptr, st);
   }
@@ -579,10 +594,21 @@ static void gated_bwd(const T* x, int64_t x_stride, const T* wg, const T* wu, co
       a.cuts = (float*)(ws + w.dw_parts);
       gated_wide(type, kWideDw, w.dw, a, st);
     } else {
-      k_tile_dw<T><<<dim3((unsigned)(2 * pad / 64), (unsigned)db, (unsigned)n), 256, 0, st>>>(dgu, x, x_stride, s, share, dwg,
+      k_tile_dw<T, G><<<dim3((unsigned)(2 * pad / 64), (unsigned)db, (unsigned)n), 256, 0, st>>>(dgu, x, x_stride, s, share, dwg,
                                                                                               dwu, parts);
     }
     if (parts) gated_join<T>(parts, n, 2 * s.hidden * s.dim, s.hidden * s.dim, dwg, dwu, st);
+  }
+}
+
+template <typename T>
+static void gated_bwd(const T* x, int64_t x_stride, const T* wg, const T* wu, const T* bg, const T* bu, int act, GatedShape s,
+                      const T* dh, int64_t dh_stride, const void* kept, T* dx, T* dwg, T* dwu, T* dbg, T* dbu, char* ws,
+                      hipStream_t st) {
+  if (gated_exact(type_of<T>(), s)) {
+    gated_bwd_as<T, float>(x, x_stride, wg, wu, bg, bu, act, s, dh, dh_stride, kept, dx, dwg, dwu, dbg, dbu, ws, st);
+  } else {
+    gated_bwd_as<T, T>(x, x_stride, wg, wu, bg, bu, act, s, dh, dh_stride, kept, dx, dwg, dwu, dbg, dbu, ws, st);
   }
 }
 

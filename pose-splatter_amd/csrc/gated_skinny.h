@@ -14,6 +14,7 @@ struct GatedSkinny {
   void *h, *dgu;   // one of them: the forward, or the gradients of the projections
   float* parts;    // gradients: column sums [2][hidden], or NULL
   int act;
+  bool dgu32;      // dgu is written in fp32
 };
 
 void gated_skinny(int type, const GatedSkinny& a, hipStream_t st);

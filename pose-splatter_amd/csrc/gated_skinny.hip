@@ -126,8 +126,14 @@ __global__ __launch_bounds__(WAVES * 64) void k_skinny(GatedSkinny a) {
       gv = in ? d * uv * slope : 0.f;   // (the padding holds zeros)
       uv = in ? d * act : 0.f;
       if (row < s.rows) {
-        ((T*)a.dgu)[row * 2 * pad + n] = from_f<T>(gv);
-        ((T*)a.dgu)[row * 2 * pad + pad + n] = from_f<T>(uv);
+        const int64_t to = row * 2 * pad + n;
+        if (a.dgu32) {
+          ((float*)a.dgu)[to] = gv;
+          ((float*)a.dgu)[to + pad] = uv;
+        } else {
+          ((T*)a.dgu)[to] = from_f<T>(gv);
+          ((T*)a.dgu)[to + pad] = from_f<T>(uv);
+        }
       }
       lds[0][0][mt][from] = gv;   // (this thread alone reads and writes the place)
       lds[0][1][mt][from] = uv;

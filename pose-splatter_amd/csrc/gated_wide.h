@@ -17,6 +17,7 @@ struct GatedWide {
   float* parts;   // gradients: column sums [ceil(rows / side) * 2][2][hidden], or NULL
   float* cuts;    // dx, dW: the cut tiles' sums [shares][cut][side][side]
   int act;
+  bool dgu32;     // gradients: dgu is written in fp32
   int mt, nt, whole, cut, shares;   // set by the launch: tiles, and how they are cut (gated_wide_rounds)
 };
 

@@ -274,7 +274,10 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
       if constexpr (MODE == kWideFwd) {
         store_upto((T*)a.h + m * s.hidden + n, left_n, g);
       } else if constexpr (MODE == kWideGrad) {
-        if (n < pad) {
+        if (n < pad && a.dgu32) {
+          store_vec((float*)a.dgu + m * 2 * pad + n, g);
+          store_vec((float*)a.dgu + m * 2 * pad + pad + n, u);
+        } else if (n < pad) {
           store_vec((T*)a.dgu + m * 2 * pad + n, g);
           store_vec((T*)a.dgu + m * 2 * pad + pad + n, u);
         }

@@ -54,7 +54,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     biases [hidden] or both None, all of one type; activation "silu", "gelu" (the error
     function's form), "relu" or "sigmoid".  Sums are fp32; in bf16 and fp16 the backward rounds
     the projections' gradients to the type before the products that use them, as separate
-    layers would.  Differentiable (once) w.r.t. every tensor.  For its backward a forward keeps x and
+    layers would (in small cases they stay fp32).  Differentiable (once) w.r.t. every tensor.  For its backward a forward keeps x and
     the weights, and from dim 256 on (128 in fp32) both projections, 6 bytes an element of
     [rows, hidden] (8 in fp32); below that, and for up to 64 rows, the backward computes them again."""
     act = ACTIVATIONS.get(activation)
