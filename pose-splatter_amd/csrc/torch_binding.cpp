@@ -23,7 +23,7 @@ using torch::autograd::variable_list;
 
 // libgsr's calls, taken by bind() from the library that the ctypes binding has loaded (so that both sides
 // of the package use one library, wherever it lies).
-struct {
+struct Calls {
   decltype(&::gsr_last_error) last_error;
   decltype(&::gsr_layer_norm_fwd) layer_norm_fwd;
   decltype(&::gsr_layer_norm_workspace) layer_norm_workspace;
@@ -38,19 +38,21 @@ struct {
 void bind(const std::string& path) {
   void* lib = dlopen(path.c_str(), RTLD_NOW | RTLD_LOCAL);
   TORCH_CHECK(lib, "cannot load ", path, ": ", dlerror());
+  Calls c;
   const auto take = [&](auto& f, const char* name) {
     f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(dlsym(lib, name));
     TORCH_CHECK(f, path, " has no ", name);
   };
-  take(gsr.last_error, "gsr_last_error");
-  take(gsr.layer_norm_fwd, "gsr_layer_norm_fwd");
-  take(gsr.layer_norm_workspace, "gsr_layer_norm_workspace");
-  take(gsr.layer_norm_bwd, "gsr_layer_norm_bwd");
-  take(gsr.gated_fwd, "gsr_gated_fwd");
-  take(gsr.gated_kept, "gsr_gated_kept");
-  take(gsr.gated_workspace, "gsr_gated_workspace");
-  take(gsr.gated_bwd, "gsr_gated_bwd");
-  take(gsr.adamw_step, "gsr_adamw_step");
+  take(c.last_error, "gsr_last_error");
+  take(c.layer_norm_fwd, "gsr_layer_norm_fwd");
+  take(c.layer_norm_workspace, "gsr_layer_norm_workspace");
+  take(c.layer_norm_bwd, "gsr_layer_norm_bwd");
+  take(c.gated_fwd, "gsr_gated_fwd");
+  take(c.gated_kept, "gsr_gated_kept");
+  take(c.gated_workspace, "gsr_gated_workspace");
+  take(c.gated_bwd, "gsr_gated_bwd");
+  take(c.adamw_step, "gsr_adamw_step");
+  gsr = c;   // only a library that has them all
 }
 
 int type_of(const Tensor& t, const char* what) {

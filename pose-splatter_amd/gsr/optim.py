@@ -83,11 +83,20 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
                  moment_bits: int = 32, capturable: bool = False):
-        if moment_bits not in (8, 32):
-            raise ValueError(f"AdamW: moment_bits must be 8 or 32, got {moment_bits}")
-        adamw_step([], [], [], [], lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, step=1)   # checks them
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
-                                      moment_bits=int(moment_bits), capturable=bool(capturable)))
+                                      moment_bits=moment_bits, capturable=bool(capturable)))
+
+    def add_param_group(self, param_group: dict) -> None:
+        """As torch's; a group's own values are checked like the defaults."""
+        super().add_param_group(param_group)
+        g = self.param_groups[-1]
+        try:
+            if g["moment_bits"] not in (8, 32):
+                raise ValueError(f"AdamW: moment_bits must be 8 or 32, got {g['moment_bits']}")
+            adamw_step([], [], [], [], lr=g["lr"], betas=g["betas"], eps=g["eps"], weight_decay=g["weight_decay"], step=1)
+        except (ValueError, TypeError):
+            self.param_groups.pop()
+            raise
 
     def _state(self, p: torch.Tensor, group: dict) -> dict:
         s = self.state[p]

@@ -306,6 +306,28 @@ def test_captured_steps(cuda, bits):
 
 
 @pytest.mark.gpu
+def test_groups_and_absent_gradients(cuda):
+    """Groups with their own lr and moment bits step as optimizers of their own; a parameter without a gradient
+    keeps its value and its own step count."""
+    from gsr.optim import AdamW
+    torch.manual_seed(3)
+    start = [torch.randn(300, device=cuda) for _ in range(3)]
+    grads = [[torch.randn(300, device=cuda) for _ in range(3)] for _ in range(4)]
+    ps = [torch.nn.Parameter(t.clone()) for t in start]
+    opt = AdamW([{"params": ps[:1], "lr": 1e-2}, {"params": ps[1:], "moment_bits": 8}], lr=1e-3)
+    alone = [torch.nn.Parameter(t.clone()) for t in start]
+    single = [AdamW([alone[0]], lr=1e-2), AdamW([alone[1]], lr=1e-3, moment_bits=8), AdamW([alone[2]], lr=1e-3, moment_bits=8)]
+    for k, gs in enumerate(grads):
+        for i in range(3):
+            ps[i].grad = alone[i].grad = None if (i == 2 and k == 1) else gs[i]
+        opt.step()
+        for o in single:
+            o.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, alone))
+    assert [opt.state[p]["step"] for p in ps] == [4, 4, 3]
+
+
+@pytest.mark.gpu
 def test_refused_while_capturing(cuda):
     from gsr.optim import AdamW
     p = torch.nn.Parameter(torch.zeros(8, device=cuda))
@@ -383,6 +405,11 @@ def test_refusals():
         AdamW([f(4).requires_grad_()], moment_bits=16)
     with pytest.raises(ValueError, match="betas"):
         AdamW([f(4).requires_grad_()], betas=(1.0, 0.9))
+    opt = AdamW([f(4).requires_grad_()])
+    for bad, msg in (({"moment_bits": 16}, "moment_bits"), ({"lr": -1.0}, "lr"), ({"betas": (0.9, 1.5)}, "betas")):
+        with pytest.raises(ValueError, match=msg):
+            opt.add_param_group({"params": [f(3).requires_grad_()], **bad})
+    assert len(opt.param_groups) == 1
     adamw_step([], [], [], [], step=1)
     L = _lib.lib()
     args = _lib.AdamwArgs(lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.0, step=1, bits=32)
