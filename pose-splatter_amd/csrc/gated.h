@@ -25,23 +25,36 @@ __device__ __forceinline__ float sigmoid(float g) {
   }
 }
 
-// a = act(g), and its slope.
-template <typename T>
-__device__ __forceinline__ void activate(int act, float g, float& a, float& slope) {
+// a = act(g), and its slope, of N elements: one switch for all of them, so that their chains of
+// transcendentals interleave.
+template <typename T, int N>
+__device__ __forceinline__ void activate(int act, const float (&g)[N], float (&a)[N], float (&slope)[N]) {
   if (act == GSR_ACT_SILU) {
-    const float s = sigmoid<T>(g);
-    a = g * s;
-    slope = s * (1.f + g * (1.f - s));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float s = sigmoid<T>(g[i]);
+      a[i] = g[i] * s;
+      slope[i] = s * (1.f + g[i] * (1.f - s));
+    }
   } else if (act == GSR_ACT_GELU) {
-    const float area = 0.5f + 0.5f * erff(g * 0.70710678f);
-    a = g * area;
-    slope = area + g * (0.39894228f * expf(-0.5f * g * g));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float area = 0.5f + 0.5f * erff(g[i] * 0.70710678f);
+      a[i] = g[i] * area;
+      slope[i] = area + g[i] * (0.39894228f * expf(-0.5f * g[i] * g[i]));
+    }
   } else if (act == GSR_ACT_RELU) {
-    a = g < 0.f ? 0.f : g;   // (NaN stays NaN)
-    slope = g > 0.f ? 1.f : 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      a[i] = g[i] < 0.f ? 0.f : g[i];   // (NaN stays NaN)
+      slope[i] = g[i] > 0.f ? 1.f : 0.f;
+    }
   } else {
-    a = sigmoid<T>(g);
-    slope = a * (1.f - a);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      a[i] = sigmoid<T>(g[i]);
+      slope[i] = a[i] * (1.f - a[i]);
+    }
   }
 }
 

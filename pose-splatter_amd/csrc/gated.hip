@@ -167,23 +167,19 @@ __global__ __launch_bounds__(256) void k_tile_gated(const T* x, int64_t x_stride
         g[i] = acc[0][nb][mb][i] + gb[i];
         u[i] = acc[1][nb][mb][i] + ub[i];
       }
+      float a[4], slope[4];
+      activate<T>(act, g, a, slope);
       if (!dgu) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float a, slope;
-          activate<T>(act, g[i], a, slope);
-          g[i] = a * u[i];
-        }
+        for (int i = 0; i < 4; ++i) g[i] = a[i] * u[i];
         if (m < s.rows) store_upto(h + m * s.hidden + n, left, g);
       } else if (m < s.rows) {
         float d[4];
         load_upto(dh + m * dh_stride + n, left, d);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float a, slope;
-          activate<T>(act, g[i], a, slope);
-          g[i] = i < left ? d[i] * u[i] * slope : 0.f;   // (the padding holds zeros)
-          u[i] = i < left ? d[i] * a : 0.f;
+          g[i] = i < left ? d[i] * u[i] * slope[i] : 0.f;   // (the padding holds zeros)
+          u[i] = i < left ? d[i] * a[i] : 0.f;
           sg[i] += g[i];
           su[i] += u[i];
         }
@@ -333,12 +329,12 @@ __global__ __launch_bounds__(256) void k_gated_slopes(const void* saved, const T
       float g[8], u[8], d[8];
       kept.load(m * pad + n, g, u);
       load_upto(dh + m * dh_stride + n, left, d);
+      float a[8], slope[8];
+      activate<T>(act, g, a, slope);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float a, slope;
-        activate<T>(act, g[i], a, slope);
-        g[i] = i < left ? d[i] * u[i] * slope : 0.f;   // (the padding holds zeros)
-        u[i] = i < left ? d[i] * a : 0.f;
+        g[i] = i < left ? d[i] * u[i] * slope[i] : 0.f;   // (the padding holds zeros)
+        u[i] = i < left ? d[i] * a[i] : 0.f;
         sg[i] += g[i];
         su[i] += u[i];
       }

@@ -117,14 +117,15 @@ __global__ __launch_bounds__(WAVES * 64) void k_skinny(GatedSkinny a) {
       gv += to_f(((const T*)a.bg)[n]);
       uv += to_f(((const T*)a.bu)[n]);
     }
-    float act, slope;
-    activate<T>(a.act, gv, act, slope);
+    const float one[1] = {gv};
+    float act[1], slope[1];
+    activate<T>(a.act, one, act, slope);
     if constexpr (!GRAD) {
-      if (in) ((T*)a.h)[row * s.hidden + n] = from_f<T>(act * uv);
+      if (in) ((T*)a.h)[row * s.hidden + n] = from_f<T>(act[0] * uv);
     } else {
       const float d = in ? to_f(((const T*)a.dh)[row * a.dh_stride + n]) : 0.f;
-      gv = in ? d * uv * slope : 0.f;   // (the padding holds zeros)
-      uv = in ? d * act : 0.f;
+      gv = in ? d * uv * slope[0] : 0.f;   // (the padding holds zeros)
+      uv = in ? d * act[0] : 0.f;
       if (row < s.rows) {
         const int64_t to = row * 2 * pad + n;
         if (a.dgu32) {

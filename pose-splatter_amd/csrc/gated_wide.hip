@@ -257,15 +257,15 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
         }
         if constexpr (MODE == kWideFwd)
           if (a.kept && n < pad) Kept<T>(a.kept, s.rows, s.hidden).store(m * pad + n, g, u);
+        float act[8], slope[8];
+        activate<T>(a.act, g, act, slope);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          float act, slope;
-          activate<T>(a.act, g[i], act, slope);
           if constexpr (MODE == kWideFwd) {
-            g[i] = act * u[i];
+            g[i] = act[i] * u[i];
           } else {
-            g[i] = i < left_n ? d[i] * u[i] * slope : 0.f;   // (the padding holds zeros)
-            u[i] = i < left_n ? d[i] * act : 0.f;
+            g[i] = i < left_n ? d[i] * u[i] * slope[i] : 0.f;   // (the padding holds zeros)
+            u[i] = i < left_n ? d[i] * act[i] : 0.f;
             sg[i] += g[i];
             su[i] += u[i];
           }
