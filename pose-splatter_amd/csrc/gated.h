@@ -14,12 +14,15 @@ __host__ __device__ inline int64_t gated_pad(int64_t hidden) {
   return (hidden + kGatedPad - 1) / kGatedPad * kGatedPad;
 }
 
-// exp and reciprocal as exact as T's results can show: fp32 takes the library's, 16-bit types the
-// hardware's v_exp_f32 and v_rcp_f32 (within 2^-20 relative where sigmoid is not 0 or 1).
+// exp and reciprocal as exact as T's results can show: fp32 takes the library's exp and v_rcp_f32 with a Newton
+// step (1 + exp is 1 at least, so nothing but its overflow needs care; a third of a division's
+// instructions), 16-bit types v_exp_f32 and v_rcp_f32 (within 2^-20 relative where sigmoid is not 0
+// or 1).
 template <typename T>
 __device__ __forceinline__ float sigmoid(float g) {
   if constexpr (sizeof(T) == 4) {
-    return 1.f / (1.f + expf(-g));
+    const float y = 1.f + expf(-g), r = __builtin_amdgcn_rcpf(y);
+    return y < 0x1p126f ? fmaf(fmaf(-y, r, 1.f), r, r) : r;
   } else {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504f));
   }

@@ -10,13 +10,14 @@
 // the gradients as the products' epilogue.  It then takes dx from K = [dg | du] and both
 // weight gradients from M = [dg | du].
 //
-// Most cases run on square tiles of 256 or 128 (gated_wide.hip), up to 64 rows on gated_skinny.hip's kernel;
-// here is what serves the others:
+// Most cases run on square tiles of 256 or 128 (gated_wide.hip), projections of up to 64 rows on gated_skinny.hip's
+// kernel, the backward of up to 15 columns on gated_narrow.hip's; here is what serves the others:
 //
 // k_tile: 64 x 64 tiles of any shape, stride and alignment, with 16x16 matrix instructions: fp32
 // ones for fp32 (exact fp32 products), bf16/fp16 ones with fp32 sums.  A weight gradient's sum
 // over rows is split over workgroups where there are few tiles; the parts are joined in order.
 #include "gated.h"
+#include "gated_narrow.h"
 #include "gated_skinny.h"
 #include "gated_wide.h"
 
@@ -454,8 +455,24 @@ struct GatedPlan {
   int64_t x, wg, wu, dgu, bias, bias_rows, dx_parts, dw_parts, total;
 };
 
+// Whether the backward is one kernel (gated_narrow.hip).
+static bool gated_is_narrow(GatedShape s) { return s.dim <= kNarrowDim; }
+
 static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
-  GatedPlan w;
+  GatedPlan w{};
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  if (backward && gated_is_narrow(s)) {
+    const NarrowPlan n = gated_narrow_plan(s);
+    w.dw_parts = take(n.dw_floats(s) * 4);
+    w.dx_parts = take(n.dx_floats(s) * 4);
+    w.total = at;
+    return w;
+  }
   const int64_t pad = gated_pad(s.hidden);
   w.fwd = gated_side(type, s.rows, 2 * pad, s.dim, s);
   w.exact = gated_exact(type, s);
@@ -468,12 +485,6 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
   w.n_dw = w.dw > 64 ? 1 : gated_shares(hb * db, s.rows, 2 * s.hidden * s.dim);
   const auto cuts = [type](int side, int64_t r, int64_t c, int64_t k) {
     return gated_wide_rounds(side, ceil_div64(r, side), ceil_div64(c, side), gated_wide_steps(type, k)).bytes(side);
-  };
-  int64_t at = 0;
-  const auto take = [&](int64_t bytes) {
-    const int64_t here = at;
-    at += (bytes + 255) / 256 * 256;
-    return here;
   };
   if (s.rows <= kSkinnyRows) w.fwd = 64;   // (the kernel for few rows)
   const bool xw = w.fwd > 64 || (backward && w.dw > 64), ww = w.fwd > 64 || (backward && w.dx > 64);
@@ -601,7 +612,12 @@ template <typename T>
 static void gated_bwd(const T* x, int64_t x_stride, const T* wg, const T* wu, const T* bg, const T* bu, int act, GatedShape s,
                       const T* dh, int64_t dh_stride, const void* kept, T* dx, T* dwg, T* dwu, T* dbg, T* dbu, char* ws,
                       hipStream_t st) {
-  if (gated_exact(type_of<T>(), s)) {
+  if (gated_is_narrow(s)) {
+    const GatedPlan w = gated_plan(s, type_of<T>(), true);
+    GatedNarrow a{s, x, wg, wu, bg, bu, dh, x_stride, dh_stride, act, dx, dwg, dwu, dbg, dbu};
+    a.dw_parts = (float*)(ws + w.dw_parts), a.dx_parts = (float*)(ws + w.dx_parts);
+    gated_narrow(type_of<T>(), a, st);
+  } else if (gated_exact(type_of<T>(), s)) {
     gated_bwd_as<T, float>(x, x_stride, wg, wu, bg, bu, act, s, dh, dh_stride, kept, dx, dwg, dwu, dbg, dbu, ws, st);
   } else {
     gated_bwd_as<T, T>(x, x_stride, wg, wu, bg, bu, act, s, dh, dh_stride, kept, dx, dwg, dwu, dbg, dbu, ws, st);
@@ -665,7 +681,7 @@ extern "C" int gsr_gated_bwd(const void* x, int64_t rows, int64_t dim, int64_t x
   if (const int e = gated_check("gsr_gated_bwd", s, x_stride, type, act)) return e;
   GSR_REQUIRE(rows <= 1 || dh_stride >= hidden, "gsr_gated_bwd: dh row stride %lld below hidden", (long long)dh_stride);
   GSR_REQUIRE(wg && wu && (rows == 0 || (x && dh)), "gsr_gated_bwd: null pointer");
-  GSR_REQUIRE(workspace_bytes >= gsr_gated_workspace(rows, dim, hidden, type, 1) && (workspace || rows == 0),
+  GSR_REQUIRE(workspace_bytes >= gsr_gated_workspace(rows, dim, hidden, type, 1) && (workspace || workspace_bytes == 0),
               "gsr_gated_bwd: workspace too small (%zu bytes)", workspace_bytes);
   const auto st = (hipStream_t)stream;
   char* ws = (char*)workspace;

@@ -376,6 +376,75 @@ def test_head_trains(cuda):
         assert float((p.grad.double().cpu() - leaf[k].grad).abs().max()) <= 4096 * U * float(leaf[k].grad.abs().max()) + 1e-5, k
 
 
+# dim <= 15: one row, one column; rows that end inside 16 and 64; each width of a step of 4; few rows and many columns
+# (dx in shares); more row tiles than workgroups
+NARROW = [(1, 15, 2050), (15, 4, 16), (64, 7, 17), (70, 15, 400), (129, 12, 128), (400, 2, 1000), (20000, 1, 7), (33100, 5, 40),
+          (40000, 15, 33)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows,dim,hidden", NARROW)
+def test_narrow(cuda, rows, dim, hidden, kind):
+    bias = dim % 2 == 1
+    act = ("silu", "gelu", "sigmoid")[rows % 3]
+    args, dh = _case(rows, dim, hidden, kind, bias, rows + dim)
+    want, tol = _reference(*args, dh, act, TYPES[kind])
+    for name, got, v, t in zip(NAMES, _run(cuda, args, dh, act), want, tol):
+        _check(got, v, t, f"{name} {rows}x{dim}->{hidden} {kind} {act}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows", [50, 300])
+def test_narrow_views_and_parts(cuda, kind, rows):
+    """Rows of wider buffers that hold NaN around them, at odd addresses, give the same bits; so does a
+    backward pass that is asked for one gradient only."""
+    from gsr.layers import gated_linear
+    args, dh = _case(rows, 9, 205, kind, True, 3)
+    full = _run(cuda, args, dh, "silu")
+
+    def inside(t, left, right):
+        wide = torch.full((t.shape[0], left + t.shape[1] + right), float("nan"), device=cuda, dtype=t.dtype)
+        wide[:, left:left + t.shape[1]] = t
+        return wide[:, left:left + t.shape[1]]
+    leaves = [inside(args[0].to(cuda), 1, 2).requires_grad_(True)] + [t.to(cuda).requires_grad_(True) for t in args[1:]]
+    h = gated_linear(*leaves)
+    for a, b in zip(full, [h, *torch.autograd.grad(h, leaves, inside(dh.to(cuda), 3, 1))]):
+        assert torch.equal(a, b)
+    for which in range(5):
+        leaves = [t.to(cuda).requires_grad_(k == which) for k, t in enumerate(args)]
+        (g,) = torch.autograd.grad(gated_linear(*leaves), [leaves[which]], dh.to(cuda))
+        assert torch.equal(g, full[1 + which])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows", [40, 300])
+def test_narrow_bad_values_stay_alone(cuda, kind, rows):
+    """A row of x that is not finite reaches its own dx and no other row's; a weight row that is not
+    finite its own gradients and no other weight row's, also where rows end inside a tile."""
+    args, dh = _case(rows, 6, 70, kind, True, 9)
+    first = _run(cuda, args, dh, "silu")
+    bad = [t.clone() for t in args]
+    bad[0][1, 3], bad[0][rows - 1, 0] = float("nan"), float("inf")
+    again = _run(cuda, bad, dh, "silu")
+    keep = torch.ones(rows, dtype=torch.bool)
+    keep[1] = keep[rows - 1] = False
+    for k in (0, 1):
+        assert torch.equal(first[k].cpu()[keep], again[k].cpu()[keep])
+        assert bool(again[k][1].isnan().all()) and not bool(again[k][rows - 1].isfinite().all())
+    bad = [t.clone() for t in args]
+    bad[1][20, 2], bad[4][60] = float("nan"), float("inf")
+    again = _run(cuda, bad, dh, "silu")
+    keep = torch.ones(70, dtype=torch.bool)
+    keep[20] = keep[60] = False
+    assert torch.equal(first[0].cpu()[:, keep], again[0].cpu()[:, keep])
+    for k in (2, 3, 4, 5):
+        assert torch.equal(first[k].cpu()[keep], again[k].cpu()[keep])
+    assert bool(again[2][20].isnan().all())
+
+
 def test_refusals():
     from gsr import _lib
     from gsr.layers import GatedLinear, gated_linear
@@ -413,9 +482,9 @@ def test_refusals():
                     (dict(stride=7), b"row stride"), (dict(t=3), b"bad type"), (dict(act=4), b"bad activation"),
                     ({}, b"null pointer"), (dict(hidden=1 << 21), b"bad dim")]:
         assert fwd(**kw) == -1 and msg in L.gsr_last_error(), kw
-    bwd = lambda ws, n, dh=1: L.gsr_gated_bwd(1, 4, 8, 8, 0, 1, 1, 6, None, None, 0, dh, 6, None, 1, 1, 1, None, None, ws,  # noqa: E731
+    bwd = lambda ws, n, dh=1: L.gsr_gated_bwd(1, 4, 24, 24, 0, 1, 1, 6, None, None, 0, dh, 6, None, 1, 1, 1, None, None, ws,  # noqa: E731
                                               n, None)
     assert bwd(1, 16) == -1 and b"workspace" in L.gsr_last_error()
     assert bwd(1, 1 << 20, dh=None) == -1 and b"null" in L.gsr_last_error()
-    assert L.gsr_gated_workspace(4, 8, 6, 0, 1) >= 4 * 128 * 4 and L.gsr_gated_workspace(4, 8, 6, 7, 1) == 0
+    assert L.gsr_gated_workspace(4, 24, 6, 0, 1) >= 4 * 128 * 4 and L.gsr_gated_workspace(4, 24, 6, 7, 1) == 0
     assert L.gsr_gated_workspace(4, 8, 6, 1, 0) == 0 and L.gsr_gated_workspace(0, 8, 6, 1, 1) == 0
