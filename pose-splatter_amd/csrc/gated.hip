@@ -484,7 +484,7 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
   w.n_dx = w.dx > 64 ? 1 : gated_shares(rb * db, 2 * pad, s.rows * s.dim);
   w.n_dw = w.dw > 64 ? 1 : gated_shares(hb * db, s.rows, 2 * s.hidden * s.dim);
   const auto cuts = [type](int side, int64_t r, int64_t c, int64_t k) {
-    return gated_wide_rounds(side, ceil_div64(r, side), ceil_div64(c, side), gated_wide_steps(type, k)).bytes(side);
+    return gated_wide_rounds(type, side, ceil_div64(r, side), ceil_div64(c, side), gated_wide_steps(type, k)).bytes(side);
   };
   if (s.rows <= kSkinnyRows) w.fwd = 64;   // (the kernel for few rows)
   const bool xw = w.fwd > 64 || (backward && w.dw > 64), ww = w.fwd > 64 || (backward && w.dx > 64);

@@ -26,7 +26,7 @@ struct WideRounds {
   int whole, cut, shares;
   int64_t bytes(int side) const { return cut ? (int64_t)cut * shares * side * side * 4 : 0; }
 };
-WideRounds gated_wide_rounds(int side, int64_t mt, int64_t nt, int64_t steps);
+WideRounds gated_wide_rounds(int type, int side, int64_t mt, int64_t nt, int64_t steps);
 
 // Steps of 128 bytes of K.
 inline int64_t gated_wide_steps(int type, int64_t k) { return ceil_div64(k * (int64_t)type_size(type), 128); }

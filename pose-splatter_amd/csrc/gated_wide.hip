@@ -343,23 +343,37 @@ static void wide_launch(int mode, const GatedWide& a, hipStream_t st) {
   }
 }
 
-// The rounds of a product of mt x nt tiles: `slots` workgroups run at once, so the tiles of an
-// incomplete last round are cut along K into as many shares as fill it, each at least eight steps.
-WideRounds gated_wide_rounds(int side, int64_t mt, int64_t nt, int64_t steps) {
-  const int64_t slots = side == 256 ? 256 : 512, tiles = mt * nt;
-  WideRounds r{(int)tiles, 0, 1};
-  const int64_t cut = tiles % slots;
-  int64_t shares = cut ? slots / cut : 1;
-  shares = shares < steps / 8 ? shares : steps / 8;
-  if (shares > 1) r = WideRounds{(int)(tiles - cut), (int)cut, (int)shares};
-  return r;
+// How a product of mt x nt tiles is cut.  Work goes by CU: tiles that do not make up whole rounds of 256 are
+// cut along K into the shares, each at least eight steps, that end first by a model in steps of K:
+// a CU takes its workgroups' steps, `open` for each one's first loads and last stores, a tenth more
+// where one of 128 has the CU to itself (two fill each other's gaps; 256 always has), and for each
+// share `part`, its sums' way through memory, beside the join's launch.  Fitted to fp32 (72 tiles of
+// 188 steps: 3 shares 138 us, 7 118; 250 of 32: whole 72, 2 78; 128 of 128: 2 142, 4 137; 16 of
+// 500: 16 73, 32 80; 141 of 94: whole 186, 3 135) and bf16 (256 tiles of 128, 88 steps: whole 51, 2
+// 57).
+WideRounds gated_wide_rounds(int type, int side, int64_t mt, int64_t nt, int64_t steps) {
+  const int64_t tiles = mt * nt, cut = tiles % 256;
+  const double open = type == GSR_F32 ? 2. : side == 256 ? 3.5 : 4., part = type == GSR_F32 ? .015 : side == 256 ? .08 : .06;
+  const double join = type == GSR_F32 ? 1.5 : side == 256 ? 2. : 6.;
+  const int64_t most = steps / 8 < 64 ? steps / 8 : 64;
+  int64_t shares = 1;
+  double best = 0.;
+  for (int64_t n = 1; cut && (n == 1 || n <= most); ++n) {
+    const int64_t each = ceil_div64(cut * n, 256);   // workgroups a CU
+    if (n > 1 && each > (side == 256 ? 1 : 2)) break;   // all run at once
+    double cost = each * ((double)steps / n + open);
+    if (each == 1 && side == 128 && tiles < 256) cost *= 1.1;
+    if (n > 1) cost += join + part * cut * n;
+    if (n == 1 || cost < best) best = cost, shares = n;
+  }
+  return shares > 1 ? WideRounds{(int)(tiles - cut), (int)cut, (int)shares} : WideRounds{(int)tiles, 0, 1};
 }
 
 void gated_wide(int type, int mode, int side, GatedWide a, hipStream_t st) {
   const int64_t pad = gated_pad(a.s.hidden);
   a.mt = ceil_div(mode == kWideDw ? 2 * pad : a.s.rows, side);
   a.nt = mode <= kWideGrad ? ceil_div(pad, side / 2) : ceil_div(a.s.dim, side);
-  const WideRounds r = gated_wide_rounds(side, a.mt, a.nt, gated_wide_steps(type, mode == kWideDw ? a.s.rows : 2 * pad));
+  const WideRounds r = gated_wide_rounds(type, side, a.mt, a.nt, gated_wide_steps(type, mode == kWideDw ? a.s.rows : 2 * pad));
   a.whole = r.whole, a.cut = r.cut, a.shares = r.shares;
   if (type == GSR_F32) {
     wide_launch<float, 128>(mode, a, st);
