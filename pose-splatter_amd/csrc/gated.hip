@@ -404,16 +404,18 @@ __global__ __launch_bounds__(256) void k_gated_pad(GatedPads<T> a) {
 // Tile side of a product of rows x cols outputs over k.  256 (16 bits) where every CU gets at least 96
 // steps of K: 16384 x 2048 -> 5632, at 352 a CU, forward 660 us against 726 with 128, dW 593
 // against 877; at 88 the two are within 5 %; at 31 (16000 x 512 -> 2048) 111 us against 101.
-// 64 (any alignment, no padded copies) for dims whose K is hardly a step; and where the 512 workgroups
-// of 128 would get fewer than 8 steps in fp32, whose products are long enough to run side by side
-// (256 x 1024 -> 2816, 5.5 steps: forward 56 us against 70; 16000 x 256 -> 512, 16: 84 against 77),
-// or with few rows (dx of 4 x 1024 -> 2816, 1.4: 10 us against 14; of 1 x 4096 -> 11264, 22: 106
-// against 40).
+// 64 (any alignment, no padded copies) for dims whose K is hardly a step, and dx and dW of 64 columns,
+// half a tile; and where 128 has fewer than two steps a CU, its tiles cut along K as well, in fp32 or
+// with few rows.  Forward and backward, 128 against 64: fp32 500 x 1000 -> 1000 100 us against 190, 256
+// x 1024 -> 2816 128 against 197, 16000 x 128 -> 256 105 against 126; 200 x 100 -> 1000 59 against 43,
+// 2000 x 128 -> 128 52 against 48; dx of 16 x 2048 -> 4096 bf16 19 us against 25, of 40 x 1024 ->
+// 2816 14.5 against 14.0.
 static int gated_side(int type, int64_t rows, int64_t cols, int64_t k, GatedShape s) {
   const bool few = s.rows <= kSkinnyRows;
   if (s.dim < 64 || (few && s.dim % 8)) return 64;
   const int64_t steps = gated_wide_steps(type, k);
-  if (type == GSR_F32 || few) return ceil_div64(rows, 128) * ceil_div64(cols, 128) * steps >= 512 * 8 ? 128 : 64;
+  if (type == GSR_F32 && cols <= 64) return 64;
+  if (type == GSR_F32 || few) return ceil_div64(rows, 128) * ceil_div64(cols, 128) * steps >= 512 ? 128 : 64;
   return ceil_div64(rows, 256) * ceil_div64(cols, 256) * steps >= 256 * 96 ? 256 : 128;
 }
 
@@ -452,7 +454,7 @@ struct GatedPlan {
   bool exact;                    // the backward's products take the projections' gradients in fp32
   int64_t n_dx, n_dw;            // shares
   int64_t kdim;                  // dim in whole 16-byte pieces
-  int64_t x, wg, wu, dgu, bias, bias_rows, dx_parts, dw_parts, total;
+  int64_t x, wg, wu, cuts, dgu, bias, bias_rows, dx_parts, dw_parts, total;   // (cuts: the forward's)
 };
 
 // Whether the backward is one kernel (gated_narrow.hip).
@@ -491,6 +493,9 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
   w.x = take(xw ? s.rows * w.kdim * es : 0);
   w.wg = take(ww ? s.hidden * w.kdim * es : 0);
   w.wu = take(ww ? s.hidden * w.kdim * es : 0);
+  w.cuts = take(w.fwd > 64 && !backward
+                    ? gated_wide_rounds(type, w.fwd, ceil_div64(s.rows, w.fwd), ceil_div64(pad, w.fwd / 2), gated_wide_steps(type, s.dim)).bytes(w.fwd)
+                    : 0);
   w.keep = w.fwd > 64 && gated_keeps(type, s.dim);
   w.bias_rows = s.rows <= kSkinnyRows ? 1 : w.fwd > 64 ? ceil_div64(s.rows, w.fwd) * 2 : rb;
   w.dgu = take(backward ? s.rows * 2 * pad * (w.exact ? 4 : es) : 0);
@@ -544,7 +549,7 @@ static void gated_fwd(const T* x, int64_t x_stride, const T* wg, const T* wu, co
   const GatedPlan w = gated_plan(s, type, false);
   if (w.fwd > 64) {
     GatedWide a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, true, true, ws, st);
-    a.h = h, a.kept = w.keep ? kept : nullptr;
+    a.h = h, a.kept = w.keep ? kept : nullptr, a.cuts = (float*)(ws + w.cuts);
     gated_wide(type, kWideFwd, w.fwd, a, st);
     return;
   }

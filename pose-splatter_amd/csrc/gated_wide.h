@@ -15,7 +15,7 @@ struct GatedWide {
   const void *x, *wg, *wu, *bg, *bu, *dh;
   void *h, *kept, *dgu, *dx, *dwg, *dwu;   // kept: NULL, or the forward's projections (Kept)
   float* parts;   // gradients: column sums [ceil(rows / side) * 2][2][hidden], or NULL
-  float* cuts;    // dx, dW: the cut tiles' sums [shares][cut][side][side]
+  float* cuts;    // forward, dx, dW: the cut tiles' sums [shares][cut][side][side]
   int act;
   bool dgu32;     // gradients: dgu is written in fp32
   int mt, nt, whole, cut, shares;   // set by the launch: tiles, and how they are cut (gated_wide_rounds)

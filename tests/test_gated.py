@@ -376,6 +376,27 @@ def test_head_trains(cuda):
         assert float((p.grad.double().cpu() - leaf[k].grad).abs().max()) <= 4096 * U * float(leaf[k].grad.abs().max()) + 1e-5, k
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows,dim,hidden", [(100, 4000, 1000), (70, 1001, 517), (300, 2056, 700), (129, 1024, 64), (500, 1000, 1000),
+                                             (65, 4096, 1)])
+def test_few_tiles(cuda, rows, dim, hidden, kind):
+    """Long rows and few tiles: every product's K in shares, the forward's among them."""
+    bias = rows % 2 == 1
+    act = ("silu", "gelu", "sigmoid")[hidden % 3]
+    args, dh = _case(rows, dim, hidden, kind, bias, rows + dim)
+    want, tol = _reference(*args, dh, act, TYPES[kind])
+    out = _run(cuda, args, dh, act)
+    for name, got, v, t in zip(NAMES, out, want, tol):
+        _check(got, v, t, f"{name} {rows}x{dim}->{hidden} {kind} {act}")
+    again = [a.clone() if k == 0 else a for k, a in enumerate(args)]
+    again[0][3, 5] = float("nan")
+    keep = torch.arange(rows) != 3
+    bad = _run(cuda, again, dh, act)
+    for k in (0, 1):
+        assert torch.equal(bad[k].cpu()[keep], out[k].cpu()[keep]) and bool(bad[k][3].isnan().all())
+
+
 # dim <= 15: one row, one column; rows that end inside 16 and 64; each width of a step of 4; few rows and many columns
 # (dx in shares); more row tiles than workgroups
 NARROW = [(1, 15, 2050), (15, 4, 16), (64, 7, 17), (70, 15, 400), (129, 12, 128), (400, 2, 1000), (20000, 1, 7), (33100, 5, 40),
