@@ -397,6 +397,31 @@ def test_few_tiles(cuda, rows, dim, hidden, kind):
         assert torch.equal(bad[k].cpu()[keep], out[k].cpu()[keep]) and bool(bad[k][3].isnan().all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [8, 256])
+def test_more_rows_than_a_grid_side(cuda, dim):
+    """4.2 million rows (65536 blocks of 64 and more): the first and last ones against the definition, the
+    bias gradient against a sum of what the rows give."""
+    from gsr.layers import gated_linear
+    rows, hidden = 65536 * 64 + 100, 8
+    g = torch.Generator(device=cuda).manual_seed(1)
+    (_, wg, wu, bg, bu), _ = _case(1, dim, hidden, "bf16", True, 4)
+    x = torch.randn(rows, dim, device=cuda, generator=g, dtype=torch.bfloat16)
+    dh = torch.randn(rows, hidden, device=cuda, generator=g, dtype=torch.bfloat16)
+    leaves = [x.requires_grad_(True)] + [t.to(cuda).requires_grad_(True) for t in (wg, wu, bg, bu)]
+    h = gated_linear(*leaves)
+    dx, db = torch.autograd.grad(h, [leaves[0], leaves[4]], dh)
+    for at in (slice(0, 100), slice(rows - 200, rows)):
+        want, tol = _reference(x.detach()[at].cpu(), wg, wu, bg, bu, dh[at].cpu(), "silu", torch.bfloat16)
+        _check(h[at], want[0], tol[0], "h")
+        _check(dx[at], want[1], tol[1], "dx")
+    gate = torch.nn.functional.silu(x.detach().double() @ wg.to(cuda).double().T + bg.to(cuda).double())
+    terms = dh.double() * gate
+    # (each term is off by at most 2^-12 of |dh| (1 + |gate|), their sum by c(rows) of sum|terms|, then bf16)
+    limit = 2.0 ** -12 * (dh.double().abs() * (1 + gate.abs())).sum(0) + (rows + 16) * U * terms.abs().sum(0)
+    assert bool(((db.double() - terms.sum(0)).abs() <= limit + 2.0 ** -8 * terms.sum(0).abs()).all())
+
+
 # dim <= 15: one row, one column; rows that end inside 16 and 64; each width of a step of 4; few rows and many columns
 # (dx in shares); more row tiles than workgroups
 NARROW = [(1, 15, 2050), (15, 4, 16), (64, 7, 17), (70, 15, 400), (129, 12, 128), (400, 2, 1000), (20000, 1, 7), (33100, 5, 40),
