@@ -487,6 +487,9 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
   }
   const int64_t pad = gated_pad(s.hidden);
   w.fwd = gated_side(type, s.rows, 2 * pad, s.dim, s);
+  // (fp32's forward: from eight steps on, which shares of two cut well; 325 x 592 -> 398 19 us against 37 in 64 x 64
+  // tiles, and its backward 34 against 68, from kept projections)
+  if (type == GSR_F32 && s.rows > kSkinnyRows && gated_wide_steps(type, s.dim) >= 8) w.fwd = 128;
   w.exact = gated_exact(type, s);
   w.dx = w.exact ? 64 : gated_side(type, s.rows, s.dim, 2 * pad, s);
   w.dw = w.exact ? 64 : gated_side(type, 2 * pad, s.dim, s.rows, s);

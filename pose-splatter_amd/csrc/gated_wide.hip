@@ -381,10 +381,11 @@ static void wide_launch(int mode, const GatedWide& a, hipStream_t st) {
 }
 
 // How a product of mt x nt tiles is cut.  Work goes by CU: tiles that do not make up whole rounds of 256 are
-// cut along K into the shares, each at least eight steps, that end first by a model in steps of K:
-// a CU takes its workgroups' steps, `open` for each one's first loads and last stores, a tenth more
-// where one of 128 has the CU to itself (two fill each other's gaps; 256 always has), and for each
-// share `part`, its sums' way through memory, beside the join's launch.  Fitted to fp32 (72 tiles of
+// cut along K into the shares (each at least eight steps, or two of fp32's, which take four times as
+// long) that end first by a model in steps of K: a CU takes its workgroups' steps, `open` for each
+// one's first loads and last stores, a tenth more where one of 128 has the CU to itself (two fill each
+// other's gaps; 256 always has), and for each share `part`, its sums' way through memory, beside the
+// join's launch.  Fitted to fp32 (72 tiles of
 // 188 steps: 3 shares 138 us, 7 118; 250 of 32: whole 72, 2 78; 128 of 128: 2 142, 4 137; 16 of
 // 500: 16 73, 32 80; 141 of 94: whole 186, 3 135) and bf16 (256 tiles of 128, 88 steps: whole 51, 2
 // 57).  A forward's cut tiles get their activation in the join: 100 x 4000 -> 1000 fp32 31 us against
@@ -393,7 +394,7 @@ WideRounds gated_wide_rounds(int type, int side, int64_t mt, int64_t nt, int64_t
   const int64_t tiles = mt * nt, cut = tiles % 256;
   const double open = type == GSR_F32 ? 2. : side == 256 ? 3.5 : 4., part = type == GSR_F32 ? .015 : side == 256 ? .08 : .06;
   const double join = type == GSR_F32 ? 1.5 : side == 256 ? 2. : 6.;
-  const int64_t most = steps / 8 < 64 ? steps / 8 : 64;
+  const int64_t least = type == GSR_F32 ? 2 : 8, most = steps / least < 64 ? steps / least : 64;
   int64_t shares = 1;
   double best = 0.;
   for (int64_t n = 1; cut && (n == 1 || n <= most); ++n) {

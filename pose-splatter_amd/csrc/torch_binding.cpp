@@ -33,6 +33,7 @@ struct Calls {
   decltype(&::gsr_gated_workspace) gated_workspace;
   decltype(&::gsr_gated_bwd) gated_bwd;
   decltype(&::gsr_adamw_step) adamw_step;
+  decltype(&::gsr_adamw_decode_root) adamw_decode_root;
 } gsr;
 
 void bind(const std::string& path) {
@@ -52,6 +53,7 @@ void bind(const std::string& path) {
   take(c.gated_workspace, "gsr_gated_workspace");
   take(c.gated_bwd, "gsr_gated_bwd");
   take(c.adamw_step, "gsr_adamw_step");
+  take(c.adamw_decode_root, "gsr_adamw_decode_root");
   gsr = c;   // only a library that has them all
 }
 
@@ -277,10 +279,36 @@ bool same_layout(const Tensor& a, const Tensor& b) {
   return true;
 }
 
-void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& ms,
-                const std::vector<Tensor>& vs, double lr, const std::optional<Tensor>& lr_dev, double beta1, double beta2, double eps,
-                double weight_decay, int64_t step, const std::optional<std::vector<Tensor>>& steps,
-                const std::optional<std::vector<Tensor>>& m_units, const std::optional<std::vector<Tensor>>& v_units) {
+// The tensors of a list, read in place: converting hundreds of them one by one costs more than the step.
+class Tensors {
+  py::object seq_;   // keeps them alive
+  std::vector<const Tensor*> t_;
+
+ public:
+  Tensors(py::handle list, const char* what) : seq_(py::reinterpret_steal<py::object>(PySequence_Fast(list.ptr(), what))) {
+    if (!seq_) throw py::error_already_set();
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq_.ptr());
+    PyObject** items = PySequence_Fast_ITEMS(seq_.ptr());
+    t_.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      TORCH_CHECK_TYPE(THPVariable_Check(items[i]), what, ", got a ", Py_TYPE(items[i])->tp_name);
+      t_.push_back(&THPVariable_Unpack(items[i]));
+    }
+  }
+  size_t size() const { return t_.size(); }
+  const Tensor& operator[](size_t i) const { return *t_[i]; }
+};
+
+void adamw_step(py::handle param_list, py::handle grad_list, py::handle m_list, py::handle v_list, double lr,
+                const std::optional<Tensor>& lr_dev, double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                py::handle step_list, py::handle m_unit_list, py::handle v_unit_list) {
+  const Tensors params(param_list, "adamw_step: params must be a list of tensors"),
+      grads(grad_list, "adamw_step: grads must be a list of tensors"), ms(m_list, "adamw_step: exp_avgs must be a list of tensors"),
+      vs(v_list, "adamw_step: exp_avg_sqs must be a list of tensors");
+  const auto maybe = [](py::handle list, const char* what) { return list.is_none() ? std::nullopt : std::optional<Tensors>(Tensors(list, what)); };
+  const auto steps = maybe(step_list, "adamw_step: step must be a number, a tensor or a list of tensors"),
+             m_units = maybe(m_unit_list, "adamw_step: exp_avg_units must be a list of tensors"),
+             v_units = maybe(v_unit_list, "adamw_step: exp_avg_root_units must be a list of tensors");
   const size_t count = params.size();
   TORCH_CHECK_VALUE(m_units.has_value() == v_units.has_value(), "adamw_step: exp_avg_units and exp_avg_root_units go together");
   const bool byte = m_units.has_value();
@@ -302,14 +330,14 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
     std::vector<gsr_adamw_tensor> list;
   };
   std::vector<Group> groups;
-  std::vector<std::pair<uintptr_t, uintptr_t>> written;
+  std::vector<std::pair<uintptr_t, uintptr_t>> written[5];   // what is written, a list each
   std::vector<Tensor> kept;   // gradients copied into their parameter's layout
-  written.reserve(count * 5);
-  const auto writes = [&](const Tensor& t) {
+  const auto writes = [&](int list, const Tensor& t) {
     const auto at = (uintptr_t)t.data_ptr();
-    written.emplace_back(at, at + t.numel() * t.element_size());
-    return t.data_ptr();
+    written[list].emplace_back(at, at + t.numel() * t.element_size());
+    return (void*)at;
   };
+  for (auto& w : written) w.reserve(count);
   const auto mtype = byte ? at::kFloat8_e4m3fn : at::kFloat, vtype = byte ? at::kByte : at::kFloat;
   for (size_t i = 0; i < count; ++i) {
     const Tensor &p = params[i], &m = ms[i], &v = vs[i];
@@ -343,16 +371,29 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
       kept.push_back(g);
     }
     gsr_adamw_tensor t{};
-    t.p = writes(p), t.g = g.data_ptr(), t.m = writes(m), t.v = writes(v), t.n = n;
-    if (byte) t.m_unit = (float*)writes((*m_units)[i]), t.v_unit = (float*)writes((*v_units)[i]);
+    t.p = writes(0, p), t.g = g.data_ptr(), t.m = writes(1, m), t.v = writes(2, v), t.n = n;
+    if (byte) t.m_unit = (float*)writes(3, (*m_units)[i]), t.v_unit = (float*)writes(4, (*v_units)[i]);
     if (steps) t.step = (*steps)[i].data_ptr<int64_t>();
     auto at = std::find_if(groups.begin(), groups.end(), [&](const Group& x) { return x.p == pt && x.g == gt; });
-    if (at == groups.end()) at = groups.insert(at, Group{pt, gt, {}});
+    if (at == groups.end()) {
+      at = groups.insert(at, Group{pt, gt, {}});
+      at->list.reserve(count);
+    }
     at->list.push_back(t);
   }
-  std::sort(written.begin(), written.end());
-  for (size_t i = 1; i < written.size(); ++i)
-    TORCH_CHECK_VALUE(written[i].first >= written[i - 1].second, "adamw_step: a tensor is listed twice, or tensors to be written overlap");
+  // Nothing is written twice: all of it in order of its addresses (each list mostly is in order).
+  for (auto& w : written)
+    if (!std::is_sorted(w.begin(), w.end())) std::sort(w.begin(), w.end());
+  size_t at[5] = {};
+  for (uintptr_t end = 0;;) {
+    int first = -1;
+    for (int k = 0; k < 5; ++k)
+      if (at[k] < written[k].size() && (first < 0 || written[k][at[k]] < written[first][at[first]])) first = k;
+    if (first < 0) break;
+    const auto& w = written[first][at[first]++];
+    TORCH_CHECK_VALUE(w.first >= end, "adamw_step: a tensor is listed twice, or tensors to be written overlap");
+    end = w.second;
+  }
   on_device(params[0], "adamw_step");
   gsr_adamw_args args{};
   args.lr = lr, args.beta1 = beta1, args.beta2 = beta2, args.eps = eps, args.weight_decay = weight_decay;
@@ -363,8 +404,24 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
   void* stream = stream_of(device);
   for (const Group& g : groups)
     check(gsr.adamw_step(g.list.data(), (int32_t)g.list.size(), g.p, g.g, &args, stream), "gsr_adamw_step");
-  for (const Tensor& p : params)
-    if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+  for (size_t i = 0; i < count; ++i)
+    if (!params[i].is_inference()) params[i].unsafeGetTensorImpl()->bump_version();
+}
+
+Tensor decode_root(const Tensor& codes, const Tensor& units) {
+  TORCH_CHECK_VALUE(codes.scalar_type() == at::kByte && codes.is_contiguous(), "decode_root: codes must be contiguous uint8, got ",
+                    codes.scalar_type());
+  TORCH_CHECK_VALUE(units.scalar_type() == at::kFloat && units.dim() == 1 && units.size(0) == units_of(codes.numel()) &&
+                        units.is_contiguous() && units.device() == codes.device(),
+                    "decode_root: units must be contiguous float32 [", units_of(codes.numel()), "] on ", codes.device(), ", got ",
+                    units.scalar_type(), " ", units.sizes(), " on ", units.device());
+  on_device(codes, "decode_root");
+  const c10::OptionalDeviceGuard guard(codes.device());
+  Tensor out = at::empty(codes.sizes(), codes.options().dtype(at::kFloat));
+  check(gsr.adamw_decode_root(codes.data_ptr<uint8_t>(), units.data_ptr<float>(), codes.numel(), out.data_ptr<float>(),
+                              stream_of(codes.device())),
+        "gsr_adamw_decode_root");
+  return out;
 }
 
 }  // namespace
@@ -374,5 +431,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_norm", &layer_norm);
   m.def("gated_linear", &gated_linear);
   m.def("adamw_step", &adamw_step);
+  m.def("decode_root", &decode_root);
   m.attr("ABI_VERSION") = GSR_ABI_VERSION;
 }

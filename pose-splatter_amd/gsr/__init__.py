@@ -3,6 +3,8 @@
 Package layout:
   _lib.py    ctypes binding of the C ABI (include/gsr.h); fails loudly if missing
   render.py  projection → binning → rasterisation orchestration + autograd
+  layers.py  layer norm and gated block of a trainable parameter head (head.GatedHead)
+  optim.py   AdamW over many tensors, moments in 32 or 8 bits
   scenes.py  deterministic synthetic scenes for the benchmark configs
 """
 from ._lib import GsrLibraryError, LIB_PATH

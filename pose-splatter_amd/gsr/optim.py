@@ -20,8 +20,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import check, lib, native
-from .render import _require_device, _stream
+from ._lib import native
+from .render import _require_device
 
 __all__ = ["AdamW", "adamw_step", "decode_root"]
 
@@ -58,18 +58,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, lr=1e-3, betas=(0.9, 0.9
 def decode_root(codes: torch.Tensor, units: torch.Tensor) -> torch.Tensor:
     """The roots sqrt(v) (float32, codes' shape) that the uint8 codes of an 8-bit second moment
     stand for; codes contiguous, units [ceil(numel / 256)] float32."""
-    if codes.dtype != torch.uint8 or not codes.is_contiguous():
-        raise ValueError(f"decode_root: codes must be contiguous uint8, got {codes.dtype}")
-    if units.dtype != torch.float32 or units.shape != (_units(codes.numel()),) or not units.is_contiguous() \
-            or units.device != codes.device:
-        raise ValueError(f"decode_root: units must be contiguous float32 [{_units(codes.numel())}] on {codes.device}, "
-                         f"got {units.dtype} {tuple(units.shape)} on {units.device}")
-    _require_device(codes, "decode_root")
-    out = torch.empty(codes.shape, device=codes.device, dtype=torch.float32)
-    with torch.cuda.device(codes.device):
-        check(lib().gsr_adamw_decode_root(codes.data_ptr(), units.data_ptr(), codes.numel(), out.data_ptr(),
-                                          _stream(codes.device)), "gsr_adamw_decode_root")
-    return out
+    return native().decode_root(codes, units)
 
 
 class AdamW(torch.optim.Optimizer):
