@@ -703,7 +703,7 @@ int gsr_layer_norm_bwd(const void* x, const void* dy, int64_t rows, int64_t dim,
  * bwd: from dh [rows, hidden] (row stride dh_stride) the gradients dx [rows, dim], dwg, dwu
  * [hidden, dim], dbg, dbu [hidden] (each may be NULL), contiguous.  dg and du are rounded to the
  * type before the products that use them, as the projections' outputs' gradients would be, save in
- * small cases, which multiply them in fp32.
+ * small cases and for dim <= 15, which multiply them in fp32.
  * kept: device, 256-byte aligned, gsr_gated_kept bytes, or NULL: g and u as the forward leaves them
  * for its backward.  Without it (where the bytes are 0, or by choice) the backward computes both
  * projections again.

