@@ -704,9 +704,9 @@ int gsr_layer_norm_bwd(const void* x, const void* dy, int64_t rows, int64_t dim,
  * [hidden, dim], dbg, dbu [hidden] (each may be NULL), contiguous.  dg and du are rounded to the
  * type before the products that use them, as the projections' outputs' gradients would be, save in
  * small cases and for dim <= 15, which multiply them in fp32.
- * kept: device, 256-byte aligned, gsr_gated_kept bytes, or NULL: g and u as the forward leaves them
- * for its backward.  Without it (where the bytes are 0, or by choice) the backward computes both
- * projections again.
+ * kept: device, 256-byte aligned, gsr_gated_kept bytes, or NULL: what the forward leaves for its
+ * backward, g and u, and copies of x and the weights where dim is not whole 16-byte pieces.  Without
+ * it (where the bytes are 0, or by choice) the backward makes them again.
  * workspace: device, 256-byte aligned, gsr_gated_workspace bytes (0: NULL).  Fixed-order sums. */
 #define GSR_ACT_SILU 0
 #define GSR_ACT_GELU 1     /* g Phi(g), the error function's form */

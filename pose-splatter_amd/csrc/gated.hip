@@ -461,6 +461,8 @@ static bool gated_exact(int type, GatedShape s) {
 struct GatedPlan {
   int fwd, dx, dw;               // tile sides
   bool keep;                     // the forward keeps its projections
+  bool keep_pads;                // and the padded copies of x and the weights, where dim is the reason for them
+  int64_t kept_pads, kept;       // their place behind the projections; bytes in all
   bool exact;                    // the backward's products take the projections' gradients in fp32
   int64_t n_dx, n_dw;            // shares
   int64_t kdim;                  // dim in whole 16-byte pieces
@@ -510,6 +512,9 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
                     ? gated_wide_rounds(type, w.fwd, ceil_div64(s.rows, w.fwd), ceil_div64(pad, w.fwd / 2), gated_wide_steps(type, s.dim)).bytes(w.fwd)
                     : 0);
   w.keep = w.fwd > 64 && gated_keeps(type, s.dim);
+  w.keep_pads = w.fwd > 64 && w.kdim != s.dim && (w.dx > 64 || w.dw > 64 || !w.keep);
+  w.kept_pads = !w.keep ? 0 : type == GSR_F32 ? Kept<float>::bytes(s.rows, s.hidden) : Kept<bf16>::bytes(s.rows, s.hidden);
+  w.kept = w.kept_pads + (w.keep_pads ? (s.rows + 2 * s.hidden) * w.kdim * es : 0);
   w.bias_rows = s.rows <= kSkinnyRows ? 1 : w.fwd > 64 ? ceil_div64(s.rows, w.fwd) * 2 : rb;
   w.dgu = take(backward ? s.rows * 2 * pad * (w.exact ? 4 : es) : 0);
   const int64_t kept_rows = w.keep ? ceil_div64(s.rows, gated_slopes_rows(s)) : 0;
@@ -523,10 +528,12 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
   return w;
 }
 
-// The wide products' operands, copied into whole 16-byte pieces where they are not.
+// The wide products' operands, copied into whole 16-byte pieces where they are not: for the backward too
+// (`pads`, NULL: not wanted) or in the workspace.  `made`: pads holds the copies already.
 template <typename T>
 static GatedWide gated_wide_args(const T* x, int64_t x_stride, const T* wg, const T* wu, const void* bg, const void* bu, int act,
-                                 GatedShape s, const GatedPlan& w, bool use_x, bool use_w, char* ws, hipStream_t st) {
+                                 GatedShape s, const GatedPlan& w, bool use_x, bool use_w, char* ws, T* pads, bool made,
+                                 hipStream_t st) {
   GatedWide a{};
   a.s = s;
   a.kdim = w.kdim, a.x_stride = x_stride, a.w_stride = s.dim;
@@ -534,14 +541,16 @@ static GatedWide gated_wide_args(const T* x, int64_t x_stride, const T* wg, cons
   GatedPads<T> p{};
   p.dim = s.dim, p.kdim = w.kdim;
   if (use_x && !gated_aligned(x, s.dim, x_stride)) {
-    p.p[0] = x, p.to[0] = (T*)(ws + w.x), p.rows[0] = s.rows, p.stride[0] = x_stride;
+    p.p[0] = x, p.to[0] = pads ? pads : (T*)(ws + w.x), p.rows[0] = s.rows, p.stride[0] = x_stride;
     a.x = p.to[0], a.x_stride = w.kdim;
   }
   if (use_w && !(gated_aligned(wg, s.dim, s.dim) && gated_aligned(wu, s.dim, s.dim))) {
-    p.p[1] = wg, p.to[1] = (T*)(ws + w.wg), p.rows[1] = s.hidden, p.stride[1] = s.dim;
-    p.p[2] = wu, p.to[2] = (T*)(ws + w.wu), p.rows[2] = s.hidden, p.stride[2] = s.dim;
+    T* const to = pads ? pads + s.rows * w.kdim : nullptr;
+    p.p[1] = wg, p.to[1] = to ? to : (T*)(ws + w.wg), p.rows[1] = s.hidden, p.stride[1] = s.dim;
+    p.p[2] = wu, p.to[2] = to ? to + s.hidden * w.kdim : (T*)(ws + w.wu), p.rows[2] = s.hidden, p.stride[2] = s.dim;
     a.wg = p.to[1], a.wu = p.to[2], a.w_stride = w.kdim;
   }
+  if (made) return a;
   const int64_t pieces = (p.rows[0] + p.rows[1] + p.rows[2]) * (w.kdim / (16 / (int64_t)sizeof(T))), blocks = ceil_div64(pieces, 256);
   if (pieces) k_gated_pad<T><<<(unsigned)(blocks < 8192 ? blocks : 8192), 256, 0, st>>>(p);
   return a;
@@ -562,7 +571,8 @@ static void gated_fwd(const T* x, int64_t x_stride, const T* wg, const T* wu, co
   }
   const GatedPlan w = gated_plan(s, type, false);
   if (w.fwd > 64) {
-    GatedWide a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, true, true, ws, st);
+    T* const pads = kept && w.keep_pads ? (T*)((char*)kept + w.kept_pads) : nullptr;
+    GatedWide a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, true, true, ws, pads, false, st);
     a.h = h, a.kept = w.keep ? kept : nullptr, a.cuts = (float*)(ws + w.cuts);
     gated_wide(type, kWideFwd, w.fwd, a, st);
     return;
@@ -587,8 +597,9 @@ static void gated_bwd_as(const T* x, int64_t x_stride, const T* wg, const T* wu,
   GatedWide a{};
   if (w.fwd > 64 || w.dx > 64 || w.dw > 64) {
     const bool again = w.fwd > 64 && !keep;   // both projections are computed again
+    T* const pads = kept && w.keep_pads ? (T*)((char*)kept + w.kept_pads) : nullptr;
     a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, again || (weights && w.dw > 64), again || (dx && w.dx > 64), ws,
-                           st);
+                           pads, pads != nullptr, st);
     a.dh = dh, a.dh_stride = dh_stride, a.dgu = dgu, a.dgu32 = w.exact, a.dx = dx, a.dwg = dwg, a.dwu = dwu;
   }
   if (keep) {
@@ -667,8 +678,8 @@ extern "C" size_t gsr_gated_workspace(int64_t rows, int64_t dim, int64_t hidden,
 
 extern "C" size_t gsr_gated_kept(int64_t rows, int64_t dim, int64_t hidden, int32_t type) {
   const GatedShape s{rows, dim, hidden};
-  if (gated_check("gsr_gated_kept", s, dim, type, GSR_ACT_SILU) || rows == 0 || !gated_plan(s, type, false).keep) return 0;
-  return (size_t)(type == GSR_F32 ? Kept<float>::bytes(rows, hidden) : Kept<bf16>::bytes(rows, hidden));
+  if (gated_check("gsr_gated_kept", s, dim, type, GSR_ACT_SILU) || rows == 0) return 0;
+  return (size_t)gated_plan(s, type, false).kept;
 }
 
 extern "C" int gsr_gated_fwd(const void* x, int64_t rows, int64_t dim, int64_t x_stride, int32_t type, const void* wg,

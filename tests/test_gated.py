@@ -398,6 +398,29 @@ def test_few_tiles(cuda, rows, dim, hidden, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows,dim,hidden", [(300, 301, 300), (777, 509, 200), (200, 264, 136), (4200, 129, 1000)])
+def test_without_what_the_forward_keeps(cuda, rows, dim, hidden, kind):
+    """The C ABI's backward where the caller kept nothing: everything is made again."""
+    from gsr import _lib
+    L, t = _lib.lib(), {"f32": _lib.F32, "bf16": _lib.BF16, "f16": _lib.F16}[kind]
+    args, dh = _case(rows, dim, hidden, kind, True, 21)
+    want, tol = _reference(*args, dh, "silu", TYPES[kind])
+    dev = [v.to(cuda) for v in (*args, dh)]
+    out = [torch.full(s, float("nan"), device=cuda, dtype=TYPES[kind])
+           for s in ((rows, hidden), (rows, dim), (hidden, dim), (hidden, dim), (hidden,), (hidden,))]
+    x, wg, wu, bg, bu, d = (v.data_ptr() for v in dev)
+    stream = torch.cuda.current_stream().cuda_stream
+    ws = [torch.empty(max(1, L.gsr_gated_workspace(rows, dim, hidden, t, b)), device=cuda, dtype=torch.uint8) for b in (0, 1)]
+    _lib.check(L.gsr_gated_fwd(x, rows, dim, dim, t, wg, wu, hidden, bg, bu, 0, out[0].data_ptr(), None, ws[0].data_ptr(),
+                               ws[0].numel(), stream), "gsr_gated_fwd")
+    _lib.check(L.gsr_gated_bwd(x, rows, dim, dim, t, wg, wu, hidden, bg, bu, 0, d, hidden, None, *(o.data_ptr() for o in out[1:]),
+                               ws[1].data_ptr(), ws[1].numel(), stream), "gsr_gated_bwd")
+    for name, got, v, lim in zip(NAMES, out, want, tol):
+        _check(got, v, lim, f"{name} {rows}x{dim}->{hidden} {kind}")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dim", [8, 256])
 def test_more_rows_than_a_grid_side(cuda, dim):
     """4.2 million rows (65536 blocks of 64 and more): the first and last ones against the definition, the
