@@ -11,7 +11,9 @@
 // row while they reduce this one.  Each backward workgroup writes one row of partial dw and db,
 // which a second kernel adds in a fixed order: no atomics, the same bits every run.
 // Sums, statistics and partials are fp32; only y, dx, dw and db are rounded to their types.
-// 32768 x 4096 bf16: forward 111 us (4.85 TB/s, a copy's rate), backward 158 (5.1 TB/s).
+// 32768 x 4096 bf16: forward 106 us (5.1 TB/s), backward 160 (5.0 TB/s).
+#include <type_traits>
+
 #include "types.h"
 
 namespace gsr {
@@ -56,7 +58,34 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* lds) {
   }
 }
 
-template <typename T, int LANES, int NV>
+// The columns of a lane's k-th vector of a row.  EARLY, for rows of a vector or more: where one does not end
+// on a whole vector, its last one ends with the row instead and begins skip() columns early.  Those
+// belong to the lane before too, which writes the same values to them; sums leave them out.  Without
+// it that lane goes element by element, and every row's wave waits for up to seven more loads and
+// stores: 32768 x 4095 bf16 forward 166 us against 121, backward 261 against 193.
+template <int V, int LANES, bool EARLY>
+struct NormCols {
+  using Index = std::conditional_t<EARLY, int, int64_t>;   // (64 bits: what the backward without it schedules best)
+  Index dim;
+  int lane, last, early;   // the vector that ends the row (of some lane), and how early it begins
+  __device__ __forceinline__ NormCols(int64_t d) : dim((Index)d), lane(threadIdx.x % LANES), last(((int)d - 1) / (LANES * V)) {
+    const int c = (last * LANES + lane) * V;
+    early = EARLY && c < dim && c + V > dim ? c + V - (int)dim : 0;
+  }
+  // Makes what follows compute from `early` anew: kept over the rows, it would take registers by the dozen.
+  __device__ __forceinline__ void forget() {
+    if constexpr (EARLY) asm volatile("" : "+v"(early));
+  }
+  __device__ __forceinline__ int skip(int k) const { return EARLY && k == last ? early : 0; }
+  __device__ __forceinline__ Index at(int k) const { return (Index)(k * LANES + lane) * V - skip(k); }
+  __device__ __forceinline__ Index n(int k) const {
+    const Index left = dim - (Index)(k * LANES + lane) * V;
+    return EARLY ? (left > 0 ? V : 0) : left;
+  }
+  __device__ __forceinline__ bool in(int k, int i) const { return i >= skip(k) && i < n(k); }
+};
+
+template <typename T, int LANES, int NV, bool EARLY>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_norm_fwd(const T* x, int64_t rows, int64_t dim, int64_t stride,
                                                                         const void* w, const void* b, int wtype, float eps,
                                                                         T* y, float2* stats) {
@@ -64,13 +93,13 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_norm_fwd(const T*
   constexpr bool HOLD = LANES <= 256;   // (1024 threads leave no registers for the weights)
   __shared__ float lds[LANES > 64 ? 2 * (LANES / 64) : 1];
   const int lane = threadIdx.x % LANES;
+  NormCols<V, LANES, EARLY> cols(dim);
   float wv[HOLD ? NV : 1][V], bv[HOLD ? NV : 1][V];
   if constexpr (HOLD)
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t c = (int64_t)(k * LANES + lane) * V;
-      load_param(w, wtype, c, dim - c, wv[k], 1.f);
-      load_param(b, wtype, c, dim - c, bv[k], 0.f);
+      load_param(w, wtype, cols.at(k), cols.n(k), wv[k], 1.f);
+      load_param(b, wtype, cols.at(k), cols.n(k), bv[k], 0.f);
     }
   const int64_t step = (int64_t)gridDim.x * RPB;
   int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES;
@@ -78,8 +107,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_norm_fwd(const T*
   const auto fetch = [&](int64_t r) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t c = (int64_t)(k * LANES + lane) * V;
-      next[k].load(x + r * stride + c, dim - c);
+      next[k].load(x + r * stride + cols.at(k), cols.n(k));
     }
   };
   if (row < rows) fetch(row);
@@ -90,19 +118,19 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_norm_fwd(const T*
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         v[k][i] = next[k].at(i);
-        s[0] += v[k][i];
+        s[0] += !EARLY || i >= cols.skip(k) ? v[k][i] : 0.f;   // (columns that are not there hold zeros)
       }
     if (row + step < rows) fetch(row + step);
+    cols.forget();
     row_sum<LANES>(s, lds);
     const float mean = s[0] / (float)dim;
     s[0] = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t c = (int64_t)(k * LANES + lane) * V;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         v[k][i] -= mean;
-        s[0] += c + i < dim ? v[k][i] * v[k][i] : 0.f;
+        s[0] += cols.in(k, i) ? v[k][i] * v[k][i] : 0.f;
       }
     }
     row_sum<LANES>(s, lds + (LANES > 64 ? LANES / 64 : 0));
@@ -111,16 +139,15 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_norm_fwd(const T*
     T* yr = y + row * dim;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t c = (int64_t)(k * LANES + lane) * V;
-      if (c < dim) {
+      if (cols.n(k) > 0) {
         const int h = HOLD ? k : 0;
         if constexpr (!HOLD) {
-          load_param(w, wtype, c, dim - c, wv[0], 1.f);
-          load_param(b, wtype, c, dim - c, bv[0], 0.f);
+          load_param(w, wtype, cols.at(k), cols.n(k), wv[0], 1.f);
+          load_param(b, wtype, cols.at(k), cols.n(k), bv[0], 0.f);
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) v[k][i] = v[k][i] * rstd * wv[h][i] + bv[h][i];
-        store_upto(yr + c, dim - c, v[k]);
+        store_upto(yr + cols.at(k), cols.n(k), v[k]);
       }
     }
   }
@@ -168,7 +195,7 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(const T* x, int64_t rows
 // parts: [gridDim.x][2][dim] partial sums of dw and db (NULL: neither is wanted).  x and dy stay as they
 // were loaded (a row's two values of 16 bits in one register) and are widened again for dx: the
 // registers saved are waves that keep more loads in flight.
-template <typename T, int LANES, int NV>
+template <typename T, int LANES, int NV, bool EARLY>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256, LANES > 256 ? 1 : NV <= 2 ? 3 : 2) void k_norm_bwd(
     const T* x, const T* dy, int64_t rows, int64_t dim, int64_t stride, int64_t dy_stride, const void* w, int wtype,
     const float2* stats, T* dx, float* parts) {
@@ -178,10 +205,10 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256, LANES > 256 ? 1 : NV <= 
   __shared__ float lds[LANES > 64 ? 4 * W : 1];
   const int lane = threadIdx.x % LANES;
   const float inv = 1.f / (float)dim;
+  NormCols<V, LANES, EARLY> cols(dim);
   float wv[HOLD ? NV : 1][V], aw[NV][V] = {}, ab[NV][V] = {};
   const auto weights = [&](int k) {
-    const int64_t c = (int64_t)(k * LANES + lane) * V;
-    load_param(w, wtype, c, dim - c, wv[HOLD ? k : 0], 1.f);
+    load_param(w, wtype, cols.at(k), cols.n(k), wv[HOLD ? k : 0], 1.f);
   };
   if constexpr (HOLD)
 #pragma unroll
@@ -191,13 +218,12 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256, LANES > 256 ? 1 : NV <= 
   int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES;
   Raw<T> nx[NV], ng[NV];
   float2 next_st;
-  const auto fetch = [&](int64_t r) {   // (columns past dim: dy is zero there, whatever xhat is)
+  const auto fetch = [&](int64_t r) {
     next_st = stats[r];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t c = (int64_t)(k * LANES + lane) * V;
-      nx[k].load(x + r * stride + c, dim - c);
-      ng[k].load(dy + r * dy_stride + c, dim - c);
+      nx[k].load(x + r * stride + cols.at(k), cols.n(k));
+      ng[k].load(dy + r * dy_stride + cols.at(k), cols.n(k));
     }
   };
   if (HOLD && row < rows) fetch(row);
@@ -208,13 +234,15 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256, LANES > 256 ? 1 : NV <= 
 #pragma unroll
     for (int k = 0; k < NV; ++k) cx[k] = nx[k], cg[k] = ng[k];
     if (HOLD && row + step < rows) fetch(row + step);
+    cols.forget();
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       if constexpr (!HOLD) weights(k);
+      const int skip = cols.skip(k);   // (columns that are not there hold zeros of dy)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float z = (cx[k].at(i) - st.x) * st.y, d = cg[k].at(i);
+        const float z = (cx[k].at(i) - st.x) * st.y, d = !EARLY || i >= skip ? cg[k].at(i) : 0.f;
         aw[k][i] += d * z;
         ab[k][i] += d;
         s[0] += d * wv[HOLD ? k : 0][i];
@@ -227,15 +255,14 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256, LANES > 256 ? 1 : NV <= 
       const float m0 = s[0] * inv, m1 = s[1] * inv;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int64_t c = (int64_t)(k * LANES + lane) * V;
-        if constexpr (!HOLD) weights(k);
+          if constexpr (!HOLD) weights(k);
         float g[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const float z = (cx[k].at(i) - st.x) * st.y;
           g[i] = (cg[k].at(i) * wv[HOLD ? k : 0][i] - m0 - z * m1) * st.y;
         }
-        if (c < dim) store_upto(dx + row * dim + c, dim - c, g);
+        if (cols.n(k) > 0) store_upto(dx + row * dim + cols.at(k), cols.n(k), g);
       }
     }
   }
@@ -260,10 +287,12 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256, LANES > 256 ? 1 : NV <= 
     for (int k = 0; k < NV; ++k) {
       if (threadIdx.x % 64 < LANES)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          sum[threadIdx.x / 64][0][lane * V + i] = aw[k][i];
-          sum[threadIdx.x / 64][1][lane * V + i] = ab[k][i];
-        }
+        for (int i = 0; i < V; ++i)
+          if (!EARLY || cols.in(k, i)) {   // (from the vector's own first column on: inside these COLS)
+            const int at = (int)cols.at(k) + i - k * COLS;
+            sum[threadIdx.x / 64][0][at] = aw[k][i];
+            sum[threadIdx.x / 64][1][at] = ab[k][i];
+          }
       __syncthreads();
       for (int j = threadIdx.x; j < 2 * COLS; j += THREADS) {
         const int which = j / COLS, c = j % COLS;
@@ -276,10 +305,13 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256, LANES > 256 ? 1 : NV <= 
   } else {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int64_t c = (int64_t)(k * LANES + lane) * V;
-      if (c < dim) {
-        store_upto(out + c, dim - c, aw[k]);
-        store_upto(out + dim + c, dim - c, ab[k]);
+      if (EARLY && cols.skip(k) > 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (cols.in(k, i)) out[cols.at(k) + i] = aw[k][i], out[dim + cols.at(k) + i] = ab[k][i];
+      } else if (cols.n(k) > 0) {
+        store_upto(out + cols.at(k), cols.n(k), aw[k]);
+        store_upto(out + dim + cols.at(k), cols.n(k), ab[k]);
       }
     }
   }
@@ -425,11 +457,11 @@ static void norm_fwd(const void* x, int64_t rows, int64_t dim, int64_t stride, c
   }
   const int rpb = lanes > 256 ? 1 : 256 / lanes;
   const unsigned grid = norm_grid(ceil_div64(rows, rpb));
-#define GSR_CALL(L, N)                                                                                                    \
-  k_norm_fwd<T, L, N><<<grid, L > 256 ? L : 256, 0, s>>>((const T*)x, rows, dim, stride, w, b, wtype, eps, (T*)y, \
-                                                         (float2*)stats)
+  void (*f)(const T*, int64_t, int64_t, int64_t, const void*, const void*, int, float, T*, float2*) = nullptr;
+#define GSR_CALL(L, N) f = dim >= NormVec<T>::V ? k_norm_fwd<T, L, N, true> : k_norm_fwd<T, L, N, false>
   GSR_NORM_DISPATCH(GSR_CALL)
 #undef GSR_CALL
+  f<<<grid, lanes > 256 ? lanes : 256, 0, s>>>((const T*)x, rows, dim, stride, w, b, wtype, eps, (T*)y, (float2*)stats);
 }
 
 template <typename T>
@@ -446,11 +478,14 @@ static void norm_bwd(const void* x, const void* dy, int64_t rows, int64_t dim, i
                                                                             dy_stride, (const float2*)stats, parts);
     return;
   }
-#define GSR_CALL(L, N)                                                                                                     \
-  k_norm_bwd<T, L, N><<<n, L > 256 ? L : 256, 0, s>>>((const T*)x, (const T*)dy, rows, dim, stride, dy_stride, w, wtype, \
-                                                      (const float2*)stats, (T*)dx, parts)
+  // (early vectors take registers that 32 values a lane, or 1024 lanes, do not leave: 8359 x 7187 bf16 123 us, 118 without)
+  constexpr int V = NormVec<T>::V;
+  void (*f)(const T*, const T*, int64_t, int64_t, int64_t, int64_t, const void*, int, const float2*, T*, float*) = nullptr;
+#define GSR_CALL(L, N) f = dim >= V ? k_norm_bwd<T, L, N, ((N) * V < 32 && (L) <= 256)> : k_norm_bwd<T, L, N, false>
   GSR_NORM_DISPATCH(GSR_CALL)
 #undef GSR_CALL
+  f<<<n, lanes > 256 ? lanes : 256, 0, s>>>((const T*)x, (const T*)dy, rows, dim, stride, dy_stride, w, wtype, (const float2*)stats,
+                                            (T*)dx, parts);
 }
 
 static int norm_check(const char* who, int64_t rows, int64_t dim, int64_t stride, int xtype, int wtype) {
