@@ -460,11 +460,13 @@ static bool gated_exact(int type, GatedShape s) {
 // or addresses that are not multiples of 16 bytes.
 struct GatedPlan {
   int fwd, dx, dw;               // tile sides
+  bool beside;                   // dx and dW run side by side
   bool keep;                     // the forward keeps its projections
   bool keep_pads;                // and the padded copies of x and the weights, where dim is the reason for them
   int64_t kept_pads, kept;       // their place behind the projections; bytes in all
   bool exact;                    // the backward's products take the projections' gradients in fp32
   int64_t n_dx, n_dw;            // shares
+  WideRounds r_fwd, r_dx, r_dw;  // and those of the wide products
   int64_t kdim;                  // dim in whole 16-byte pieces
   int64_t x, wg, wu, cuts, dgu, bias, bias_rows, dx_parts, dw_parts, total;   // (cuts: the forward's)
 };
@@ -500,17 +502,25 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
   const int64_t rb = ceil_div64(s.rows, 64), hb = 2 * pad / 64, db = ceil_div64(s.dim, 64);
   w.n_dx = w.dx > 64 ? 1 : gated_shares(rb * db, 2 * pad, s.rows * s.dim);
   w.n_dw = w.dw > 64 ? 1 : gated_shares(hb * db, s.rows, 2 * s.hidden * s.dim);
-  const auto cuts = [type](int side, int64_t r, int64_t c, int64_t k) {
-    return gated_wide_rounds(type, side, ceil_div64(r, side), ceil_div64(c, side), gated_wide_steps(type, k)).bytes(side);
-  };
+  const auto tiles = [](int side, int64_t r, int64_t c) { return ceil_div64(r, side) * ceil_div64(c, side); };
+  const int64_t x_steps = gated_wide_steps(type, 2 * pad), w_steps = gated_wide_steps(type, s.rows);
+  WideRounds r[2];
+  w.beside = w.dx == 128 && w.dw == 128 &&
+             gated_wide_back_rounds(type, {tiles(128, s.rows, s.dim), tiles(128, 2 * pad, s.dim)}, {x_steps, w_steps}, r);
+  if (w.beside) {
+    w.r_dx = r[0], w.r_dw = r[1];
+  } else {
+    if (w.dx > 64) w.r_dx = gated_wide_rounds(type, w.dx, ceil_div64(s.rows, w.dx), ceil_div64(s.dim, w.dx), x_steps);
+    if (w.dw > 64) w.r_dw = gated_wide_rounds(type, w.dw, ceil_div64(2 * pad, w.dw), ceil_div64(s.dim, w.dw), w_steps);
+  }
   if (s.rows <= kSkinnyRows) w.fwd = 64;   // (the kernel for few rows)
   const bool xw = w.fwd > 64 || (backward && w.dw > 64), ww = w.fwd > 64 || (backward && w.dx > 64);
   w.x = take(xw ? s.rows * w.kdim * es : 0);
   w.wg = take(ww ? s.hidden * w.kdim * es : 0);
   w.wu = take(ww ? s.hidden * w.kdim * es : 0);
-  w.cuts = take(w.fwd > 64 && !backward
-                    ? gated_wide_rounds(type, w.fwd, ceil_div64(s.rows, w.fwd), ceil_div64(pad, w.fwd / 2), gated_wide_steps(type, s.dim)).bytes(w.fwd)
-                    : 0);
+  if (w.fwd > 64)
+    w.r_fwd = gated_wide_rounds(type, w.fwd, ceil_div64(s.rows, w.fwd), ceil_div64(pad, w.fwd / 2), gated_wide_steps(type, s.dim));
+  w.cuts = take(w.fwd > 64 && !backward ? w.r_fwd.bytes(w.fwd) : 0);
   w.keep = w.fwd > 64 && gated_keeps(type, s.dim);
   w.keep_pads = w.fwd > 64 && w.kdim != s.dim && (w.dx > 64 || w.dw > 64 || !w.keep);
   w.kept_pads = !w.keep ? 0 : type == GSR_F32 ? Kept<float>::bytes(s.rows, s.hidden) : Kept<bf16>::bytes(s.rows, s.hidden);
@@ -519,9 +529,9 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
   w.dgu = take(backward ? s.rows * 2 * pad * (w.exact ? 4 : es) : 0);
   const int64_t kept_rows = w.keep ? ceil_div64(s.rows, gated_slopes_rows(s)) : 0;
   w.bias = take(backward ? (kept_rows > w.bias_rows ? kept_rows : w.bias_rows) * 2 * s.hidden * 4 : 0);
-  w.dx_parts = take(!backward ? 0 : w.dx > 64 ? cuts(w.dx, s.rows, s.dim, 2 * pad) : w.n_dx > 1 ? w.n_dx * s.rows * s.dim * 4 : 0);
+  w.dx_parts = take(!backward ? 0 : w.dx > 64 ? w.r_dx.bytes(w.dx) : w.n_dx > 1 ? w.n_dx * s.rows * s.dim * 4 : 0);
   w.dw_parts = take(!backward  ? 0
-                    : w.dw > 64 ? cuts(w.dw, 2 * pad, s.dim, s.rows)
+                    : w.dw > 64 ? w.r_dw.bytes(w.dw)
                     : w.n_dw > 1 ? w.n_dw * 2 * s.hidden * s.dim * 4
                                  : 0);
   w.total = at;
@@ -574,7 +584,7 @@ static void gated_fwd(const T* x, int64_t x_stride, const T* wg, const T* wu, co
     T* const pads = kept && w.keep_pads ? (T*)((char*)kept + w.kept_pads) : nullptr;
     GatedWide a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, true, true, ws, pads, false, st);
     a.h = h, a.kept = w.keep ? kept : nullptr, a.cuts = (float*)(ws + w.cuts);
-    gated_wide(type, kWideFwd, w.fwd, a, st);
+    gated_wide(type, kWideFwd, w.fwd, a, w.r_fwd, st);
     return;
   }
   const dim3 grid((unsigned)ceil_div64(s.rows, 64), (unsigned)ceil_div64(s.hidden, 64));
@@ -608,18 +618,22 @@ static void gated_bwd_as(const T* x, int64_t x_stride, const T* wg, const T* wu,
     gated_skinny(type, GatedSkinny{s, x, wg, wu, bg, bu, dh, x_stride, dh_stride, nullptr, dgu, bias, act, w.exact}, st);
   } else if (w.fwd > 64) {
     a.parts = bias;
-    gated_wide(type, kWideGrad, w.fwd, a, st);
+    gated_wide(type, kWideGrad, w.fwd, a, w.r_fwd, st);
   } else {
     k_tile_gated<T, G><<<dim3((unsigned)rb, (unsigned)(pad / 64)), 256, 0, st>>>(x, x_stride, wg, wu, bg, bu, act, s, nullptr, dh,
                                                                             dh_stride, dgu, bias);
   }
   if (bias) gated_join<T>(bias, w.bias_rows, 2 * s.hidden, s.hidden, dbg, dbu, st);
+  if (dx && weights && w.beside) {
+    gated_wide_back(type, a, w.r_dx, (float*)(ws + w.dx_parts), w.r_dw, (float*)(ws + w.dw_parts), st);
+    return;
+  }
   if (dx) {
     const int64_t n = w.n_dx, share = ceil_div64(ceil_div64(2 * pad, n), 64) * 64;
     float* parts = n > 1 ? (float*)(ws + w.dx_parts) : nullptr;
     if (w.dx > 64) {
       a.cuts = (float*)(ws + w.dx_parts);
-      gated_wide(type, kWideDx, w.dx, a, st);
+      gated_wide(type, kWideDx, w.dx, a, w.r_dx, st);
     } else {
       k_tile_dx<T, G><<<dim3((unsigned)rb, (unsigned)db, (unsigned)n), 256, 0, st>>>(dgu, wg, wu, s, share, dx, parts);
     }
@@ -630,7 +644,7 @@ static void gated_bwd_as(const T* x, int64_t x_stride, const T* wg, const T* wu,
     float* parts = n > 1 ? (float*)(ws + w.dw_parts) : nullptr;
     if (w.dw > 64) {
       a.cuts = (float*)(ws + w.dw_parts);
-      gated_wide(type, kWideDw, w.dw, a, st);
+      gated_wide(type, kWideDw, w.dw, a, w.r_dw, st);
     } else {
       k_tile_dw<T, G><<<dim3((unsigned)(2 * pad / 64), (unsigned)db, (unsigned)n), 256, 0, st>>>(dgu, x, x_stride, s, share, dwg,
                                                                                               dwu, parts);

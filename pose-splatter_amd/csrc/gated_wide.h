@@ -27,11 +27,15 @@ struct WideRounds {
   int64_t bytes(int side) const { return cut ? (int64_t)cut * shares * side * side * 4 : 0; }
 };
 WideRounds gated_wide_rounds(int type, int side, int64_t mt, int64_t nt, int64_t steps);
+bool gated_wide_back_rounds(int type, const int64_t (&tiles)[2], const int64_t (&steps)[2], WideRounds (&r)[2]);
 
 // Steps of 128 bytes of K.
 inline int64_t gated_wide_steps(int type, int64_t k) { return ceil_div64(k * (int64_t)type_size(type), 128); }
 
 // side 128, or 256 in 16 bits
-void gated_wide(int type, int mode, int side, GatedWide a, hipStream_t st);
+void gated_wide(int type, int mode, int side, GatedWide a, const WideRounds& r, hipStream_t st);
+
+// dx and the weight gradients in one launch (side 128).
+void gated_wide_back(int type, GatedWide a, const WideRounds& rx, float* x_cuts, const WideRounds& rw, float* w_cuts, hipStream_t st);
 
 }  // namespace gsr

@@ -35,17 +35,17 @@ struct Count {
   static constexpr int value = N;
 };
 
+// Workgroup `id` of a product; lds: kWideSlots operand tiles.
 template <typename T, int MODE, int SIDE>
-__global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(GatedWide a) {
+__device__ __forceinline__ void wide_product(const GatedWide& a, int id, char (*lds)[SIDE * 128]) {
   constexpr bool DUAL = MODE == kWideFwd || MODE == kWideGrad, AKC = MODE != kWideDw, BKC = DUAL;
   constexpr int NB = SIDE / 64, HALF = SIDE / 2, BYTES = SIDE * 128;   // blocks a wave and side; its rows
   constexpr int ES = sizeof(T), K = kWideK<T>;
-  __shared__ __attribute__((aligned(1024))) char lds[kWideSlots][BYTES];
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wm = wave % 2, wn = wave / 2;
   const GatedShape s = a.s;
   const int64_t pad = gated_pad(s.hidden);
   // Whole tiles first; those that would leave CUs idle in the last round are cut into shares of K.
-  int tm, tn, id = blockIdx.x, share = -1;
+  int tm, tn, share = -1;
   if constexpr (MODE != kWideGrad) {
     if (id >= a.whole) {
       share = (id - a.whole) / a.cut;
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
   wide_wait<0>();   // (the loads past K's end write zeros)
   __syncthreads();
   constexpr int LD = HALF + 4;   // floats a row: a wave's columns and 4 to spread the banks
-  static_assert(4 * 32 * LD * sizeof(float) <= sizeof(lds), "the waves' rows fit the tiles' memory");
+  static_assert(4 * 32 * LD * sizeof(float) <= kWideSlots * BYTES, "the waves' rows fit the tiles' memory");
   float* mine = (float*)&lds[0][0] + wave * 32 * LD;
   constexpr int COLS = DUAL ? HALF / 2 : HALF, LANES = COLS / 8, ROWS = 64 / LANES;   // lanes a row, rows a pass
   const int c = lane % LANES * 8;
@@ -317,11 +317,29 @@ __global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(Gate
   }
 }
 
+template <typename T, int MODE, int SIDE>
+__global__ __launch_bounds__(kWideThreads, SIDE == 256 ? 1 : 2) void k_wide(GatedWide a) {
+  __shared__ __attribute__((aligned(1024))) char lds[kWideSlots][SIDE * 128];
+  wide_product<T, MODE, SIDE>(a, blockIdx.x, lds);
+}
+
+// dx by the first `split` workgroups and the weight gradients by the others, side by side: neither alone fills
+// the card to its end.
+template <typename T>
+__global__ __launch_bounds__(kWideThreads, 2) void k_wide_back(GatedWide x, GatedWide w, int split) {
+  __shared__ __attribute__((aligned(1024))) char lds[kWideSlots][128 * 128];
+  if ((int)blockIdx.x < split) {
+    wide_product<T, kWideDx, 128>(x, blockIdx.x, lds);
+  } else {
+    wide_product<T, kWideDw, 128>(w, blockIdx.x - split, lds);
+  }
+}
+
 // The cut tiles' results: the sums of their shares, in order.
 template <typename T, int MODE, int SIDE>
-__global__ __launch_bounds__(256) void k_wide_join(GatedWide a) {
+__device__ __forceinline__ void wide_join(const GatedWide& a, int block) {
   constexpr int EACH = SIDE * SIDE / 8 / 256;   // workgroups a tile
-  const int tile = blockIdx.x / EACH, at = (blockIdx.x % EACH * 256 + threadIdx.x) * 8;
+  const int tile = block / EACH, at = (block % EACH * 256 + threadIdx.x) * 8;
   int tm, tn;
   wide_tile_of(a.whole + tile, a.mt, a.nt, &tm, &tn);
   const float* p = a.cuts + (int64_t)tile * SIDE * SIDE + at;
@@ -335,6 +353,18 @@ __global__ __launch_bounds__(256) void k_wide_join(GatedWide a) {
     for (int j = 0; j < 8; ++j) v[j] += w[j];
   }
   wide_store<T, MODE>(a, (int64_t)tm * SIDE + at / SIDE, (int64_t)tn * SIDE + at % SIDE, v);
+}
+
+template <typename T, int MODE, int SIDE>
+__global__ __launch_bounds__(256) void k_wide_join(GatedWide a) { wide_join<T, MODE, SIDE>(a, blockIdx.x); }
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_wide_join_back(GatedWide x, GatedWide w, int split) {
+  if ((int)blockIdx.x < split) {
+    wide_join<T, kWideDx, 128>(x, blockIdx.x);
+  } else {
+    wide_join<T, kWideDw, 128>(w, blockIdx.x - split);
+  }
 }
 
 // The forward's: both projections' sums, and from them the outputs.
@@ -412,12 +442,52 @@ WideRounds gated_wide_rounds(int type, int side, int64_t mt, int64_t nt, int64_t
   return shares > 1 ? WideRounds{(int)(tiles - cut), (int)cut, (int)shares} : WideRounds{(int)tiles, 0, 1};
 }
 
-void gated_wide(int type, int mode, int side, GatedWide a, hipStream_t st) {
-  const int64_t pad = gated_pad(a.s.hidden);
-  a.mt = ceil_div(mode == kWideDw ? 2 * pad : a.s.rows, side);
-  a.nt = mode <= kWideGrad ? ceil_div(pad, side / 2) : ceil_div(a.s.dim, side);
-  const WideRounds r = gated_wide_rounds(type, side, a.mt, a.nt, gated_wide_steps(type, mode == kWideFwd ? a.kdim : mode == kWideDw ? a.s.rows : 2 * pad));
-  a.whole = r.whole, a.cut = r.cut, a.shares = r.shares;
+// The same for dx and dW side by side (128), where all their workgroups run at once (else false).  Shares of one
+// length in both, a little more than makes 512 of them, by the same model: of two workgroups a CU, the
+// longer kind paired with the shorter where there are at most 256 of it.  Backward passes, side
+// by side against one after the other: fp32 16000 x 256 -> 512 161 us against 173, 500 x 1000 -> 1000
+// 53 against 62; bf16 777 x 509 -> 1363 23 against 32, 4096 x 256 -> 4096 89 against 96.
+bool gated_wide_back_rounds(int type, const int64_t (&tiles)[2], const int64_t (&steps)[2], WideRounds (&r)[2]) {
+  const bool f32 = type == GSR_F32;
+  const double open = f32 ? 2. : 4., part = f32 ? .015 : .06, join = f32 ? 1.5 : 6.;
+  const double all = (double)(tiles[0] * steps[0] + tiles[1] * steps[1]);
+  const int64_t least = f32 ? 2 : 8;
+  double best = 0.;
+  for (int j = 0; j < 16; ++j) {
+    const double length = all / 512 * (1. + j / 16.);
+    int64_t n[2], count[2];
+    double unit[2], cost = 0.;
+    for (int i = 0; i < 2; ++i) {
+      n[i] = (int64_t)(steps[i] / length) + 1;
+      const int64_t most = steps[i] / least < 64 ? steps[i] / least : 64;
+      n[i] = n[i] < most ? n[i] : most < 1 ? 1 : most;
+      count[i] = tiles[i] * n[i];
+      unit[i] = (double)steps[i] / n[i] + open;
+      if (n[i] > 1) cost += part * count[i];
+    }
+    if (n[0] > 1 || n[1] > 1) cost += join;
+    const int64_t total = count[0] + count[1];
+    if (total > 512) continue;
+    const int big = unit[1] > unit[0];
+    cost += total <= 256 ? 1.1 * unit[big] : count[big] <= 256 ? unit[big] + unit[!big] : 2 * unit[big];
+    if (best == 0. || cost < best) {
+      best = cost;
+      for (int k = 0; k < 2; ++k) r[k] = n[k] > 1 ? WideRounds{0, (int)tiles[k], (int)n[k]} : WideRounds{(int)tiles[k], 0, 1};
+    }
+  }
+  return best > 0.;
+}
+
+static void wide_tiles(int mode, int side, const WideRounds& r, GatedWide* a) {
+  const int64_t pad = gated_pad(a->s.hidden);
+  a->mt = ceil_div(mode == kWideDw ? 2 * pad : a->s.rows, side);
+  a->nt = mode <= kWideGrad ? ceil_div(pad, side / 2) : ceil_div(a->s.dim, side);
+  a->whole = r.whole, a->cut = r.cut, a->shares = r.shares;
+}
+
+void gated_wide(int type, int mode, int side, GatedWide a, const WideRounds& r, hipStream_t st) {
+  wide_tiles(mode, side, r, &a);
+  if (mode == kWideGrad) a.whole = a.mt * a.nt, a.cut = 0;
   if (type == GSR_F32) {
     wide_launch<float, 128>(mode, a, st);
   } else if (type == GSR_BF16 && side == 256) {
@@ -428,6 +498,27 @@ void gated_wide(int type, int mode, int side, GatedWide a, hipStream_t st) {
     wide_launch<f16, 256>(mode, a, st);
   } else {
     wide_launch<f16, 128>(mode, a, st);
+  }
+}
+
+template <typename T>
+static void wide_back_launch(const GatedWide& x, const GatedWide& w, hipStream_t st) {
+  const int nx = x.whole + x.cut * x.shares, nw = w.whole + w.cut * w.shares, jx = x.cut * (128 * 128 / 8 / 256), jw = w.cut * (128 * 128 / 8 / 256);
+  k_wide_back<T><<<nx + nw, kWideThreads, 0, st>>>(x, w, nx);
+  if (jx + jw) k_wide_join_back<T><<<jx + jw, 256, 0, st>>>(x, w, jx);
+}
+
+void gated_wide_back(int type, GatedWide a, const WideRounds& rx, float* x_cuts, const WideRounds& rw, float* w_cuts, hipStream_t st) {
+  GatedWide x = a, w = a;
+  wide_tiles(kWideDx, 128, rx, &x);
+  wide_tiles(kWideDw, 128, rw, &w);
+  x.cuts = x_cuts, w.cuts = w_cuts;
+  if (type == GSR_F32) {
+    wide_back_launch<float>(x, w, st);
+  } else if (type == GSR_BF16) {
+    wide_back_launch<bf16>(x, w, st);
+  } else {
+    wide_back_launch<f16>(x, w, st);
   }
 }
 
