@@ -7,8 +7,9 @@
 //   dWg, dWu            rows are the columns of [dg | du], K the rows of x
 //
 // 16384 x 2048 -> 5632 bf16: forward 650 us (1160 TFLOP/s, writing its kept projections as well), dx
-// 545 (1390), dW 595 (1270); 16000 x 256 -> 512 fp32 79, 72 and 73 us (106 to 116 of the card's 153
-// TFLOP/s in fp32: one or two rounds of tiles, whose first loads and last stores nothing hides).
+// 545 (1390), dW 595 (1270); 16000 x 256 -> 512 fp32 79, and dx and dW side by side 133 us (106 and 126
+// of the card's 153 TFLOP/s in fp32: one or two rounds of tiles, whose first loads and last stores
+// nothing hides).
 #include "gated_wide.h"
 
 #include "wide.h"
