@@ -122,6 +122,16 @@ struct Kept {
       *(uint4*)(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
     }
   }
+  __device__ __forceinline__ void store_one(int64_t at, float g, float v) const {
+    if constexpr (sizeof(T) == 4) {
+      ((float*)hi)[at] = g;
+      u[at] = v;
+    } else {
+      const uint32_t a = __float_as_uint(g), b = __float_as_uint(v);
+      hi[at] = a >> 16 | (b & 0xFFFF0000u);
+      lo[at] = (uint16_t)((a >> 8 & 0xFFu) | (b & 0xFF00u));
+    }
+  }
   __device__ __forceinline__ void load(int64_t at, float (&g)[8], float (&v)[8]) const {
     if constexpr (sizeof(T) == 4) {
       load_vec((const float*)hi + at, g);

@@ -420,9 +420,10 @@ __global__ __launch_bounds__(256) void k_gated_pad(GatedPads<T> a) {
 // x 1024 -> 2816 128 against 197, 16000 x 128 -> 256 105 against 126; 200 x 100 -> 1000 59 against 43,
 // 2000 x 128 -> 128 52 against 48; dx of 16 x 2048 -> 4096 bf16 19 us against 25, of 40 x 1024 ->
 // 2816 14.5 against 14.0.
+static bool gated_pads_few(int type, GatedShape s);
 static int gated_side(int type, int64_t rows, int64_t cols, int64_t k, GatedShape s) {
   const bool few = s.rows <= kSkinnyRows;
-  if (s.dim < 64 || (few && s.dim % 8)) return 64;
+  if (s.dim < 64 || (few && s.dim % 8 && !gated_pads_few(type, s))) return 64;
   const int64_t steps = gated_wide_steps(type, k);
   if (type == GSR_F32 && cols <= 64) return 64;
   if (type == GSR_F32 || few) return ceil_div64(rows, 128) * ceil_div64(cols, 128) * steps >= 512 ? 128 : 64;
@@ -443,6 +444,13 @@ static bool gated_aligned(const T* p, int64_t dim, int64_t stride) {
 // 1487, 4096 x 256 -> 2816 55 against 62, x 128 50 against 54 and not worth its memory; fp32 4096 x
 // 128 -> 2816 111 against 146.
 static bool gated_keeps(int type, int64_t dim) { return dim >= (type == GSR_F32 ? 128 : 256); }
+
+// Whether few rows' operands are copied to whole 16-byte pieces: 16-bit weights of odd rows, which the kernel for few
+// rows would read at 0.8 TB/s, large enough for the copy's launch to pay (60 x 2699 -> 5750 bf16,
+// forward and backward: 98 us against 266).
+static bool gated_pads_few(int type, GatedShape s) {
+  return s.rows <= kSkinnyRows && type != GSR_F32 && s.dim % 8 && s.hidden * s.dim >= 1 << 21;
+}
 
 // Whether a 16-bit block's backward keeps the projections' gradients in fp32 and multiplies them so: where
 // products are short (in 64 x 64 tiles 2^24 products, a few us at the fp32 rate) or dx has few
@@ -514,15 +522,16 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
     if (w.dw > 64) w.r_dw = gated_wide_rounds(type, w.dw, ceil_div64(2 * pad, w.dw), ceil_div64(s.dim, w.dw), w_steps);
   }
   if (s.rows <= kSkinnyRows) w.fwd = 64;   // (the kernel for few rows)
-  const bool xw = w.fwd > 64 || (backward && w.dw > 64), ww = w.fwd > 64 || (backward && w.dx > 64);
+  const bool pads = w.fwd > 64 || gated_pads_few(type, s);
+  const bool xw = pads || (backward && w.dw > 64), ww = pads || (backward && w.dx > 64);
   w.x = take(xw ? s.rows * w.kdim * es : 0);
   w.wg = take(ww ? s.hidden * w.kdim * es : 0);
   w.wu = take(ww ? s.hidden * w.kdim * es : 0);
   if (w.fwd > 64)
     w.r_fwd = gated_wide_rounds(type, w.fwd, ceil_div64(s.rows, w.fwd), ceil_div64(pad, w.fwd / 2), gated_wide_steps(type, s.dim));
   w.cuts = take(w.fwd > 64 && !backward ? w.r_fwd.bytes(w.fwd) : 0);
-  w.keep = w.fwd > 64 && gated_keeps(type, s.dim);
-  w.keep_pads = w.fwd > 64 && w.kdim != s.dim && (w.dx > 64 || w.dw > 64 || !w.keep);
+  w.keep = (w.fwd > 64 || s.rows <= kSkinnyRows) && gated_keeps(type, s.dim);
+  w.keep_pads = pads && w.kdim != s.dim && (w.dx > 64 || w.dw > 64 || !w.keep);
   w.kept_pads = !w.keep ? 0 : type == GSR_F32 ? Kept<float>::bytes(s.rows, s.hidden) : Kept<bf16>::bytes(s.rows, s.hidden);
   w.kept = w.kept_pads + (w.keep_pads ? (s.rows + 2 * s.hidden) * w.kdim * es : 0);
   w.bias_rows = s.rows <= kSkinnyRows ? 1 : w.fwd > 64 ? ceil_div64(s.rows, w.fwd) * 2 : rb;
@@ -575,13 +584,20 @@ template <typename T>
 static void gated_fwd(const T* x, int64_t x_stride, const T* wg, const T* wu, const T* bg, const T* bu, int act, GatedShape s,
                       T* h, void* kept, char* ws, hipStream_t st) {
   const int type = type_of<T>();
+  const GatedPlan w = gated_plan(s, type, false);
+  T* const pads = kept && w.keep_pads ? (T*)((char*)kept + w.kept_pads) : nullptr;
   if (s.rows <= kSkinnyRows) {
-    gated_skinny(type, GatedSkinny{s, x, wg, wu, bg, bu, nullptr, x_stride, 0, h, nullptr, nullptr, act, false}, st);
+    GatedSkinny f{s, x, wg, wu, bg, bu, nullptr, x_stride, 0, h, nullptr, nullptr, act, false, w.keep ? kept : nullptr};
+    // (up to 16 rows the copy pays with a backward to follow: 1 x 4095 -> 11264 bf16 forward alone 77 us without it, 122
+    // with; with the backward 495 and 238)
+    if (gated_pads_few(type, s) && (pads || s.rows > 16)) {
+      const GatedWide a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, true, true, ws, pads, false, st);
+      f.s.dim = w.kdim, f.x = a.x, f.x_stride = a.x_stride, f.wg = a.wg, f.wu = a.wu;
+    }
+    gated_skinny(type, f, st);
     return;
   }
-  const GatedPlan w = gated_plan(s, type, false);
   if (w.fwd > 64) {
-    T* const pads = kept && w.keep_pads ? (T*)((char*)kept + w.kept_pads) : nullptr;
     GatedWide a = gated_wide_args<T>(x, x_stride, wg, wu, bg, bu, act, s, w, true, true, ws, pads, false, st);
     a.h = h, a.kept = w.keep ? kept : nullptr, a.cuts = (float*)(ws + w.cuts);
     gated_wide(type, kWideFwd, w.fwd, a, w.r_fwd, st);

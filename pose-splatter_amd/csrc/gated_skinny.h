@@ -15,6 +15,7 @@ struct GatedSkinny {
   float* parts;    // gradients: column sums [2][hidden], or NULL
   int act;
   bool dgu32;      // dgu is written in fp32
+  void* kept;      // forward: NULL, or what it keeps of the projections (Kept)
 };
 
 void gated_skinny(int type, const GatedSkinny& a, hipStream_t st);

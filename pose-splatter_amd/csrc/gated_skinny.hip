@@ -122,7 +122,10 @@ __global__ __launch_bounds__(WAVES * 64) void k_skinny(GatedSkinny a) {
     float act[1], slope[1];
     activate<T>(a.act, one, act, slope);
     if constexpr (!GRAD) {
-      if (in) ((T*)a.h)[row * s.hidden + n] = from_f<T>(act[0] * uv);
+      if (in) {
+        if (a.kept) Kept<T>(a.kept, s.rows, s.hidden).store_one(row * pad + n, gv, uv);
+        ((T*)a.h)[row * s.hidden + n] = from_f<T>(act[0] * uv);
+      }
     } else {
       const float d = in ? to_f(((const T*)a.dh)[row * a.dh_stride + n]) : 0.f;
       gv = in ? d * uv * slope[0] : 0.f;   // (the padding holds zeros)

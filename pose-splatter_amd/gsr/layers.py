@@ -58,7 +58,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     w.r.t. every tensor.  For its backward a forward keeps x and the weights, from dim 256 on (128
     in fp32, where a case is not small) both projections, 6 bytes an element of [rows, hidden] (8
     in fp32), and where dim is not a multiple of 8 (4) a copy of x and the weights that is; below
-    that, and for up to 64 rows, the backward computes the projections again."""
+    that the backward computes the projections again."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"gated_linear: activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")

@@ -399,6 +399,23 @@ def test_few_tiles(cuda, rows, dim, hidden, kind):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows,dim,hidden", [(60, 2699, 800), (5, 2501, 900), (17, 2050, 1027), (64, 300, 7001), (1, 4095, 601)])
+def test_few_odd_rows(cuda, rows, dim, hidden, kind):
+    """Up to 64 rows of odd length: with a backward to follow (kept projections and copies) and without."""
+    from gsr.layers import gated_linear
+    bias = rows % 2 == 1
+    act = ("silu", "gelu", "sigmoid")[rows % 3]
+    args, dh = _case(rows, dim, hidden, kind, bias, rows + dim)
+    want, tol = _reference(*args, dh, act, TYPES[kind])
+    for name, got, v, t in zip(NAMES, _run(cuda, args, dh, act), want, tol):
+        _check(got, v, t, f"{name} {rows}x{dim}->{hidden} {kind} {act}")
+    with torch.no_grad():
+        h = gated_linear(*(None if a is None else a.to(cuda) for a in args), activation=act)
+    _check(h, want[0], tol[0], f"h alone {rows}x{dim}->{hidden} {kind} {act}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("rows,dim,hidden", [(300, 301, 300), (777, 509, 200), (200, 264, 136), (4200, 129, 1000)])
 def test_without_what_the_forward_keeps(cuda, rows, dim, hidden, kind):
     """The C ABI's backward where the caller kept nothing: everything is made again."""
