@@ -261,20 +261,12 @@ def _adamw(s, t):
     return p, m, v if s["case"]["bits"] == 32 else root
 
 
-_modules = None
-
-
 def _own():
-    """The framework's modules, imported by the first call (as a user's program imports them once)."""
-    global _modules
-    if _modules is not None:
-        return _modules
     package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pose-splatter_amd")
     if package not in sys.path:
         sys.path.insert(0, package)
     from gsr import layers, optim
-    _modules = layers, optim
-    return _modules
+    return layers, optim
 
 
 def run(state):
