@@ -32,6 +32,11 @@ def _units(numel: int) -> int:
     return -(-numel // _BLOCK)
 
 
+def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one shape order their elements in memory alike."""
+    return a.numel() == 0 or all(n == 1 or x == y for n, x, y in zip(a.shape, a.stride(), b.stride()))
+
+
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 1e-2, step, exp_avg_units=None, exp_avg_root_units=None) -> None:
     """One AdamW step over lists of tensors, in place:
@@ -145,11 +150,18 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict: dict) -> None:
         """As torch's, but the moments keep their own types (torch would cast them to the
-        parameters')."""
+        parameters').  8-bit moments are taken only by a parameter of their own memory order (their
+        units belong to runs of 256 elements in that order); 32-bit ones follow the parameter's."""
         for mine, saved in zip(self.param_groups, state_dict["param_groups"]):
             if saved.get("moment_bits", 32) != mine["moment_bits"]:
                 raise ValueError(f"AdamW: the checkpoint's moments have {saved.get('moment_bits', 32)} bits, "
                                  f"this optimizer's {mine['moment_bits']}")
+            for p, key in zip(mine["params"], saved["params"]):
+                s = state_dict["state"].get(key)
+                if s and mine["moment_bits"] == 8 and not all(_same_order(s[k], p) for k in ("exp_avg", "exp_avg_sq")):
+                    raise ValueError(f"AdamW: the checkpoint's 8-bit moments of parameter {key} have strides "
+                                     f"{s['exp_avg'].stride()}, another memory order than the parameter's {p.stride()}: load "
+                                     "them into a parameter of their order")
         super().load_state_dict(state_dict)
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
             for p, key in zip(group["params"], saved["params"]):
