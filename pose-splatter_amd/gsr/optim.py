@@ -158,7 +158,12 @@ class AdamW(torch.optim.Optimizer):
                                  f"this optimizer's {mine['moment_bits']}")
             for p, key in zip(mine["params"], saved["params"]):
                 s = state_dict["state"].get(key)
-                if s and mine["moment_bits"] == 8 and not all(_same_order(s[k], p) for k in ("exp_avg", "exp_avg_sq")):
+                if not s:
+                    continue
+                if any(s[k].shape != p.shape for k in ("exp_avg", "exp_avg_sq")):
+                    raise ValueError(f"AdamW: the checkpoint's moments of parameter {key} have the shape "
+                                     f"{tuple(s['exp_avg'].shape)}, the parameter {tuple(p.shape)}")
+                if mine["moment_bits"] == 8 and not all(_same_order(s[k], p) for k in ("exp_avg", "exp_avg_sq")):
                     raise ValueError(f"AdamW: the checkpoint's 8-bit moments of parameter {key} have strides "
                                      f"{s['exp_avg'].stride()}, another memory order than the parameter's {p.stride()}: load "
                                      "them into a parameter of their order")

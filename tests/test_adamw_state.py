@@ -75,3 +75,15 @@ def test_words_change_their_memory_order():
     opt.load_state_dict(_saved(a, state))
     for name in ("exp_avg", "exp_avg_sq"):
         assert torch.equal(opt.state[b][name], state[name]) and opt.state[b][name].stride() == b.stride()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_of_another_shape(bits):
+    """A state of other shapes is refused: it would be repeated over the parameter."""
+    from gsr.optim import AdamW
+    a, b = torch.nn.Parameter(torch.zeros(1, 300)), torch.nn.Parameter(torch.zeros(7, 300))
+    state = _bytes_state(a) if bits == 8 else {"step": 2, "exp_avg": torch.randn(1, 300), "exp_avg_sq": torch.rand(1, 300)}
+    opt = AdamW([b], moment_bits=bits)
+    with pytest.raises(ValueError, match="shape"):
+        opt.load_state_dict(_saved(a, state, moment_bits=bits))
+    assert not opt.state
