@@ -83,14 +83,17 @@ class AdamW(torch.optim.Optimizer):
     def add_param_group(self, param_group: dict) -> None:
         """As torch's; a group's own values are checked like the defaults."""
         super().add_param_group(param_group)
-        g = self.param_groups[-1]
         try:
-            if g["moment_bits"] not in (8, 32):
-                raise ValueError(f"AdamW: moment_bits must be 8 or 32, got {g['moment_bits']}")
-            adamw_step([], [], [], [], lr=g["lr"], betas=g["betas"], eps=g["eps"], weight_decay=g["weight_decay"], step=1)
+            self._check_group(self.param_groups[-1])
         except (ValueError, TypeError):
             self.param_groups.pop()
             raise
+
+    @staticmethod
+    def _check_group(g: dict) -> None:
+        if g["moment_bits"] not in (8, 32):
+            raise ValueError(f"AdamW: moment_bits must be 8 or 32, got {g['moment_bits']}")
+        adamw_step([], [], [], [], lr=g["lr"], betas=g["betas"], eps=g["eps"], weight_decay=g["weight_decay"], step=1)
 
     def _state(self, p: torch.Tensor, group: dict) -> dict:
         s = self.state[p]
@@ -151,24 +154,18 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict: dict) -> None:
         """As torch's, but the moments keep their own types (torch would cast them to the
         parameters').  8-bit moments are taken only by a parameter of their own memory order (their
-        units belong to runs of 256 elements in that order); 32-bit ones follow the parameter's."""
+        units belong to runs of 256 elements in that order); 32-bit ones follow the parameter's.
+        A torch.optim.AdamW checkpoint is taken too, its moments as float32, unless its update is
+        another one (amsgrad, maximize, decay in the gradient)."""
+        options = [{k: g[k] for k in ("moment_bits", "capturable")} for g in self.param_groups]
         for mine, saved in zip(self.param_groups, state_dict["param_groups"]):
-            if saved.get("moment_bits", 32) != mine["moment_bits"]:
-                raise ValueError(f"AdamW: the checkpoint's moments have {saved.get('moment_bits', 32)} bits, "
-                                 f"this optimizer's {mine['moment_bits']}")
-            for p, key in zip(mine["params"], saved["params"]):
-                s = state_dict["state"].get(key)
-                if not s:
-                    continue
-                if any(s[k].shape != p.shape for k in ("exp_avg", "exp_avg_sq")):
-                    raise ValueError(f"AdamW: the checkpoint's moments of parameter {key} have the shape "
-                                     f"{tuple(s['exp_avg'].shape)}, the parameter {tuple(p.shape)}")
-                if mine["moment_bits"] == 8 and not all(_same_order(s[k], p) for k in ("exp_avg", "exp_avg_sq")):
-                    raise ValueError(f"AdamW: the checkpoint's 8-bit moments of parameter {key} have strides "
-                                     f"{s['exp_avg'].stride()}, another memory order than the parameter's {p.stride()}: load "
-                                     "them into a parameter of their order")
+            self._check_saved(mine, saved, state_dict["state"])
         super().load_state_dict(state_dict)
-        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+        for group, saved, own in zip(self.param_groups, state_dict["param_groups"], options):
+            for k, v in own.items():
+                group.setdefault(k, v)
+            if isinstance(group["lr"], torch.Tensor) and group["params"]:
+                group["lr"] = group["lr"].to(group["params"][0].device, torch.float32)
             for p, key in zip(group["params"], saved["params"]):
                 s = state_dict["state"].get(key)
                 if not s:
@@ -179,9 +176,33 @@ class AdamW(torch.optim.Optimizer):
                         new[name] = (torch.tensor(int(v), dtype=torch.int64, device=p.device) if group["capturable"]
                                      else int(v))
                     elif name in ("exp_avg", "exp_avg_sq"):
+                        v = v.to(p.device, torch.float32 if group["moment_bits"] == 32 else v.dtype)
                         to = torch.empty_strided(p.shape, p.stride(), dtype=v.dtype, device=p.device)
                         raw = torch.uint8 if v.element_size() == 1 else v.dtype
-                        to.view(raw).copy_(v.to(p.device).view(raw))
+                        to.view(raw).copy_(v.view(raw))
                         new[name] = to
                     else:
                         new[name] = v.to(p.device, copy=True)
+
+    def _check_saved(self, mine: dict, saved: dict, state: dict) -> None:
+        if saved.get("moment_bits", 32) != mine["moment_bits"]:
+            raise ValueError(f"AdamW: the checkpoint's moments have {saved.get('moment_bits', 32)} bits, "
+                             f"this optimizer's {mine['moment_bits']}")
+        for option in ("amsgrad", "maximize"):
+            if saved.get(option):
+                raise ValueError(f"AdamW: the checkpoint's steps are taken with {option}=True, which this optimizer has not")
+        if not saved.get("decoupled_weight_decay", True) and saved["weight_decay"] != 0:
+            raise ValueError("AdamW: the checkpoint's weight decay is part of the gradient, this optimizer's is decoupled")
+        lr = saved["lr"]
+        self._check_group({**mine, **saved, "lr": lr.float() if isinstance(lr, torch.Tensor) else lr})
+        for p, key in zip(mine["params"], saved["params"]):
+            s = state.get(key)
+            if not s:
+                continue
+            if any(s[k].shape != p.shape for k in ("exp_avg", "exp_avg_sq")):
+                raise ValueError(f"AdamW: the checkpoint's moments of parameter {key} have the shape "
+                                 f"{tuple(s['exp_avg'].shape)}, the parameter {tuple(p.shape)}")
+            if mine["moment_bits"] == 8 and not all(_same_order(s[k], p) for k in ("exp_avg", "exp_avg_sq")):
+                raise ValueError(f"AdamW: the checkpoint's 8-bit moments of parameter {key} have strides "
+                                 f"{s['exp_avg'].stride()}, another memory order than the parameter's {p.stride()}: load "
+                                 "them into a parameter of their order")

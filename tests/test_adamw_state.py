@@ -87,3 +87,105 @@ def test_moments_of_another_shape(bits):
     with pytest.raises(ValueError, match="shape"):
         opt.load_state_dict(_saved(a, state, moment_bits=bits))
     assert not opt.state
+
+
+def _torch_checkpoint(dtype=torch.float32, cls=torch.optim.AdamW, **kw):
+    g = torch.Generator().manual_seed(4)
+    ps = [torch.nn.Parameter(torch.randn(s, generator=g).to(dtype)) for s in ((5, 7), (9,))]
+    opt = cls(ps, lr=3e-3, betas=(0.8, 0.95), **kw)
+    for _ in range(3):
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=g).to(dtype)
+        opt.step()
+    return ps, opt.state_dict()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_torch_checkpoint_is_taken_whole(dtype, capturable):
+    """torch.optim.AdamW's state: its groups' values, its moments in fp32 whatever their type, its step
+    counts, and the options that it does not know as this optimizer was made with."""
+    from gsr.optim import AdamW
+    ps, saved = _torch_checkpoint(dtype)
+    saved["param_groups"][0]["capturable"] = capturable
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    opt = AdamW(qs)
+    opt.load_state_dict(copy.deepcopy(saved))
+    group = opt.param_groups[0]
+    assert group["moment_bits"] == 32 and group["capturable"] is capturable
+    assert (group["lr"], group["betas"]) == (3e-3, (0.8, 0.95))
+    for i, q in enumerate(qs):
+        s = opt.state[q]
+        assert int(s["step"]) == 3 and (not capturable or s["step"].dtype == torch.int64)
+        for k in ("exp_avg", "exp_avg_sq"):
+            assert s[k].dtype == torch.float32 and torch.equal(s[k], saved["state"][i][k].float())
+        q.grad = torch.ones_like(q)
+    with pytest.raises(RuntimeError, match="CUDA"):   # (the next step gets as far as the device)
+        opt.step()
+    opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(3))]})
+    assert opt.param_groups[1]["moment_bits"] == 32
+
+
+def test_torch_checkpoint_of_another_step():
+    """Groups whose update is another one are refused, and nothing is changed."""
+    from gsr.optim import AdamW
+    for cls, kw, word in ((torch.optim.AdamW, dict(maximize=True), "maximize"), (torch.optim.AdamW, dict(amsgrad=True), "amsgrad"),
+                          (torch.optim.Adam, dict(weight_decay=0.1), "decoupled")):
+        ps, saved = _torch_checkpoint(cls=cls, **kw)
+        opt = AdamW(ps, lr=7e-3)
+        with pytest.raises(ValueError, match=word):
+            opt.load_state_dict(saved)
+        assert not opt.state and opt.param_groups[0]["lr"] == 7e-3
+    ps, saved = _torch_checkpoint(cls=torch.optim.Adam)   # (no decay: the same step)
+    AdamW(ps).load_state_dict(saved)
+    for key, bad in (("lr", -1.0), ("betas", (0.9, 1.0)), ("eps", -1.0)):
+        ps, saved = _torch_checkpoint()
+        saved["param_groups"][0][key] = bad
+        opt = AdamW(ps, lr=7e-3)
+        with pytest.raises(ValueError, match=key):
+            opt.load_state_dict(saved)
+        assert not opt.state and opt.param_groups[0]["lr"] == 7e-3
+
+
+def test_step_size_tensor_of_a_checkpoint():
+    """A step size saved as a tensor comes back as one fp32 value on the parameters' device."""
+    from gsr.optim import AdamW
+    ps, saved = _torch_checkpoint()
+    saved["param_groups"][0]["lr"] = torch.tensor([2e-3], dtype=torch.float64)
+    opt = AdamW(ps)
+    opt.load_state_dict(saved)
+    lr = opt.param_groups[0]["lr"]
+    assert lr.dtype == torch.float32 and lr.device == ps[0].device and float(lr) == float(torch.tensor(2e-3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tensor_lr", [False, True])
+def test_torch_checkpoint_continues(cuda, dtype, tensor_lr):
+    """Steps after the reload against the recursion in 64 bits from the saved state.  A step's parameter is
+    rounded to its type once, half a step of it, and carries fp32's rounding (32 u of |p| and of a
+    step's size): added over four steps."""
+    from gsr.optim import AdamW
+    ps, saved = _torch_checkpoint(dtype)
+    if tensor_lr:
+        saved["param_groups"][0] |= dict(lr=torch.tensor(3e-3), capturable=True)
+    qs = [torch.nn.Parameter(p.detach().to(cuda)) for p in ps]
+    opt = AdamW(qs)
+    opt.load_state_dict(saved)
+    g = torch.Generator().manual_seed(8)
+    want = [p.detach().double() for p in ps]
+    ms, vs = ([saved["state"][i][k].double() for i in range(2)] for k in ("exp_avg", "exp_avg_sq"))
+    off = [torch.zeros(p.shape, dtype=torch.float64) for p in ps]
+    b1, b2, lr, eps, wd = 0.8, 0.95, float(torch.tensor(3e-3)) if tensor_lr else 3e-3, 1e-8, 0.01
+    for step in range(4, 8):
+        for i, q in enumerate(qs):
+            grad = torch.randn(q.shape, generator=g).to(dtype)
+            q.grad = grad.to(cuda)
+            ms[i] = b1 * ms[i] + (1 - b1) * grad.double()
+            vs[i] = b2 * vs[i] + (1 - b2) * grad.double() ** 2
+            delta = lr / (1 - b1 ** step) * ms[i] / ((vs[i] / (1 - b2 ** step)).sqrt() + eps)
+            want[i] = want[i] * (1 - lr * wd) - delta
+            off[i] += torch.finfo(dtype).eps / 2 * want[i].abs() * 1.01 + 32 * 2.0 ** -24 * (want[i].abs() + delta.abs() + lr)
+        opt.step()
+    for q, w, tol in zip(qs, want, off):
+        assert bool(((q.detach().cpu().double() - w).abs() <= tol).all())
