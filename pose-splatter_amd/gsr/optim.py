@@ -158,9 +158,22 @@ class AdamW(torch.optim.Optimizer):
         A torch.optim.AdamW checkpoint is taken too, its moments as float32, unless its update is
         another one (amsgrad, maximize, decay in the gradient)."""
         options = [{k: g[k] for k in ("moment_bits", "capturable")} for g in self.param_groups]
-        for mine, saved in zip(self.param_groups, state_dict["param_groups"]):
-            self._check_saved(mine, saved, state_dict["state"])
-        super().load_state_dict(state_dict)
+        final = {}   # what the caller's own hooks leave of state_dict
+
+        def check(_, sd):
+            for mine, saved in zip(self.param_groups, sd["param_groups"]):
+                self._check_saved(mine, saved, sd["state"])
+            final.update(sd)
+
+        hooks = [self.register_load_state_dict_pre_hook(check),   # after the caller's, the next before
+                 self.register_load_state_dict_post_hook(lambda _: self._take(final, options), prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for h in hooks:
+                h.remove()
+
+    def _take(self, state_dict: dict, options: list) -> None:
         for group, saved, own in zip(self.param_groups, state_dict["param_groups"], options):
             for k, v in own.items():
                 group.setdefault(k, v)

@@ -189,3 +189,24 @@ def test_torch_checkpoint_continues(cuda, dtype, tensor_lr):
         opt.step()
     for q, w, tol in zip(qs, want, off):
         assert bool(((q.detach().cpu().double() - w).abs() <= tol).all())
+
+
+def test_load_hooks_see_what_is_loaded():
+    """A pre-hook's state_dict is the one that is loaded; a post-hook finds the state as it stays."""
+    from gsr.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(300, dtype=torch.bfloat16))
+    saved = _saved(p, {"step": 2, "exp_avg": torch.rand(300), "exp_avg_sq": torch.rand(300)})
+    opt = AdamW([p])
+    seen = {}
+
+    def double(_, sd):
+        sd = copy.deepcopy(sd)
+        sd["state"][0]["exp_avg"] *= 2
+        return sd
+    opt.register_load_state_dict_pre_hook(double)
+    opt.register_load_state_dict_post_hook(lambda o: seen.update(o.state[p]))
+    opt.load_state_dict(saved)
+    assert torch.equal(opt.state[p]["exp_avg"], 2 * saved["state"][0]["exp_avg"])
+    assert seen["exp_avg"].dtype == torch.float32 and seen["exp_avg"] is opt.state[p]["exp_avg"]
+    opt.load_state_dict(saved)   # (once more: the hooks are still the caller's two)
+    assert len(opt._optimizer_load_state_dict_pre_hooks) == len(opt._optimizer_load_state_dict_post_hooks) == 1
