@@ -143,9 +143,14 @@ class AdamW(torch.optim.Optimizer):
                 if group["moment_bits"] == 8:
                     units = dict(exp_avg_units=[s["exp_avg_unit"] for s in states],
                                  exp_avg_root_units=[s["exp_avg_root_unit"] for s in states])
-                adamw_step([p for p, _ in items], [p.grad for p, _ in items], [s["exp_avg"] for s in states],
-                           [s["exp_avg_sq"] for s in states], lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                           weight_decay=group["weight_decay"], step=steps, **units)
+                try:
+                    adamw_step([p for p, _ in items], [p.grad for p, _ in items], [s["exp_avg"] for s in states],
+                               [s["exp_avg_sq"] for s in states], lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                               weight_decay=group["weight_decay"], step=steps, **units)
+                except Exception:
+                    if group["capturable"]:   # (a refused step was none)
+                        torch._foreach_sub_(steps, 1)
+                    raise
                 if not group["capturable"]:
                     for s in states:
                         s["step"] = steps

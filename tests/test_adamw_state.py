@@ -210,3 +210,20 @@ def test_load_hooks_see_what_is_loaded():
     assert seen["exp_avg"].dtype == torch.float32 and seen["exp_avg"] is opt.state[p]["exp_avg"]
     opt.load_state_dict(saved)   # (once more: the hooks are still the caller's two)
     assert len(opt._optimizer_load_state_dict_pre_hooks) == len(opt._optimizer_load_state_dict_post_hooks) == 1
+
+
+@pytest.mark.gpu
+def test_refused_step_is_not_counted(cuda):
+    """A step that is refused (the parameter changed its memory order under its moments) leaves the device's
+    step count, the parameter and the moments as they were."""
+    from gsr.optim import AdamW
+    p = torch.nn.Parameter(torch.randn(6, 5, device=cuda))
+    opt = AdamW([p], capturable=True)
+    p.grad = torch.randn(6, 5, device=cuda)
+    opt.step()
+    p.data = p.data.T.contiguous().T
+    before = [p.detach().clone(), *(v.clone() for v in opt.state[p].values())]
+    with pytest.raises(ValueError, match="strides"):
+        opt.step()
+    after = [p.detach(), *opt.state[p].values()]
+    assert int(opt.state[p]["step"]) == 1 and all(torch.equal(a, b) for a, b in zip(before, after))
