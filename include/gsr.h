@@ -191,7 +191,9 @@ int gsr_version(void);
 /* Revision 14 (round 6): gsr3d_raster_fwd, gsr3d_raster_fwd_lazy, gsr3d_raster_bwd and
  * gsr3d_raster_bwd_loss take box_masks (before the stream): the forward's per-chunk box
  * survivor masks, stats->masks bit 2. */
-#define GSR_ABI_VERSION 15
+/* Revision 15: the layer and optimizer calls.  Revision 16: gsr_adamw_args takes `rounding` in
+ * the place of a reserved field that was 0. */
+#define GSR_ABI_VERSION 16
 int gsr_abi_version(void);
 const char* gsr_last_error(void);
 
@@ -728,12 +730,17 @@ int gsr_gated_bwd(const void* x, int64_t rows, int64_t dim, int64_t x_stride, in
  * bits 32: m, v are fp32 [n].  bits 8: m holds e4m3 codes and v codes of sqrt(v), n bytes each,
  * in blocks of GSR_ADAMW_BLOCK elements with one fp32 unit a block (m_unit, v_unit
  * [ceil(n / GSR_ADAMW_BLOCK)]); zeroed codes and units are zero moments.  A code c of sqrt(v)
- * stands for c units below 16, else for (16 + c % 16) * 2^(c / 16 - 1).  A gradient that is not
+ * stands for c units below 16, else for (16 + c % 16) * 2^(c / 16 - 1).  rounding, of 8-bit moments:
+ * GSR_ROUND_NEAREST (ties to even; changes below half a code step are lost in every step), or
+ * GSR_ROUND_UNBIASED: up or down by a hash of the element's place in its tensor and the step count, so that the
+ * expected m and v (but for roots below one unit, which are held as one) are the unrounded ones.  A gradient that is not
  * finite makes its element's moments NaN or infinite, in 8 bits its whole block's.
  * A tensor's step count (>= 1) and lr are read from the device where its `step` / lr_dev is not
  * NULL (a captured step), else taken from the host values.  The tensors must not overlap.  gsr_adamw_decode_root
  * writes the n roots sqrt(v) that codes stand for. */
 #define GSR_ADAMW_BLOCK 256
+#define GSR_ROUND_NEAREST 0
+#define GSR_ROUND_UNBIASED 1
 typedef struct {
   void* p;
   const void* g;
@@ -748,7 +755,7 @@ typedef struct {
   double lr, beta1, beta2, eps, weight_decay;
   int64_t step;
   const float* lr_dev;
-  int32_t bits, reserved;
+  int32_t bits, rounding;
 } gsr_adamw_args;
 int gsr_adamw_step(const gsr_adamw_tensor* tensors, int32_t count, int32_t ptype, int32_t gtype,
                    const gsr_adamw_args* args, void* stream);

@@ -302,7 +302,7 @@ class Tensors {
 
 void adamw_step(py::handle param_list, py::handle grad_list, py::handle m_list, py::handle v_list, double lr,
                 const std::optional<Tensor>& lr_dev, double beta1, double beta2, double eps, double weight_decay, int64_t step,
-                py::handle step_list, py::handle m_unit_list, py::handle v_unit_list) {
+                py::handle step_list, py::handle m_unit_list, py::handle v_unit_list, bool unbiased) {
   const Tensors params(param_list, "adamw_step: params must be a list of tensors"),
       grads(grad_list, "adamw_step: grads must be a list of tensors"), ms(m_list, "adamw_step: exp_avgs must be a list of tensors"),
       vs(v_list, "adamw_step: exp_avg_sqs must be a list of tensors");
@@ -401,6 +401,7 @@ void adamw_step(py::handle param_list, py::handle grad_list, py::handle m_list, 
   args.step = steps ? 0 : step;
   args.lr_dev = lr_dev ? lr_dev->data_ptr<float>() : nullptr;
   args.bits = byte ? 8 : 32;
+  args.rounding = unbiased ? GSR_ROUND_UNBIASED : GSR_ROUND_NEAREST;
   const c10::OptionalDeviceGuard guard(device);
   void* stream = stream_of(device);
   for (const Group& g : groups)

@@ -30,7 +30,7 @@ INPUT_GSPLAT = 1
 F32, BF16, F16 = 0, 1, 2
 ADAMW_BLOCK = 256   # GSR_ADAMW_BLOCK: elements that share a unit of an 8-bit moment
 
-ABI_VERSION = 15   # include/gsr.h GSR_ABI_VERSION this binding is written for
+ABI_VERSION = 16   # include/gsr.h GSR_ABI_VERSION this binding is written for
 # gsr_set_bwd2d_parts at load (profiles/r05_ab5_bwd2d_parts_sweep.txt; GSR_BWD2D_PART_WGS overrides it
 # for measurements, tools/parts_sweep.sh)
 BWD2D_PART_WORKGROUPS = int(os.environ.get("GSR_BWD2D_PART_WGS", "4608"))
@@ -90,7 +90,7 @@ class AdamwArgs(ctypes.Structure):
     """gsr_adamw_args (include/gsr.h)."""
     _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
                 ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double), ("step", ctypes.c_int64),
-                ("lr_dev", ctypes.c_void_p), ("bits", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+                ("lr_dev", ctypes.c_void_p), ("bits", ctypes.c_int32), ("rounding", ctypes.c_int32)]
 
 
 _P = ctypes.c_void_p

@@ -10,10 +10,12 @@ moments of 2 M Gaussian rows are twice the scene itself.
 ``adamw_step`` is the step alone, on lists of tensors.  8-bit moments: blocks of 256 elements
 (in memory order) with one fp32 unit each; the first moment as float8_e4m3fn codes, the second
 as uint8 codes of its root (16 steps a doubling, so that eight bits span the range that the step
-needs: the step divides by the root, not by the moment).  Both round to nearest.  The step
-itself uses the new moments before they are rounded.  What rounding costs: a root's code moves
-once its value has changed by 1/32 relative to its block's largest, so slow changes inside a
-block are followed in steps.  No CPU path: the functions raise on CPU tensors.
+needs: the step divides by the root, not by the moment).  The step itself uses the new moments
+before they are rounded.  ``AdamW`` rounds them up or down without bias, so that over many steps
+they follow the moments that are not rounded; one step's rounding is off by less than a code's
+step (1/8 of a mean, 1/16 of a root, or a unit).  Rounded to nearest, a change of less than half
+a code's step is lost in every step: at beta2 = 0.999 a root would stay where it first was.  No
+CPU path: the functions raise on CPU tensors.
 """
 from __future__ import annotations
 
@@ -38,7 +40,8 @@ def _same_order(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
-               weight_decay: float = 1e-2, step, exp_avg_units=None, exp_avg_root_units=None) -> None:
+               weight_decay: float = 1e-2, step, exp_avg_units=None, exp_avg_root_units=None,
+               moment_rounding: str = "nearest") -> None:
     """One AdamW step over lists of tensors, in place:
 
         m = b1 m + (1 - b1) g;   v = b2 v + (1 - b2) g^2
@@ -49,15 +52,22 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, lr=1e-3, betas=(0.9, 0.9
     exp_avgs and exp_avg_sqs are float32, with the parameters' shapes and strides.  8-bit moments
     (when the units are given): exp_avgs are float8_e4m3fn codes, exp_avg_sqs uint8 codes of
     sqrt(v) (``decode_root``), exp_avg_units and exp_avg_root_units float32 [ceil(numel / 256)];
-    zeros are zero moments.  lr: a number or one float32 value on the device.  step: the count of
+    zeros are zero moments.  moment_rounding, of 8-bit moments: "nearest" (ties to even; a change of
+    less than half a code's step is lost, so this is for single steps and conversions), or
+    "unbiased": up with the probability that keeps the expected m and v, drawn by a hash of the element's
+    place in its tensor and the step count (the same bits every run, in any list).  A root below
+    one unit (1/507904 of its block's largest) is held as one in both.  lr: a number or one float32 value on the device.  step: the count of
     this step, 1 at first: a number, one int64 value on the device for all tensors, or a list of
     such values; the device forms are read by the kernel (a step captured in a HIP graph)."""
     lr_dev = lr if isinstance(lr, torch.Tensor) else None
     if isinstance(step, torch.Tensor):
         step = [step] * len(params)
     steps = step if isinstance(step, (list, tuple)) else None
+    if moment_rounding not in ("nearest", "unbiased"):
+        raise ValueError(f'adamw_step: moment_rounding must be "nearest" or "unbiased", got {moment_rounding!r}')
     native().adamw_step(params, grads, exp_avgs, exp_avg_sqs, 0.0 if lr_dev is not None else lr, lr_dev, *betas, eps,
-                        weight_decay, 0 if steps is not None else step, steps, exp_avg_units, exp_avg_root_units)
+                        weight_decay, 0 if steps is not None else step, steps, exp_avg_units, exp_avg_root_units,
+                        moment_rounding == "unbiased")
 
 
 def decode_root(codes: torch.Tensor, units: torch.Tensor) -> torch.Tensor:
@@ -70,7 +80,7 @@ class AdamW(torch.optim.Optimizer):
     """AdamW over ``adamw_step``: torch.optim.AdamW's arguments and update.
 
     moment_bits 32 or 8: how the moments are held (state "exp_avg", "exp_avg_sq", and with 8 also
-    "exp_avg_unit", "exp_avg_root_unit").  capturable=True keeps the step counts on the device, so
+    "exp_avg_unit", "exp_avg_root_unit"); 8-bit ones are rounded without bias.  capturable=True keeps the step counts on the device, so
     that ``step()`` can be captured in a HIP graph (and takes a float32 device tensor as lr); state
     is then created by one eager step before the capture.  State is float32 or codes whatever the
     parameters' type, also after load_state_dict."""
@@ -142,7 +152,7 @@ class AdamW(torch.optim.Optimizer):
                 units = {}
                 if group["moment_bits"] == 8:
                     units = dict(exp_avg_units=[s["exp_avg_unit"] for s in states],
-                                 exp_avg_root_units=[s["exp_avg_root_unit"] for s in states])
+                                 exp_avg_root_units=[s["exp_avg_root_unit"] for s in states], moment_rounding="unbiased")
                 try:
                     adamw_step([p for p, _ in items], [p.grad for p, _ in items], [s["exp_avg"] for s in states],
                                [s["exp_avg_sq"] for s in states], lr=group["lr"], betas=group["betas"], eps=group["eps"],
