@@ -90,6 +90,10 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor or_none(const std::optional<Tensor>& t) { return t ? *t : Tensor(); }
 std::optional<Tensor> given(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 Tensor packed(const Tensor& t) { return t.defined() && !t.is_contiguous() ? t.contiguous() : t; }
+// A tensor with a tangent is refused: calls that need no autograd node would drop it without a word.
+void no_tangent(const Tensor& t, const char* who) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), who, ": no forward-mode derivative");
+}
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 // x as rows of unit stride: a view where it is one matrix of evenly spaced rows, else a copy.
@@ -144,6 +148,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
+    no_tangent(grads[0], "layer_norm");
     const int64_t rows = x.size(0), dim = x.size(1), stride = rows > 1 ? x.stride(0) : dim;
     const int wtype = (int)ctx->saved_data["wtype"].toInt(), xtype = type_of(x, "x");
     Tensor dx, dw, db, ws;
@@ -182,6 +187,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
   TORCH_CHECK_VALUE(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(),
                     "layer_norm: weight and bias must have one type");
   TORCH_CHECK_VALUE(eps >= 0, "layer_norm: eps must not be negative, got ", eps);
+  for (const Tensor* t : {&x, &w, &b}) no_tangent(*t, "layer_norm");
   on_device(x, "layer_norm");
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b))) return LayerNorm::apply(x, given(w), given(b), eps);
   return norm_forward(rows_of(x, x.size(-1)), x, w, b, eps, Tensor());
@@ -221,6 +227,7 @@ struct Gated : torch::autograd::Function<Gated> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &bg = saved[3], &bu = saved[4], &kept = saved[5];
+    no_tangent(grads[0], "gated_linear");
     const int64_t rows = x.size(0), dim = x.size(1), stride = rows > 1 ? x.stride(0) : dim, hidden = wg.size(0);
     const int type = type_of(x, "x");
     Tensor d[5];
@@ -262,6 +269,7 @@ Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, c
   }
   TORCH_CHECK_VALUE(dim <= 1 << 20 && hidden <= 1 << 20 && x.numel() / dim <= 1 << 26,
                     "gated_linear: at most 2^26 rows and 2^20 columns, got ", x.sizes(), ", ", w_gate.sizes());
+  for (const Tensor* t : {&x, &wg, &wu, &bg, &bu}) no_tangent(*t, "gated_linear");
   on_device(x, "gated_linear");
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(wg) || wants_grad(wu) || wants_grad(bg) || wants_grad(bu)))
     return Gated::apply(x, wg, wu, given(bg), given(bu), act);
