@@ -700,8 +700,8 @@ int gsr_layer_norm_bwd(const void* x, const void* dy, int64_t rows, int64_t dim,
                        void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gated block: h = act(g) * u with g = x wg^T + bg, u = x wu^T + bu.  x [rows, dim] (row stride
- * x_stride, any alignment), wg / wu [hidden, dim] and h [rows, hidden] contiguous, bg / bu [hidden]
- * or NULL; all of one type.  act: GSR_ACT_*.  rows <= 2^26, dim and hidden <= 2^20.
+ * x_stride, any alignment), wg / wu [hidden, dim] and h [rows, hidden] contiguous, bg and bu [hidden]
+ * or both NULL; all of one type.  act: GSR_ACT_*.  rows <= 2^26, dim and hidden <= 2^20.
  * bwd: from dh [rows, hidden] (row stride dh_stride) the gradients dx [rows, dim], dwg, dwu
  * [hidden, dim], dbg, dbu [hidden] (each may be NULL), contiguous.  dg and du are rounded to the
  * type before the products that use them, as the projections' outputs' gradients would be, save in

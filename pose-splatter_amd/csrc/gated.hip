@@ -719,6 +719,7 @@ extern "C" int gsr_gated_fwd(const void* x, int64_t rows, int64_t dim, int64_t x
   if (const int e = gated_check("gsr_gated_fwd", s, x_stride, type, act)) return e;
   if (rows == 0) return 0;
   GSR_REQUIRE(x && wg && wu && h, "gsr_gated_fwd: null pointer");
+  GSR_REQUIRE(!bg == !bu, "gsr_gated_fwd: bg and bu go together");
   GSR_REQUIRE(workspace_bytes >= gsr_gated_workspace(rows, dim, hidden, type, 0) && (workspace || workspace_bytes == 0),
               "gsr_gated_fwd: workspace too small (%zu bytes)", workspace_bytes);
   char* ws = (char*)workspace;
@@ -742,6 +743,7 @@ extern "C" int gsr_gated_bwd(const void* x, int64_t rows, int64_t dim, int64_t x
   if (const int e = gated_check("gsr_gated_bwd", s, x_stride, type, act)) return e;
   GSR_REQUIRE(rows <= 1 || dh_stride >= hidden, "gsr_gated_bwd: dh row stride %lld below hidden", (long long)dh_stride);
   GSR_REQUIRE(wg && wu && (rows == 0 || (x && dh)), "gsr_gated_bwd: null pointer");
+  GSR_REQUIRE(!bg == !bu, "gsr_gated_bwd: bg and bu go together");
   GSR_REQUIRE(workspace_bytes >= gsr_gated_workspace(rows, dim, hidden, type, 1) && (workspace || workspace_bytes == 0),
               "gsr_gated_bwd: workspace too small (%zu bytes)", workspace_bytes);
   const auto st = (hipStream_t)stream;
