@@ -722,6 +722,7 @@ extern "C" int gsr_gated_fwd(const void* x, int64_t rows, int64_t dim, int64_t x
   GSR_REQUIRE(!bg == !bu, "gsr_gated_fwd: bg and bu go together");
   GSR_REQUIRE(workspace_bytes >= gsr_gated_workspace(rows, dim, hidden, type, 0) && (workspace || workspace_bytes == 0),
               "gsr_gated_fwd: workspace too small (%zu bytes)", workspace_bytes);
+  GSR_REQUIRE(((uintptr_t)workspace | (uintptr_t)kept) % 256 == 0, "gsr_gated_fwd: workspace and kept must start at 256 bytes");
   char* ws = (char*)workspace;
   const auto st = (hipStream_t)stream;
   if (type == GSR_F32) {
@@ -746,6 +747,7 @@ extern "C" int gsr_gated_bwd(const void* x, int64_t rows, int64_t dim, int64_t x
   GSR_REQUIRE(!bg == !bu, "gsr_gated_bwd: bg and bu go together");
   GSR_REQUIRE(workspace_bytes >= gsr_gated_workspace(rows, dim, hidden, type, 1) && (workspace || workspace_bytes == 0),
               "gsr_gated_bwd: workspace too small (%zu bytes)", workspace_bytes);
+  GSR_REQUIRE(((uintptr_t)workspace | (uintptr_t)kept) % 256 == 0, "gsr_gated_bwd: workspace and kept must start at 256 bytes");
   const auto st = (hipStream_t)stream;
   char* ws = (char*)workspace;
   if (rows == 0) {   // sums over no rows

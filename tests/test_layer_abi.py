@@ -22,3 +22,11 @@ def test_biases_go_together(rows, bg, bu):
     """One bias without the other is refused whatever kernel the sizes take."""
     for code, error in _gated(rows, ctypes.c_void_p(bg), ctypes.c_void_p(bu)):
         assert code == -1 and b"bg and bu" in error
+
+
+@pytest.mark.parametrize("rows", [1, 64, 5000])
+def test_buffers_are_aligned(rows):
+    """workspace and kept start at multiples of 256 bytes, as their parts' offsets assume."""
+    for kw in (dict(ws=256 + 16), dict(kept=256 + 128), dict(ws=255, kept=512)):
+        for code, error in _gated(rows, None, None, hidden=600, dim=300, **kw):
+            assert code == -1 and b"256 bytes" in error
