@@ -531,7 +531,7 @@ static GatedPlan gated_plan(GatedShape s, int type, bool backward) {
     w.r_fwd = gated_wide_rounds(type, w.fwd, ceil_div64(s.rows, w.fwd), ceil_div64(pad, w.fwd / 2), gated_wide_steps(type, s.dim));
   w.cuts = take(w.fwd > 64 && !backward ? w.r_fwd.bytes(w.fwd) : 0);
   w.keep = (w.fwd > 64 || s.rows <= kSkinnyRows) && gated_keeps(type, s.dim);
-  w.keep_pads = pads && w.kdim != s.dim && (w.dx > 64 || w.dw > 64 || !w.keep);
+  w.keep_pads = pads && w.kdim != s.dim && (w.dx > 64 || w.dw > 64 || (w.fwd > 64 && !w.keep));   // (what reads them)
   w.kept_pads = !w.keep ? 0 : type == GSR_F32 ? Kept<float>::bytes(s.rows, s.hidden) : Kept<bf16>::bytes(s.rows, s.hidden);
   w.kept = w.kept_pads + (w.keep_pads ? (s.rows + 2 * s.hidden) * w.kdim * es : 0);
   w.bias_rows = s.rows <= kSkinnyRows ? 1 : w.fwd > 64 ? ceil_div64(s.rows, w.fwd) * 2 : rb;
