@@ -36,3 +36,28 @@ def test_few_short_odd_rows(cuda, rows, dim, hidden, kind):
     want, tol = _reference(*args, dh, act, TYPES[kind])
     for name, got, v, t in zip(NAMES, _run(cuda, args, dh, act), want, tol):
         _check(got, v, t, f"{name} {rows}x{dim}->{hidden} {kind} {act}")
+
+
+# A backward of up to 15 columns: rows' parts of the weights' gradients, columns' parts of dx
+@pytest.mark.parametrize("rows,dim,hidden", [(32768, 15, 65536), (1 << 26, 15, 16), (1 << 20, 15, 1 << 16), (100000, 15, 1 << 20),
+                                             (65, 15, 1 << 20), (1 << 24, 1, 1 << 20), (1, 1, 1 << 20), (16000, 8, 12288)])
+def test_narrow_workspace_is_bounded(rows, dim, hidden):
+    """512 MB for either, or one part of dx, or two of the weights' gradients where those are more."""
+    from gsr import _lib
+    weights, dx = 2 * hidden * (dim + 4) // 4 * 4 * 4, rows * dim * 4
+    got = _lib.lib().gsr_gated_workspace(rows, dim, hidden, _lib.BF16, 1)
+    assert got <= max(512 << 20, 2 * weights) + max(512 << 20, dx) + 512
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_narrow_rows_share_their_parts(cuda, kind):
+    """So wide a hidden layer that workgroups add several tiles of rows to one part, and columns share dx."""
+    rows, dim, hidden = 4210, 15, 65500
+    args, dh = _case(rows, dim, hidden, kind, True, 6)
+    args, dh = [t.to(cuda) for t in args], (dh * 2 ** -5).to(cuda)
+    want, tol = _reference(*args, dh, "silu", TYPES[kind])
+    first = _run(cuda, args, dh, "silu")
+    for name, got, v, t in zip(NAMES, first, want, tol):
+        _check(got, v, t, f"{name} {kind}")
+    assert all(torch.equal(a, b) for a, b in zip(first, _run(cuda, args, dh, "silu")))
