@@ -89,7 +89,9 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 // The optional tensors of a call as tensors that may be undefined.
 Tensor or_none(const std::optional<Tensor>& t) { return t ? *t : Tensor(); }
 std::optional<Tensor> given(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
-Tensor packed(const Tensor& t) { return t.defined() && !t.is_contiguous() ? t.contiguous() : t; }
+// t as it lies in memory: a view that negates what it reads (is_neg) is written out.
+Tensor as_held(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+Tensor packed(const Tensor& t) { return as_held(t.defined() && !t.is_contiguous() ? t.contiguous() : t); }
 // A tensor with a tangent is refused: calls that need no autograd node would drop it without a word.
 void no_tangent(const Tensor& t, const char* who) {
   TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), who, ": no forward-mode derivative");
@@ -105,6 +107,7 @@ struct Rows {
 Rows rows_of(const Tensor& x, int64_t dim) {
   Tensor t = x.dim() == 2 ? x : x.reshape({-1, dim});
   if ((dim > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < dim)) t = t.contiguous();
+  t = as_held(t);
   const int64_t rows = t.size(0);
   return {t, rows, rows > 1 ? t.stride(0) : dim};
 }
@@ -328,6 +331,10 @@ void adamw_step(py::handle param_list, py::handle grad_list, py::handle m_list, 
   TORCH_CHECK_VALUE(lr_dev || lr >= 0, "adamw_step: lr must not be negative, got ", lr);
   TORCH_CHECK_VALUE(!lr_dev || (lr_dev->numel() == 1 && lr_dev->scalar_type() == at::kFloat),
                     "adamw_step: a tensor lr must be one float32 value");
+  const auto held = [](const Tensor& t) {
+    TORCH_CHECK_VALUE(!t.is_neg(), "adamw_step: views that negate what they read are taken as gradients only");
+  };
+  if (lr_dev) held(*lr_dev);
   TORCH_CHECK_VALUE(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "adamw_step: betas must be in [0, 1), got ", beta1, ", ", beta2);
   TORCH_CHECK_VALUE(eps >= 0 && weight_decay >= 0, "adamw_step: eps and weight_decay must not be negative, got ", eps, ", ", weight_decay);
   TORCH_CHECK_VALUE(steps || step >= 1, "adamw_step: step must be at least 1, got ", step);
@@ -363,6 +370,7 @@ void adamw_step(py::handle param_list, py::handle grad_list, py::handle m_list, 
                       p.strides(), ")");
     TORCH_CHECK_VALUE(same_layout(m, p) && same_layout(v, p), "adamw_step: moments must have their parameter's shape and strides ",
                       p.sizes(), ", ", p.strides());
+    for (const Tensor* t : {&p, &m, &v}) held(*t);
     const int64_t n = p.numel();
     if (byte)
       for (const Tensor* u : {&(*m_units)[i], &(*v_units)[i]})
@@ -370,12 +378,13 @@ void adamw_step(py::handle param_list, py::handle grad_list, py::handle m_list, 
                               u->device() == device,
                           "adamw_step: units ", i, " must be contiguous float32 [", units_of(n), "] on ", device, ", got ",
                           u->scalar_type(), " ", u->sizes());
+    if (byte) held((*m_units)[i]), held((*v_units)[i]);
     if (steps)
       TORCH_CHECK_VALUE((*steps)[i].numel() == 1 && (*steps)[i].scalar_type() == at::kLong && (*steps)[i].device() == device,
                         "adamw_step: step ", i, " must be one int64 value on ", device);
     if (n == 0) continue;
     Tensor g = grads[i];
-    if (!same_layout(g, p)) {
+    if (!same_layout(g, p) || g.is_neg()) {
       g = at::empty_strided(p.sizes(), p.strides(), g.options()).copy_(g);
       kept.push_back(g);
     }
@@ -425,6 +434,7 @@ Tensor decode_root(const Tensor& codes, const Tensor& units) {
                         units.is_contiguous() && units.device() == codes.device(),
                     "decode_root: units must be contiguous float32 [", units_of(codes.numel()), "] on ", codes.device(), ", got ",
                     units.scalar_type(), " ", units.sizes(), " on ", units.device());
+  TORCH_CHECK_VALUE(!units.is_neg(), "decode_root: units must not be a view that negates what it reads");
   on_device(codes, "decode_root");
   const c10::OptionalDeviceGuard guard(codes.device());
   Tensor out = at::empty(codes.sizes(), codes.options().dtype(at::kFloat));

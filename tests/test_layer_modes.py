@@ -55,3 +55,54 @@ def test_forward_mode_over_a_backward_is_refused(cuda, layer):
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(y, [t["x"]], dy, retain_graph=True)
     assert torch.equal(plain, torch.autograd.grad(y, [t["x"]], torch.ones_like(y))[0])
+
+
+def _negated(t):
+    """-t as a view that negates when it is read (what autograd makes of an imaginary part's conjugate)."""
+    return torch._neg_view(-t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layer", [_norm, _gated])
+def test_negated_views(cuda, layer):
+    """Views that hold their negative give the values they stand for, as inputs and as the output's gradient."""
+    t = {k: v.requires_grad_(True) for k, v in _inputs(cuda).items()}
+    y = layer(t)
+    dy = torch.randn(y.shape, device=cuda)
+    want = [y, *(g for g in torch.autograd.grad(y, list(t.values()), dy, allow_unused=True) if g is not None)]
+    n = {k: _negated(v.detach()).requires_grad_(True) for k, v in t.items()}
+    assert all(v.is_neg() for v in n.values())
+    y = layer(n)
+    got = [y, *(g for g in torch.autograd.grad(y, list(n.values()), _negated(dy), allow_unused=True) if g is not None)]
+    assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(want, got))
+    with torch.no_grad():
+        assert torch.equal(want[0], layer({k: v.detach() for k, v in n.items()}))
+
+
+@pytest.mark.gpu
+def test_negated_gradient_of_a_step(cuda):
+    from gsr.optim import adamw_step
+    g = torch.randn(300, device=cuda)
+    make = lambda: [torch.ones(300, device=cuda), torch.zeros(300, device=cuda), torch.zeros(300, device=cuda)]  # noqa: E731
+    a, b = make(), make()
+    adamw_step([a[0]], [g], [a[1]], [a[2]], step=1)
+    adamw_step([b[0]], [_negated(g)], [b[1]], [b[2]], step=1)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_negated_views_are_not_written():
+    from gsr.optim import adamw_step, decode_root
+    f = lambda: torch.zeros(4)  # noqa: E731
+    for k in range(3):
+        written = [f(), f(), f()]
+        written[k] = _negated(f())
+        with pytest.raises(ValueError, match="negat"):
+            adamw_step([written[0]], [f()], [written[1]], [written[2]], step=1)
+    e4, u8 = f().to(torch.float8_e4m3fn), f().to(torch.uint8)
+    for units in ((_negated(f()[:1]), f()[:1]), (f()[:1], _negated(f()[:1]))):
+        with pytest.raises(ValueError, match="negat"):
+            adamw_step([f()], [f()], [e4], [u8], step=1, exp_avg_units=[units[0]], exp_avg_root_units=[units[1]])
+    with pytest.raises(ValueError, match="negat"):
+        adamw_step([f()], [f()], [f()], [f()], step=1, lr=_negated(torch.tensor(1e-3)))
+    with pytest.raises(ValueError, match="negat"):
+        decode_root(u8, _negated(f()[:1]))
