@@ -371,26 +371,29 @@ __global__ __launch_bounds__(256) void k_norm_cols(const T* x, const T* dy, int6
 }
 
 // dw, db = the sum of n partial rows: 16 groups of lanes a column, each a fixed share of the
-// rows, then the groups in order.
+// rows, then the groups in order.  Workgroups walk the columns with the grid's stride.
 __global__ __launch_bounds__(1024) void k_norm_join(const float* parts, int n, int64_t dim, void* dw, void* db, int wtype) {
   __shared__ float sum[16][65];
   const int col = threadIdx.x % 64, grp = threadIdx.x / 64;
-  const int64_t c = (int64_t)blockIdx.x * 64 + col;
-  float s = 0.f;
-  if (c < 2 * dim) {
+  for (int64_t c0 = (int64_t)blockIdx.x * 64; c0 < 2 * dim; c0 += (int64_t)gridDim.x * 64) {
+    const int64_t c = c0 + col;
+    float s = 0.f;
+    if (c < 2 * dim) {
 #pragma unroll 8
-    for (int r = grp; r < n; r += 16) s += parts[(int64_t)r * 2 * dim + c];
-  }
-  sum[grp][col] = s;
-  __syncthreads();
-  if (grp == 0 && c < 2 * dim) {
-#pragma unroll
-    for (int k = 1; k < 16; ++k) s += sum[k][col];
-    if (c < dim) {
-      if (dw) store_param(dw, wtype, c, s);
-    } else if (db) {
-      store_param(db, wtype, c - dim, s);
+      for (int r = grp; r < n; r += 16) s += parts[(int64_t)r * 2 * dim + c];
     }
+    sum[grp][col] = s;
+    __syncthreads();
+    if (grp == 0 && c < 2 * dim) {
+#pragma unroll
+      for (int k = 1; k < 16; ++k) s += sum[k][col];
+      if (c < dim) {
+        if (dw) store_param(dw, wtype, c, s);
+      } else if (db) {
+        store_param(db, wtype, c - dim, s);
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -548,7 +551,8 @@ extern "C" int gsr_layer_norm_bwd(const void* x, const void* dy, int64_t rows, i
     GSR_LAUNCH_CHECK("gsr_layer_norm_bwd");
   }
   if (sums) {
-    k_norm_join<<<(unsigned)ceil_div64(2 * dim, 64), 1024, 0, s>>>((const float*)workspace, n, dim, dw, db, wtype);
+    const int64_t blocks = ceil_div64(2 * dim, 64);   // (a launch holds less than 2^32 threads)
+    k_norm_join<<<(unsigned)(blocks < 1 << 20 ? blocks : 1 << 20), 1024, 0, s>>>((const float*)workspace, n, dim, dw, db, wtype);
     GSR_LAUNCH_CHECK("gsr_layer_norm_bwd (join)");
   }
   return 0;
