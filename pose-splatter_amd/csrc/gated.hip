@@ -752,7 +752,9 @@ extern "C" int gsr_gated_bwd(const void* x, int64_t rows, int64_t dim, int64_t x
   char* ws = (char*)workspace;
   if (rows == 0) {   // sums over no rows
     const auto zero = [&](void* p, int64_t n) {
-      if (p) gated_join<bf16>(nullptr, 0, n, n, p, nullptr, st);
+      const int64_t most = 1 << 30;   // (a launch holds less than 2^32 threads, one a value)
+      for (int64_t at = 0; p && at < n; at += most)
+        gated_join<bf16>(nullptr, 0, n - at < most ? n - at : most, most, (bf16*)p + at, nullptr, st);
     };
     const int64_t each = type == GSR_F32 ? 2 : 1;   // zeros of any type, 16 bits at a time
     zero(dwg, hidden * dim * each);

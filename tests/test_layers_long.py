@@ -30,3 +30,16 @@ def test_layer_norm_of_one_long_row(cuda):
     assert float((dx.double() - want).abs().max()) <= 2 * G * float(rstd) * 0.5 * (2 + 2 * X * X)
     assert torch.equal(db, dy[0])
     assert float((dw.double() - (dyd * z)[0]).abs().max()) <= (G + 65 * U) * X
+
+
+@pytest.mark.gpu
+def test_no_rows_of_a_large_block(cuda):
+    """The weights' gradients of no rows are zeros, to the last of 2^31 + 2^15 of them (none of the others are
+    asked for; the inputs are not read)."""
+    from gsr import _lib
+    hidden, dim = (1 << 16) + 1, 1 << 15
+    out = torch.full((hidden, dim), 3.0, device=cuda)
+    x = out.data_ptr()
+    _lib.check(_lib.lib().gsr_gated_bwd(None, 0, dim, dim, _lib.F32, x, x, hidden, None, None, 0, None, hidden, None, None, x, None,
+                                        None, None, None, 0, torch.cuda.current_stream().cuda_stream), "gsr_gated_bwd")
+    assert not bool(out.any())
