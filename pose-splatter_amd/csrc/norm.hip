@@ -160,35 +160,35 @@ __global__ __launch_bounds__(1024) void k_norm_fwd_long(const T* x, int64_t rows
   constexpr int V = NormVec<T>::V;
   __shared__ float lds[2 * 16];
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-  const T* xr = x + row * stride;
-  float s[1] = {0.f};
-  for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
-    float v[V];
-    load_upto(xr + c, dim - c, v);
+    const T* xr = x + row * stride;
+    float s[1] = {0.f};
+    for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
+      float v[V];
+      load_upto(xr + c, dim - c, v);
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[0] += v[i];
-  }
-  row_sum<1024>(s, lds);
-  const float mean = s[0] / (float)dim;
-  s[0] = 0.f;
-  for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
-    float v[V];
-    load_upto(xr + c, dim - c, v, mean);
+      for (int i = 0; i < V; ++i) s[0] += v[i];
+    }
+    row_sum<1024>(s, lds);
+    const float mean = s[0] / (float)dim;
+    s[0] = 0.f;
+    for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
+      float v[V];
+      load_upto(xr + c, dim - c, v, mean);
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[0] += (v[i] - mean) * (v[i] - mean);
-  }
-  row_sum<1024>(s, lds + 16);
-  const float rstd = 1.f / sqrtf(s[0] / (float)dim + eps);
-  if (stats && threadIdx.x == 0) stats[row] = make_float2(mean, rstd);
-  for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
-    float v[V], wv[V], bv[V];
-    load_upto(xr + c, dim - c, v);
-    load_param(w, wtype, c, dim - c, wv, 1.f);
-    load_param(b, wtype, c, dim - c, bv, 0.f);
+      for (int i = 0; i < V; ++i) s[0] += (v[i] - mean) * (v[i] - mean);
+    }
+    row_sum<1024>(s, lds + 16);
+    const float rstd = 1.f / sqrtf(s[0] / (float)dim + eps);
+    if (stats && threadIdx.x == 0) stats[row] = make_float2(mean, rstd);
+    for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
+      float v[V], wv[V], bv[V];
+      load_upto(xr + c, dim - c, v);
+      load_param(w, wtype, c, dim - c, wv, 1.f);
+      load_param(b, wtype, c, dim - c, bv, 0.f);
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = (v[i] - mean) * rstd * wv[i] + bv[i];
-    store_upto(y + row * dim + c, dim - c, v);
-  }
+      for (int i = 0; i < V; ++i) v[i] = (v[i] - mean) * rstd * wv[i] + bv[i];
+      store_upto(y + row * dim + c, dim - c, v);
+    }
   }
 }
 
@@ -203,7 +203,6 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256, LANES > 256 ? 1 : NV <= 
   constexpr int W = LANES / 64;
   constexpr bool HOLD = LANES <= 256;   // weights and the next row in registers (1024 threads have none left)
   __shared__ float lds[LANES > 64 ? 4 * W : 1];
-  const int lane = threadIdx.x % LANES;
   const float inv = 1.f / (float)dim;
   NormCols<V, LANES, EARLY> cols(dim);
   float wv[HOLD ? NV : 1][V], aw[NV][V] = {}, ab[NV][V] = {};
@@ -255,7 +254,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256, LANES > 256 ? 1 : NV <= 
       const float m0 = s[0] * inv, m1 = s[1] * inv;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-          if constexpr (!HOLD) weights(k);
+        if constexpr (!HOLD) weights(k);
         float g[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -325,31 +324,31 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(const T* x, const T* dy,
   __shared__ float lds[2][2 * 16];
   int half = 0;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, half ^= 1) {
-  const float2 st = stats[row];
-  const T *xr = x + row * stride, *gr = dy + row * dy_stride;
-  float s[2] = {0.f, 0.f};
-  for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
-    float v[V], g[V], wv[V];
-    load_upto(xr + c, dim - c, v, st.x);
-    load_upto(gr + c, dim - c, g);
-    load_param(w, wtype, c, dim - c, wv, 1.f);
+    const float2 st = stats[row];
+    const T *xr = x + row * stride, *gr = dy + row * dy_stride;
+    float s[2] = {0.f, 0.f};
+    for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
+      float v[V], g[V], wv[V];
+      load_upto(xr + c, dim - c, v, st.x);
+      load_upto(gr + c, dim - c, g);
+      load_param(w, wtype, c, dim - c, wv, 1.f);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      s[0] += g[i] * wv[i];
-      s[1] += g[i] * wv[i] * ((v[i] - st.x) * st.y);
+      for (int i = 0; i < V; ++i) {
+        s[0] += g[i] * wv[i];
+        s[1] += g[i] * wv[i] * ((v[i] - st.x) * st.y);
+      }
     }
-  }
-  row_sum<1024>(s, lds[half]);
-  const float m0 = s[0] / (float)dim, m1 = s[1] / (float)dim;
-  for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
-    float v[V], g[V], wv[V];
-    load_upto(xr + c, dim - c, v, st.x);
-    load_upto(gr + c, dim - c, g);
-    load_param(w, wtype, c, dim - c, wv, 1.f);
+    row_sum<1024>(s, lds[half]);
+    const float m0 = s[0] / (float)dim, m1 = s[1] / (float)dim;
+    for (int64_t c = (int64_t)threadIdx.x * V; c < dim; c += 1024 * V) {
+      float v[V], g[V], wv[V];
+      load_upto(xr + c, dim - c, v, st.x);
+      load_upto(gr + c, dim - c, g);
+      load_param(w, wtype, c, dim - c, wv, 1.f);
 #pragma unroll
-    for (int i = 0; i < V; ++i) g[i] = (g[i] * wv[i] - m0 - (v[i] - st.x) * st.y * m1) * st.y;
-    store_upto(dx + row * dim + c, dim - c, g);
-  }
+      for (int i = 0; i < V; ++i) g[i] = (g[i] * wv[i] - m0 - (v[i] - st.x) * st.y * m1) * st.y;
+      store_upto(dx + row * dim + c, dim - c, g);
+    }
   }
 }
 
