@@ -106,3 +106,29 @@ def test_negated_views_are_not_written():
         adamw_step([f()], [f()], [f()], [f()], step=1, lr=_negated(torch.tensor(1e-3)))
     with pytest.raises(ValueError, match="negat"):
         decode_root(u8, _negated(f()[:1]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim,hidden", [(300, 9, 40), (300, 264, 520), (60, 2501, 900), (700, 509, 1363), (2600, 72, 1025)])
+def test_saved_tensors_elsewhere(cuda, rows, dim, hidden):
+    """What the forward keeps may be moved before the backward (other addresses, rows packed), and a graph
+    that is kept may be walked twice: the same bits."""
+    from gsr.layers import gated_linear, layer_norm
+    g = torch.Generator(device=cuda).manual_seed(rows)
+    mk = lambda *s: torch.randn(*s, device=cuda, generator=g).to(torch.bfloat16)  # noqa: E731
+    x, w, wg, wu, dh = mk(rows, dim + 5)[:, 3:3 + dim], mk(dim), mk(hidden, dim), mk(hidden, dim), mk(rows, hidden)
+
+    def graph():
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, wg, wu)]
+        return leaves, gated_linear(layer_norm(leaves[0], leaves[1]), *leaves[2:])
+    leaves, h = graph()
+    want = torch.autograd.grad(h, leaves, dh, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(h, leaves, dh)))
+    with torch.autograd.graph.save_on_cpu():
+        leaves, h = graph()
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(h, leaves, dh)))
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, wg, wu)]
+    h = torch.utils.checkpoint.checkpoint(lambda *t: gated_linear(t[0], *t[1:]), leaves[0], *leaves[2:], use_reentrant=False)
+    direct = [t.detach().requires_grad_(True) for t in (x, wg, wu)]
+    for a, b in zip(torch.autograd.grad(h, [leaves[0], *leaves[2:]], dh), torch.autograd.grad(gated_linear(*direct), direct, dh)):
+        assert torch.equal(a, b)
