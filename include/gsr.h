@@ -704,8 +704,9 @@ int gsr_layer_norm_bwd(const void* x, const void* dy, int64_t rows, int64_t dim,
  * or both NULL; all of one type.  act: GSR_ACT_*.  rows <= 2^26, dim and hidden <= 2^20.
  * bwd: from dh [rows, hidden] (row stride dh_stride) the gradients dx [rows, dim], dwg, dwu
  * [hidden, dim], dbg, dbu [hidden] (each may be NULL), contiguous.  dg and du are rounded to the
- * type before the products that use them, as the projections' outputs' gradients would be, save in
- * small cases and for dim <= 15, which multiply them in fp32.
+ * type before the products that use them, as the projections' outputs' gradients would be (in fp16
+ * one above 65504 becomes infinite, one below 2^-25 zero), save in small cases and for dim <= 15,
+ * which multiply them in fp32.
  * kept: device, 256-byte aligned, gsr_gated_kept bytes, or NULL: what the forward leaves for its
  * backward, g and u, and copies of x and the weights where dim is not whole 16-byte pieces.  Without
  * it (where the bytes are 0, or by choice) the backward makes them again.

@@ -314,7 +314,7 @@ static void gated_join(const float* parts, int64_t count, int64_t n, int64_t spl
 
 // The gradients of the projections from what the forward kept: dgu, and parts [blocks of `each` rows][2]
 // [hidden] of the column sums (NULL: not wanted).  Bound by memory: 12 bytes an element in 16 bits, 20 in
-// fp32 (8 columns a lane, 256 a workgroup; 16384 x 5632 bf16 206 us, 5.4 TB/s).
+// fp32 (8 columns a lane, 256 a workgroup; 16384 x 5632 bf16 228 us, 4.9 TB/s).
 template <typename T, typename G>
 __global__ __launch_bounds__(256) void k_gated_slopes(const void* saved, const T* dh, int64_t dh_stride, int act, GatedShape s,
                                                       int each, G* dgu, float* parts) {

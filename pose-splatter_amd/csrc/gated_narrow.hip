@@ -13,8 +13,8 @@
 // through shared memory; the rows' parts of dW (and dx's, of workgroups that share rows) go through
 // memory and are joined in order.
 //
-// Against projections, dx and dW as products of their own (gated.hip), 16000 rows, fp32: 8 -> 128 17 us
-// (38), 8 -> 12288 597 us (2515), 15 -> 2000 126 us (410); bf16 17 (31), 517 (1908), 117 (320); 65 x
+// Against projections, dx and dW as products of their own (gated.hip), 16000 rows, fp32: 8 -> 128 18 us
+// (38), 8 -> 12288 582 us (2515), 15 -> 2000 125 us (410); bf16 18 (31), 504 (1908), 115 (320); 65 x
 // 3 -> 100 13 us (22), 1 x 8 -> 12288 15 us (18).  At 8 -> 12288 it waits for the activation's vector
 // instructions (290 us of fp32), then for the weights' parts (217 us).  Two blocks of 16 columns do
 // not fit the registers: 30 -> 512 would take 144 us against 102.

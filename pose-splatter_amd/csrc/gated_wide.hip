@@ -6,10 +6,12 @@
 //   dx                  K runs through [dg | du], its other operand through Wg, then Wu
 //   dWg, dWu            rows are the columns of [dg | du], K the rows of x
 //
-// 16384 x 2048 -> 5632 bf16: forward 650 us (1160 TFLOP/s, writing its kept projections as well), dx
-// 545 (1390), dW 595 (1270); 16000 x 256 -> 512 fp32 79, and dx and dW side by side 133 us (106 and 126
-// of the card's 153 TFLOP/s in fp32: one or two rounds of tiles, whose first loads and last stores
-// nothing hides).
+// Averages of 60 passes (the quickest in brackets), 16384 x 2048 -> 5632 bf16: forward 682 us (652; 1110
+// TFLOP/s, writing its kept projections as well), dx 581 (559; 1300), dW 603 (572; 1250); 16000 x
+// 256 -> 512 fp32 90 us (85), and dx and dW side by side 149 (140): 93 and 113 of the card's 153
+// TFLOP/s in fp32.  Those are one or two rounds of tiles whose first loads and last stores nothing
+// hides; the epilogue leaves two of the ring's five slots (three of them at 256) to the next tile's
+// first loads, which are not issued there.
 #include "gated_wide.h"
 
 #include "wide.h"

@@ -11,7 +11,7 @@
 // row while they reduce this one.  Each backward workgroup writes one row of partial dw and db,
 // which a second kernel adds in a fixed order: no atomics, the same bits every run.
 // Sums, statistics and partials are fp32; only y, dx, dw and db are rounded to their types.
-// 32768 x 4096 bf16: forward 106 us (5.1 TB/s), backward 160 (5.0 TB/s).
+// 32768 x 4096 bf16: forward 104 us (5.2 TB/s), backward 159 (5.1 TB/s).
 #include <type_traits>
 
 #include "types.h"

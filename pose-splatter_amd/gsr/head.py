@@ -10,8 +10,8 @@ Replaces, in PoseSplatter.forward (src/model.py:134-160):
   per-Gaussian kernel, forward and backward (`gaussian_params_3d`, `pose_transform_3d`).
 
 The MLP is any callable on the selected features: the reference's torch nn.Sequential (two
-small GEMMs on hipBLASLt) or `GatedHead` (layer norm and gated block of gsr.layers, then one
-output projection), which trains with gsr.optim.AdamW.  No CPU path: the functions raise on CPU
+small GEMMs on hipBLASLt) or `GatedHead` (layer norm and gated block of gsr.layers, then a
+torch.nn.Linear for the output projection), which trains with gsr.optim.AdamW.  No CPU path: the functions raise on CPU
 tensors.
 """
 from __future__ import annotations
@@ -162,7 +162,7 @@ def pose_transform_3d(params: torch.Tensor, angle: float, p_3d) -> torch.Tensor:
 class GatedHead(torch.nn.Module):
     """A parameter network for ``params_from_volume_3d`` (the place of the reference's
     gaussian_param_net, src/model.py:207-208): layer norm over the voxel's channels, a gated
-    hidden layer, and the projection to the ``out`` network outputs of a Gaussian.
+    hidden layer, and the projection (torch.nn.Linear) to the ``out`` network outputs of a Gaussian.
 
         head = GatedHead(channels, hidden=128).to("cuda")
         params = params_from_volume_3d(volume, head, grid, scale, angle=a, p_3d=p)"""

@@ -1,10 +1,11 @@
 """Layers of a trainable Gaussian parameter head on libgsr: layer norm and the gated block.
 
 The reference's head is a torch nn.Sequential on [N, channels] voxel features
-(src/model.py:207-232); these are the layers of a head that stays on libgsr's kernels from the
-features to the renderer rows, forward and backward (``gsr.head.GatedHead``).  fp32, bf16 and
-fp16 tensors; arithmetic, sums and statistics are fp32, and gradients are bitwise deterministic.
-No CPU path: the functions raise on CPU tensors.
+(src/model.py:207-232); these are the hidden layers of a head on libgsr's kernels, forward and
+backward (``gsr.head.GatedHead``; its output projection is a torch.nn.Linear, a library product).
+fp32, bf16 and fp16 tensors; arithmetic, sums and statistics are fp32, and gradients are bitwise
+deterministic.  Forward-mode derivatives are refused.  No CPU path: the functions raise on CPU
+tensors.
 """
 from __future__ import annotations
 
@@ -54,8 +55,10 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     biases [hidden] or both None, all of one type; activation "silu", "gelu" (the error
     function's form), "relu" or "sigmoid".  Sums are fp32; in bf16 and fp16 the backward rounds
     the projections' gradients to the type before the products that use them, as separate
-    layers would (in small cases and up to 15 columns they stay fp32).  Differentiable (once)
-    w.r.t. every tensor.  For its backward a forward keeps x and the weights, from dim 256 on (128
+    layers would (in small cases and up to 15 columns they stay fp32): a gradient's root mean square
+    error is up to 1.4 times that of products of unrounded ones, and in fp16 a projection's gradient
+    above 65504 is infinite and one below 2^-25 is zero, so a loss is scaled for them as for any fp16
+    layer's.  Differentiable (once) w.r.t. every tensor.  For its backward a forward keeps x and the weights, from dim 256 on (128
     in fp32, where a case is not small) both projections, 6 bytes an element of [rows, hidden] (8
     in fp32), and where dim is not a multiple of 8 (4) a copy of x and the weights that is; below
     that the backward computes the projections again."""
