@@ -118,8 +118,8 @@ class AdamW(torch.optim.Optimizer):
         else:
             s["exp_avg"] = torch.empty_strided(**like, dtype=torch.uint8).zero_().view(torch.float8_e4m3fn)
             s["exp_avg_sq"] = torch.empty_strided(**like, dtype=torch.uint8).zero_()
-            s["exp_avg_unit"] = torch.zeros(_units(p.numel()), device=p.device)
-            s["exp_avg_root_unit"] = torch.zeros(_units(p.numel()), device=p.device)
+            s["exp_avg_unit"] = torch.zeros(_units(p.numel()), device=p.device, dtype=torch.float32)
+            s["exp_avg_root_unit"] = torch.zeros(_units(p.numel()), device=p.device, dtype=torch.float32)
         s["step"] = torch.zeros((), dtype=torch.int64, device=p.device) if group["capturable"] else 0
         return s
 

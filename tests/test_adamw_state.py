@@ -227,3 +227,27 @@ def test_refused_step_is_not_counted(cuda):
         opt.step()
     after = [p.detach(), *opt.state[p].values()]
     assert int(opt.state[p]["step"]) == 1 and all(torch.equal(a, b) for a, b in zip(before, after))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("default", [torch.float64, torch.bfloat16])
+def test_state_of_another_default_type(cuda, bits, default):
+    """The state's types do not follow torch's default type; parameters of no and of one element among them."""
+    from gsr.optim import AdamW
+    ps = [torch.nn.Parameter(torch.ones(s, device=cuda)) for s in ((300,), (0, 3), ())]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    before = torch.get_default_dtype()
+    try:
+        torch.set_default_dtype(default)
+        opt = AdamW(ps, moment_bits=bits)
+        opt.step()
+        opt.step()
+    finally:
+        torch.set_default_dtype(before)
+    assert all(s["exp_avg_unit"].dtype == torch.float32 for s in opt.state.values() if "exp_avg_unit" in s)
+    want = 1.0   # (equal gradients: each step is lr, and the decay)
+    for _ in range(2):
+        want = want * (1 - 1e-3 * 1e-2) - 1e-3
+    assert float((ps[0].detach() - want).abs().max()) <= 1e-6 and abs(float(ps[2]) - want) <= 1e-6
